@@ -19,8 +19,11 @@ LIB_PATH = os.path.join(PKG_DIR, "libmbtenv.so")
 # mbt_env.hip: the C ABI, the helper kernels and the run-time compiler; kernels_*.hip: the step / rollout kernel instantiations,
 # one family per translation unit (csrc/kernel_table.hpp) - compiled in parallel, each object cached under build/ by the
 # content of what it was compiled from.
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32.  hipcc forms them from ordinary float code by itself, and some of their forms have given wrong
+# results now and then on this hardware; the scalar forms are the same IEEE operations (same bits).  The host pass does not know the feature
+# and says so in a warning, which is harmless.
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC", "-Wall", "-Wno-unused-function",
-               "-mllvm", "-amdgpu-mfma-vgpr-form"]
+               "-mllvm", "-amdgpu-mfma-vgpr-form", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # (experiments: MBT_EXTRA_HIPCC_FLAGS="-DMBT_SPEED_PRECISE_GROUPS=2 ..." compiles a variant; the object cache is keyed by the flags)
 HIPCC_FLAGS += os.environ.get("MBT_EXTRA_HIPCC_FLAGS", "").split()
 LINK_FLAGS = ["-shared", "-fPIC", "-ldl", "-Wl,-rpath,/opt/rocm/lib"]

@@ -1331,8 +1331,9 @@ int jit_compile(const std::string& source, std::vector<char>& code) {
   if (api.create(&prog, source.c_str(), "mbt_user_plugins.hip", 2, headers, header_names) != 0) return fail(MBT_ERR_HIP, "hiprtcCreateProgram failed");
   // the flags of the ahead-of-time build (mbt_gym_amd/build.py): in particular -ffp-contract=off, which keeps the step and
   // the rollout instantiation bit-identical
-  const char* options[] = {"--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-Wno-unused-function"};
-  const int rc = api.compile(prog, 5, options);
+  const char* options[] = {"--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-Wno-unused-function",
+                           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"};
+  const int rc = api.compile(prog, static_cast<int>(sizeof options / sizeof options[0]), options);
   size_t log_bytes = 0;
   if (api.log_size(prog, &log_bytes) == 0 && log_bytes > 1) {
     g_jit_log.resize(log_bytes);

@@ -129,10 +129,9 @@ __device__ __forceinline__ float activate(float x) {
   return 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
 }
 
-// The same tanh on two values: what is not a transcendental runs on the packed fp32 forms (v_pk_mul_f32, v_pk_add_f32,
-// v_pk_fma_f32: two values per issue slot).  Every operation is the IEEE operation of `activate` - 2r is exact, so
-// fma(r, -2, 1) rounds once exactly like 1 - 2r - hence the SAME bits; per value 2 plain + 2 transcendental issue slots
-// instead of 3.5 + 2 (the compiler packs only the tail of the scalar form: a literal cannot be a packed operand).
+// The same tanh on two values, three plain operations and two transcendentals each.  Every operation is the IEEE operation of
+// `activate` - 2r is exact, so fma(r, -2, 1) rounds once exactly like 1 - 2r - hence the SAME bits.  (The build forbids the packed
+// fp32 instructions, mbt_gym_amd/build.py: the pair is two scalar chains.)
 typedef float float2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float2_t tanh_pair(float2_t x) {
   const float2_t two_log2e = {2.8853900817779268f, 2.8853900817779268f};
