@@ -8,6 +8,7 @@
  *   TE   gym/TradingEnvironment.py      MD   gym/ModelDynamics.py     RW  rewards/RewardFunctions.py
  *   MID  stochastic_processes/midprice_models.py    ARR  stochastic_processes/arrival_models.py
  *   FILL stochastic_processes/fill_probability_models.py   SP  stochastic_processes/StochasticProcessModel.py
+ *   PG   agents/PolicyGradientAgent.py
  *
  * Conventions
  *   - plain C types only; no exceptions cross the boundary; every call returns 0 or a negative
@@ -679,6 +680,56 @@ int mbt_philox4x32_10_host(int device, const uint32_t ctr[4], const uint32_t key
  * on the environment's stream, so mbt_env_timer_* bracket it like a rollout.  For bench.py: floor and rollout timed in one process against
  * the same buffers (16-byte observation rows only).  Touches nothing of the environment. */
 int mbt_env_record_floor_device(mbt_env* env, uint32_t steps, float* obs_traj, float* act_traj, float* rew_traj);
+
+/* ---- what a learner runs between two rollouts ----------------------------------------------------------------------
+ * Operators on DEVICE arrays of the caller (a torch tensor's data_ptr); no environment is needed.  Every call only enqueues on `stream`
+ * (NULL = the default stream) of `device` - whichever device is current - and returns; nothing is allocated, nothing synchronises, and the
+ * calls may be captured into a HIP graph.  Workspaces are the caller's, sized by the query beside the operator, and belong to ONE call until
+ * that call's work has run: calls on different streams, and graphs that may replay at the same time, each bring their own.  Outputs may not
+ * overlap inputs unless a call says so.  Sums, states and carries are held in float32 or wider whatever the element type. */
+enum { MBT_FLOAT32 = 0, MBT_BFLOAT16 = 1, MBT_FLOAT16 = 2 };
+
+/* The gated linear recurrence h_t = keep_t h_{t-1} + b_t along the middle axis of (outer, steps, inner) arrays:
+ *   MBT_GATE_CONSTANT  keep = constant,    b = x        rewards-to-go (PG:69-73) are this one, reversed
+ *   MBT_GATE_VALUE     keep = gate,        b = x
+ *   MBT_GATE_LOGIT     keep = f,           b = (1 - f) x,   f = sigmoid(gate)
+ * A non-zero byte of `reset` at t makes keep_t zero; a keep of exactly zero drops the state it would multiply whatever that holds, infinities
+ * and NaN too.  `reverse` walks from the last step to the first (h_{t-1} is then the state at t + 1, the initial state enters at the last
+ * step).  Products of gates over the time axis have to stay inside float32's range: gates within [-1, 1], or few steps. */
+enum { MBT_GATE_CONSTANT = 0, MBT_GATE_VALUE = 1, MBT_GATE_LOGIT = 2 };
+typedef struct mbt_array3 {
+  void* data;          /* NULL = absent, where that is allowed */
+  int64_t stride[3];   /* in elements, along (outer, time, inner); inputs may repeat elements (stride 0), outputs may not */
+} mbt_array3;
+typedef struct mbt_recurrence {
+  uint64_t outer, steps, inner;  /* all at least 1 */
+  int32_t dtype;                 /* of inputs, gate, states and their gradients */
+  int32_t form;                  /* MBT_GATE_* */
+  int32_t reverse;
+  int32_t reserved;
+  double constant;               /* MBT_GATE_CONSTANT */
+  mbt_array3 inputs;             /* forward, and backward unless the gate is a constant */
+  mbt_array3 gate;               /* unless the gate is a constant */
+  mbt_array3 reset;              /* bytes, or absent */
+  mbt_array3 states;             /* forward: output; backward: that output, unless the gate is a constant */
+  const float* initial;          /* (outer, inner) contiguous, or NULL = zeros */
+  float* final_state;            /* forward output, (outer, inner) contiguous: the last state in walking order, unrounded; or NULL */
+  mbt_array3 grad_states;        /* backward input */
+  const float* grad_final;       /* backward input, (outer, inner), or NULL = zeros */
+  mbt_array3 grad_inputs;        /* backward outputs, each may be absent */
+  mbt_array3 grad_gate;
+  float* grad_initial;           /* backward output, (outer, inner), or NULL */
+  void* workspace;
+  uint64_t workspace_bytes;      /* at least what mbt_recurrence_workspace says */
+} mbt_recurrence;
+/* Bytes of workspace for these sizes, strides and direction (0 is common); the same struct is then passed to the call. */
+uint64_t mbt_recurrence_workspace(const mbt_recurrence* r, int backward);
+int mbt_recurrence_forward(int device, const mbt_recurrence* r, void* stream);
+int mbt_recurrence_backward(int device, const mbt_recurrence* r, void* stream);
+/* ONE step of n = rows x columns contiguous elements: new_state = keep state + b in float32, out = new_state in the element type.
+ * reset (or NULL): a byte at row * reset_row_stride + column * reset_column_stride.  new_state may be `state` itself. */
+int mbt_recurrence_step(int device, int dtype, int form, uint64_t rows, uint64_t columns, const float* state, const void* inputs, const void* gate,
+                        const uint8_t* reset, int64_t reset_row_stride, int64_t reset_column_stride, void* out, float* new_state, void* stream);
 
 /* ---- timing on the environment's stream (HIP events) ------------------------------------------- */
 int mbt_env_timer_begin(mbt_env* env);

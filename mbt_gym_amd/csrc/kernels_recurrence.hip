@@ -1,0 +1,230 @@
+// The C entry points of the gated linear recurrence: argument checks, the choice of layout and split, launches (kernels: recurrence.hpp).
+#include "recurrence.hpp"
+
+namespace mbt_learning {
+template <typename E>
+int launch_recurrence_step(const float* state, const void* x, const void* g, const uint8_t* reset, int64_t reset_columns, int64_t rs, int64_t rc, void* out,
+                           float* new_state, int64_t n, int form, hipStream_t stream);
+
+namespace {
+
+struct Plan {
+  RecurrenceParams params;
+  int which;            // kColumnsScalar / kColumnsVector / kRows + mode
+  unsigned threads;
+  int64_t blocks;
+  size_t lds;
+  uint64_t workspace;
+};
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int log2_ceil(int64_t n) {
+  int l = 0;
+  while ((int64_t{1} << l) < n) ++l;
+  return l;
+}
+
+Axis walk(const mbt_array3& a, int64_t steps, bool down, size_t size, bool swap) {
+  Axis t = {a.data, a.stride[0], a.stride[1], a.stride[2]};
+  if (swap) {
+    t.so = a.stride[2];
+    t.si = a.stride[0];
+  }
+  if (a.data != nullptr && down) t.p = static_cast<char*>(a.data) + (steps - 1) * t.st * static_cast<int64_t>(size);
+  if (down) t.st = -t.st;
+  return t;
+}
+
+// The layout and split of one call; touches no device.
+int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
+  if (r == nullptr) return mbt_set_error(MBT_ERR_INVALID, "null argument");
+  if (!dtype_known(r->dtype)) return mbt_set_error(MBT_ERR_INVALID, "dtype %d: float32, bfloat16 and float16 are known", r->dtype);
+  if (r->form < kGateConstant || r->form > kGateLogit) return mbt_set_error(MBT_ERR_INVALID, "form %d is none of MBT_GATE_*", r->form);
+  const uint64_t limit = uint64_t{1} << 40;
+  if (r->outer < 1 || r->steps < 1 || r->inner < 1) return mbt_set_error(MBT_ERR_INVALID, "outer, steps and inner have to be at least 1");
+  if (r->outer > limit || r->steps > limit || r->inner > limit || r->outer > limit / r->inner)
+    return mbt_set_error(MBT_ERR_INVALID, "sizes beyond 2^40");
+  const bool gated = r->form != kGateConstant;
+  if (gated && r->gate.data == nullptr) return mbt_set_error(MBT_ERR_INVALID, "this form needs a gate array");
+  if ((!backward || gated) && (r->inputs.data == nullptr || r->states.data == nullptr)) return mbt_set_error(MBT_ERR_INVALID, "inputs and states are needed");
+  if (backward && r->grad_states.data == nullptr) return mbt_set_error(MBT_ERR_INVALID, "the backward pass needs grad_states");
+  if (!gated && r->grad_gate.data != nullptr) return mbt_set_error(MBT_ERR_INVALID, "a constant gate has no gradient array");
+  if (!gated && !(r->constant - r->constant == 0.0)) return mbt_set_error(MBT_ERR_INVALID, "the constant gate is not finite");
+
+  const int64_t steps = static_cast<int64_t>(r->steps);
+  const size_t size = dtype_size(r->dtype);
+  const int vector = 16 / static_cast<int>(size);
+  const mbt_array3* main[6] = {};
+  int count = 0;
+  auto add = [&](const mbt_array3& a, bool used) {
+    if (used && a.data != nullptr) main[count++] = &a;
+  };
+  add(r->inputs, !backward || gated);
+  add(r->gate, gated);
+  add(r->states, !backward || gated);
+  add(r->grad_states, backward);
+  add(r->grad_inputs, backward);
+  add(r->grad_gate, backward && gated);
+  bool time_contiguous = true, inner_contiguous = true, outer_contiguous = true;
+  for (int k = 0; k < count; ++k) {
+    time_contiguous = time_contiguous && (main[k]->stride[1] == 1);
+    inner_contiguous = inner_contiguous && (r->inner == 1 || main[k]->stride[2] == 1);
+    outer_contiguous = outer_contiguous && (r->outer == 1 || main[k]->stride[0] == 1);
+  }
+  // lanes lie along the batch axis that is contiguous; (N, 1, T) views of a time-major recording have it in front
+  const bool swap = (r->inner == 1 && r->outer > 1) || (!inner_contiguous && outer_contiguous);
+  if (swap) inner_contiguous = outer_contiguous;
+  const bool down = (r->reverse != 0) != backward;
+
+  RecurrenceParams& P = plan.params;
+  P = RecurrenceParams{};
+  P.x = walk(r->inputs, steps, down, size, swap);
+  P.g = walk(r->gate, steps, down, size, swap);
+  P.reset = walk(r->reset, steps, down, 1, swap);
+  P.h = walk(r->states, steps, down, size, swap);
+  P.dh = walk(r->grad_states, steps, down, size, swap);
+  P.dx = walk(r->grad_inputs, steps, down, size, swap);
+  P.dg = walk(r->grad_gate, steps, down, size, swap);
+  P.initial = r->initial;
+  P.final_state = backward ? nullptr : r->final_state;
+  P.dfinal = r->grad_final;
+  P.dinitial = r->grad_initial;
+  P.steps = steps;
+  P.outer = static_cast<int64_t>(swap ? r->inner : r->outer);
+  P.inner = static_cast<int64_t>(swap ? r->outer : r->inner);
+  P.batch_initial_swapped = swap ? 1 : 0;
+  P.constant = static_cast<float>(r->constant);
+  P.segments = 1;
+  P.segment = steps;
+  plan.lds = 0;
+  plan.workspace = 0;
+  const int64_t batch = P.outer * P.inner;
+  const int64_t chip = 256 * 1024;  // threads that fill it at 16 waves per compute unit
+
+  if (time_contiguous && steps > 1 && !(inner_contiguous && P.inner >= 64)) {
+    // rows: as many lanes as the steps of a row need; a long row is cut into segments, one wave each, while the chip has room for them
+    const int lanes = log2_ceil(ceil_div(steps, vector));
+    P.lanes_log2 = lanes < 6 ? lanes : 6;
+    const int64_t tile = (int64_t{1} << P.lanes_log2) * vector;
+    if (P.lanes_log2 == 6 && steps >= 8 * tile) {
+      int64_t want = chip / 64 / 2 / batch;                  // (8 waves per compute unit)
+      const int64_t most = steps / (4 * tile);              // a segment shorter than four tiles costs more in composites than it gains
+      want = want < most ? want : most;
+      if (want > 1) {
+        P.segment = ceil_div(ceil_div(steps, want), tile) * tile;
+        P.segments = static_cast<int32_t>(ceil_div(steps, P.segment));
+      }
+    }
+    plan.which = kRows + kJoined;
+    plan.threads = 256;
+    plan.blocks = ceil_div(batch * P.segments, 256 >> P.lanes_log2);
+    if (P.segments > 1) plan.workspace = static_cast<uint64_t>(batch) * P.segments * sizeof(float2);
+    return MBT_OK;
+  }
+
+  const bool wide = inner_contiguous && P.inner >= vector;
+  const int v = wide ? vector : 1;
+  const int base = wide ? kColumnsVector : kColumnsScalar;
+  P.vectors_per_outer = ceil_div(P.inner, v);
+  P.vectors = P.outer * P.vectors_per_outer;
+  const int chunk = v == 1 ? 16 : 16 / v;  // (recurrence_launch.hpp: kChunk<V, kJoined>)
+  int64_t parallel = ceil_div(chip, P.vectors);
+  if (parallel > ceil_div(steps, chunk)) parallel = ceil_div(steps, chunk);
+  if (parallel <= 2) {
+    plan.which = base + kAlone;
+    plan.threads = 256;
+    plan.blocks = ceil_div(P.vectors, 256);
+    return MBT_OK;
+  }
+  // columns of a workgroup: at most what LDS holds, at least a 128-byte line's worth, fewer when that buys chunks of time
+  int columns_log2 = v == 1 ? 6 : log2_ceil(256 / v);
+  if (columns_log2 > 6) columns_log2 = 6;
+  const int least = log2_ceil(128 / (v * static_cast<int>(size)));
+  while (columns_log2 > least && (1024 >> columns_log2) < parallel) --columns_log2;
+  while (columns_log2 > 0 && (int64_t{1} << (columns_log2 - 1)) >= P.vectors) --columns_log2;
+  int chunks_log2 = log2_ceil(parallel);
+  if (chunks_log2 > 10 - columns_log2) chunks_log2 = 10 - columns_log2;
+  if (chunks_log2 + columns_log2 < 6) chunks_log2 = 6 - columns_log2;
+  const int64_t chunks = int64_t{1} << chunks_log2, columns = int64_t{1} << columns_log2;
+  P.lanes_log2 = columns_log2;
+  P.column_blocks = ceil_div(P.vectors, columns);
+  // segments: only where one workgroup per column group leaves most of the chip idle AND the walk is long
+  const int64_t tile = chunks * chunk;
+  if (P.column_blocks < 128 && steps >= 4 * tile) {
+    int64_t want = 256 / P.column_blocks;
+    const int64_t most = steps / tile;
+    want = want < most ? want : most;
+    if (want > 1) {
+      P.segment = ceil_div(ceil_div(steps, want), tile) * tile;
+      P.segments = static_cast<int32_t>(ceil_div(steps, P.segment));
+    }
+  }
+  plan.which = base + kJoined;
+  plan.threads = static_cast<unsigned>(chunks * columns);
+  plan.blocks = P.column_blocks * P.segments;
+  plan.lds = static_cast<size_t>(plan.threads / 64) * v * columns * sizeof(float2);
+  if (P.segments > 1) plan.workspace = static_cast<uint64_t>(P.vectors) * v * P.segments * sizeof(float2);
+  return MBT_OK;
+}
+
+int run(int device, const mbt_recurrence* r, bool backward, void* stream) {
+  Plan plan;
+  int rc = make_plan(r, backward, plan);
+  if (rc != MBT_OK) return rc;
+  if (plan.blocks > 0x7fffffff) return mbt_set_error(MBT_ERR_INVALID, "%llu x %llu sequences are more than one launch can walk", (unsigned long long)r->outer, (unsigned long long)r->inner);
+  if (plan.workspace > 0 && (r->workspace == nullptr || r->workspace_bytes < plan.workspace))
+    return mbt_set_error(MBT_ERR_INVALID, "the workspace has %llu bytes; %llu are needed (mbt_recurrence_workspace)",
+                         (unsigned long long)(r->workspace == nullptr ? 0 : r->workspace_bytes), (unsigned long long)plan.workspace);
+  if (reinterpret_cast<uintptr_t>(r->workspace) % sizeof(float2) != 0) return mbt_set_error(MBT_ERR_INVALID, "the workspace is not aligned to 8 bytes");
+  DeviceScope scope;
+  rc = scope.enter(device);
+  if (rc != MBT_OK) return rc;
+  plan.params.composites = static_cast<float2*>(r->workspace);
+  auto launch = [&](int which) {
+    const unsigned blocks = static_cast<unsigned>(plan.blocks);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (r->dtype == MBT_FLOAT32) return launch_recurrence<float>(plan.params, r->form, backward, which, blocks, plan.threads, plan.lds, s);
+    if (r->dtype == MBT_BFLOAT16) return launch_recurrence<bfloat16>(plan.params, r->form, backward, which, blocks, plan.threads, plan.lds, s);
+    return launch_recurrence<float16>(plan.params, r->form, backward, which, blocks, plan.threads, plan.lds, s);
+  };
+  if (plan.params.segments > 1) {
+    rc = launch(plan.which - kJoined + kComposites);
+    if (rc != MBT_OK) return rc;
+  }
+  return launch(plan.which);
+}
+
+}  // namespace
+}  // namespace mbt_learning
+
+extern "C" {
+
+uint64_t mbt_recurrence_workspace(const mbt_recurrence* r, int backward) {
+  mbt_learning::Plan plan;
+  return mbt_learning::make_plan(r, backward != 0, plan) == MBT_OK ? plan.workspace : 0;
+}
+
+int mbt_recurrence_forward(int device, const mbt_recurrence* r, void* stream) { return mbt_learning::run(device, r, false, stream); }
+
+int mbt_recurrence_backward(int device, const mbt_recurrence* r, void* stream) { return mbt_learning::run(device, r, true, stream); }
+
+int mbt_recurrence_step(int device, int dtype, int form, uint64_t rows, uint64_t columns, const float* state, const void* inputs, const void* gate,
+                        const uint8_t* reset, int64_t reset_row_stride, int64_t reset_column_stride, void* out, float* new_state, void* stream) {
+  using namespace mbt_learning;
+  if (!dtype_known(dtype)) return mbt_set_error(MBT_ERR_INVALID, "dtype %d: float32, bfloat16 and float16 are known", dtype);
+  if (form != kGateValue && form != kGateLogit) return mbt_set_error(MBT_ERR_INVALID, "a single step takes MBT_GATE_VALUE or MBT_GATE_LOGIT");
+  if (state == nullptr || inputs == nullptr || gate == nullptr || out == nullptr || new_state == nullptr) return mbt_set_error(MBT_ERR_INVALID, "null argument");
+  if (rows < 1 || columns < 1 || rows > (uint64_t{1} << 38) / columns) return mbt_set_error(MBT_ERR_INVALID, "rows x columns has to be within 1 .. 2^38");
+  DeviceScope scope;
+  int rc = scope.enter(device);
+  if (rc != MBT_OK) return rc;
+  const int64_t n = static_cast<int64_t>(rows * columns), width = static_cast<int64_t>(columns);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == MBT_FLOAT32)
+    return launch_recurrence_step<float>(state, inputs, gate, reset, width, reset_row_stride, reset_column_stride, out, new_state, n, form, s);
+  if (dtype == MBT_BFLOAT16)
+    return launch_recurrence_step<bfloat16>(state, inputs, gate, reset, width, reset_row_stride, reset_column_stride, out, new_state, n, form, s);
+  return launch_recurrence_step<float16>(state, inputs, gate, reset, width, reset_row_stride, reset_column_stride, out, new_state, n, form, s);
+}
+
+}  // extern "C"

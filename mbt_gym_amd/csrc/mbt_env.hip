@@ -27,6 +27,7 @@
 
 #include "../../include/mbt_env.h"
 #include "kernel_table.hpp"
+#include "learning_common.hpp"
 
 namespace {
 
@@ -60,6 +61,28 @@ int check_device(int device) {
     return fail(MBT_ERR_NO_DEVICE, "device %d is %s; libmbtenv is built for gfx950 only", device, prop.gcnArchName);
   return MBT_OK;
 }
+
+}  // namespace
+
+// The same two for the learner's operators (learning_common.hpp).  The check is made once per device and process: a call of a few microseconds
+// cannot afford hipGetDeviceProperties.
+int mbt_set_error(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  return fail(code, "%s", buf);
+}
+int mbt_device_check(int device) {
+  static std::atomic<uint64_t> known{0};
+  if (device >= 0 && device < 64 && (known.load(std::memory_order_relaxed) >> device & 1)) return MBT_OK;
+  const int rc = check_device(device);
+  if (rc == MBT_OK && device < 64) known.fetch_or(1ull << device, std::memory_order_relaxed);
+  return rc;
+}
+
+namespace {
 
 // smallest float32 >= x: for float32 u, (u < x in double) <=> (u < round_up_f32(x))
 float round_up_f32(double x) {

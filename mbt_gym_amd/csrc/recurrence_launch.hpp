@@ -1,0 +1,61 @@
+// Which instantiation of recurrence.hpp a launch runs; included by one translation unit per element type.
+#pragma once
+#include "recurrence.hpp"
+
+namespace mbt_learning {
+
+template <typename E>
+constexpr int kVector = 16 / static_cast<int>(sizeof(E));  // columns (or steps) of one 16-byte access
+
+// Rows of a chunk held in registers.  A thread of a 1024-thread workgroup has 128 registers: 16 elements of each of the four or five arrays it
+// keeps fit; a thread that walks alone (256-thread workgroups) takes twice as many, which is what keeps enough bytes in flight.
+template <int V, int MODE>
+constexpr int kChunk = V == 1 ? 16 : (MODE == kAlone ? 32 : 16) / V;
+
+template <typename E, int FORM, int V, bool BACKWARD>
+void (*columns_kernel(int mode))(RecurrenceParams) {
+  if (mode == kAlone) return recurrence_columns<E, FORM, V, kChunk<V, kAlone>, BACKWARD, kAlone>;
+  if (mode == kJoined) return recurrence_columns<E, FORM, V, kChunk<V, kJoined>, BACKWARD, kJoined>;
+  return recurrence_columns<E, FORM, V, kChunk<V, kJoined>, BACKWARD, kComposites>;
+}
+
+template <typename E, int FORM, bool BACKWARD>
+void (*pick_recurrence(int which))(RecurrenceParams) {
+  if (which >= kRows) {
+    if (which - kRows == kComposites) return recurrence_rows<E, FORM, kVector<E>, BACKWARD, true>;
+    return recurrence_rows<E, FORM, kVector<E>, BACKWARD, false>;
+  }
+  if (which >= kColumnsVector) return columns_kernel<E, FORM, kVector<E>, BACKWARD>(which - kColumnsVector);
+  return columns_kernel<E, FORM, 1, BACKWARD>(which - kColumnsScalar);
+}
+
+template <typename E>
+int launch_recurrence(const RecurrenceParams& P, int form, bool backward, int which, unsigned blocks, unsigned threads, size_t lds, hipStream_t stream) {
+  void (*kernel)(RecurrenceParams) = nullptr;
+  if (form == kGateConstant) kernel = backward ? pick_recurrence<E, kGateConstant, true>(which) : pick_recurrence<E, kGateConstant, false>(which);
+  if (form == kGateValue) kernel = backward ? pick_recurrence<E, kGateValue, true>(which) : pick_recurrence<E, kGateValue, false>(which);
+  if (form == kGateLogit) kernel = backward ? pick_recurrence<E, kGateLogit, true>(which) : pick_recurrence<E, kGateLogit, false>(which);
+  kernel<<<blocks, threads, lds, stream>>>(P);
+  return launch_status("recurrence");
+}
+
+template <typename E>
+int launch_recurrence_step(const float* state, const void* x, const void* g, const uint8_t* reset, int64_t reset_columns, int64_t rs, int64_t rc, void* out,
+                           float* new_state, int64_t n, int form, hipStream_t stream) {
+  // two steps' worth of elements per thread only where the chip is full anyway: below that, more and smaller waves finish sooner
+  const bool wide = n >= (1 << 20);
+  const int v = wide ? kVector<E> : 1;
+  const unsigned blocks = static_cast<unsigned>((n + 256 * static_cast<int64_t>(v) - 1) / (256 * static_cast<int64_t>(v)));
+  const E *xe = static_cast<const E*>(x), *ge = static_cast<const E*>(g);
+  E* oe = static_cast<E*>(out);
+  if (form == kGateValue) {
+    if (wide) recurrence_step<E, kGateValue, kVector<E>><<<blocks, 256, 0, stream>>>(state, xe, ge, reset, reset_columns, rs, rc, oe, new_state, n);
+    else recurrence_step<E, kGateValue, 1><<<blocks, 256, 0, stream>>>(state, xe, ge, reset, reset_columns, rs, rc, oe, new_state, n);
+  } else {
+    if (wide) recurrence_step<E, kGateLogit, kVector<E>><<<blocks, 256, 0, stream>>>(state, xe, ge, reset, reset_columns, rs, rc, oe, new_state, n);
+    else recurrence_step<E, kGateLogit, 1><<<blocks, 256, 0, stream>>>(state, xe, ge, reset, reset_columns, rs, rc, oe, new_state, n);
+  }
+  return launch_status("recurrence step");
+}
+
+}  // namespace mbt_learning

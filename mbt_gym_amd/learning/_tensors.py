@@ -1,0 +1,38 @@
+"""What the operators' Python sides share: the checks of tensors, element types and streams."""
+import torch
+
+from mbt_gym_amd import _native
+
+DTYPES = {torch.float32: _native.FLOAT32, torch.bfloat16: _native.BFLOAT16, torch.float16: _native.FLOAT16}
+
+
+def require(tensor, name, device=None, dtypes=None, shape=None):
+    """A strided CUDA tensor (of this device, one of these dtypes, this shape), or a TypeError / ValueError that says what was given."""
+    if not isinstance(tensor, torch.Tensor):
+        raise TypeError(f"{name} has to be a torch tensor, not {type(tensor).__name__}")
+    if not tensor.is_cuda:
+        raise ValueError(f"{name} lives on {tensor.device}: the operators run on the GPU and have no CPU path")
+    if tensor.layout is not torch.strided:
+        raise TypeError(f"{name} has the layout {tensor.layout}: strided tensors only")
+    if device is not None and tensor.device != device:
+        raise ValueError(f"{name} lives on {tensor.device}, the other tensors on {device}")
+    if dtypes is not None and tensor.dtype not in dtypes:
+        raise TypeError(f"{name} is {tensor.dtype}: one of {', '.join(str(d) for d in dtypes)} is needed")
+    if shape is not None and tuple(tensor.shape) != tuple(shape):
+        raise ValueError(f"{name} has the shape {tuple(tensor.shape)}, {tuple(shape)} is needed")
+    return tensor
+
+
+def where(device):
+    """(device ordinal, handle of torch's current stream there)"""
+    return device.index, torch.cuda.current_stream(device).cuda_stream
+
+
+def dense_like(tensor):
+    """An empty tensor of the same shape whose axes lie in memory in the same order, without gaps."""
+    order = sorted(range(tensor.dim()), key=lambda d: (-tensor.stride(d), d))
+    out = torch.empty([tensor.shape[d] for d in order], dtype=tensor.dtype, device=tensor.device)
+    back = [0] * tensor.dim()
+    for position, d in enumerate(order):
+        back[d] = position
+    return out.permute(back)

@@ -1,0 +1,98 @@
+"""The learner's operators from their definitions in float64 on the CPU, with bounds on what a float32 evaluation may differ by.
+
+The bounds are derived, not fitted.  u is half a float32 step (2^-24) and v half a step of the element type.  A recurrence h = keep h + b that is
+evaluated in any association - one step after another, or chunks whose composites are joined - sends every input through at most the products and
+sums that stand between it and the output.  Per step of the walk these are two roundings (product, sum), four more for gates that are computed
+(sigmoid and its complement, each good to two ulps); joining chunks adds at most 64 (six levels within a wave, sixteen waves, the composites of
+segments in front: two roundings each).  With M the same recurrence over absolute values, the error E obeys E_t <= |keep| E_{t-1} + 6 u M_t, plus 64 u M_t
+once."""
+import numpy as np
+
+U = 2.0 ** -24
+HALF_STEP = {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}
+# below the smallest normal number the steps of a type stop shrinking: a rounding is then off by up to half of the smallest subnormal number
+# (float16: 2^-24 / 2; of the others, nothing that counts)
+HALF_SUBNORMAL = {"float32": 2.0 ** -150, "bfloat16": 2.0 ** -134, "float16": 2.0 ** -25}
+
+
+def sigmoid_pair(k):
+    with np.errstate(over="ignore"):
+        return 1.0 / (1.0 + np.exp(-k)), 1.0 / (1.0 + np.exp(k))
+
+
+def _drop(keep, state):
+    """keep * state, where a keep of zero drops the state whatever it holds"""
+    with np.errstate(invalid="ignore", over="ignore"):
+        return np.where(keep == 0.0, 0.0, keep * np.where(keep == 0.0, 0.0, state))
+
+
+class Recurrence:
+    """time first: x (T, B...), gate (T, B...) or a number, reset bool or None, initial (B...) or None"""
+
+    def __init__(self, x, gate, form, initial=None, reset=None, reverse=False, dtype="float32"):
+        self.reverse, self.form, self.v, self.w = reverse, form, HALF_STEP[dtype], HALF_SUBNORMAL[dtype]
+        turn = self.turn
+        self.x = turn(np.asarray(x, np.float64))
+        if form == "constant":
+            f, i = np.full_like(self.x, float(np.float32(gate))), np.ones_like(self.x)
+        else:
+            g = turn(np.asarray(gate, np.float64))
+            f, i = (g, np.ones_like(g)) if form == "value" else sigmoid_pair(g)
+        self.f, self.i = f, i
+        self.cut = np.zeros(self.x.shape, bool) if reset is None else turn(np.asarray(reset, bool))
+        self.keep = np.where(self.cut, 0.0, f)
+        self.h0 = np.zeros(self.x.shape[1:]) if initial is None else np.asarray(initial, np.float64)
+        h, m, e, r = self.h0, np.abs(self.h0), np.zeros_like(self.h0), np.zeros_like(self.h0)
+        self.h, self.before, self.bound, self.before_bound = (np.empty_like(self.x) for _ in range(4))
+        for t in range(len(self.x)):
+            self.before[t] = np.where(self.cut[t], 0.0, h)
+            self.before_bound[t] = np.where(self.cut[t], 0.0, e + 64 * U * m + r)
+            b = i[t] * self.x[t]
+            h = _drop(self.keep[t], h) + b
+            m = _drop(np.abs(self.keep[t]), m) + np.abs(b)
+            e = _drop(np.abs(self.keep[t]), e) + 6 * U * m
+            r = np.maximum(self.v * np.abs(h) + self.w, np.abs(self.keep[t]) * r)  # (a stored state that the backward pass starts a chunk from)
+            self.h[t], self.bound[t] = h, e + 64 * U * m
+        self.final, self.final_bound = h, e + 64 * U * m
+
+    def turn(self, a):
+        return a[::-1] if self.reverse else a
+
+    def states(self):
+        return self.turn(self.h), self.turn(self.bound + self.v * np.abs(self.h) + self.w)
+
+    def gradients(self, up, up_final=None):
+        """{name: (value, bound)} of inputs, gate, initial"""
+        up = self.turn(np.asarray(up, np.float64))
+        steps = len(up)
+        d = np.zeros_like(self.h0) if up_final is None else np.asarray(up_final, np.float64)
+        m, e, keep = np.abs(d), np.zeros_like(self.h0), np.ones_like(self.h0)
+        ds, db = np.empty_like(up), np.empty_like(up)
+        for t in range(steps - 1, -1, -1):
+            d = _drop(keep, d) + up[t]
+            m = _drop(np.abs(keep), m) + np.abs(up[t])
+            e = _drop(np.abs(keep), e) + 6 * U * m
+            ds[t], db[t] = d, e + 64 * U * m
+            keep = self.keep[t]
+        out = {"initial": (_drop(keep, d), np.abs(keep) * (e + 64 * U * m) + 6 * U * np.abs(keep * d))}
+        gx = self.i * ds
+        out["inputs"] = (self.turn(gx), self.turn(np.abs(self.i) * db + (6 * U + self.v) * np.abs(gx) + self.w))
+        if self.form == "value":
+            gg = ds * self.before
+            bound = db * np.abs(self.before) + np.abs(ds) * self.before_bound + (2 * U + self.v) * np.abs(gg) + self.w
+        else:
+            p, diff = self.f * self.i, self.before - self.x
+            gg = p * diff * ds
+            bound = p * (db * np.abs(diff) + np.abs(ds) * (self.before_bound + 2 * U * (np.abs(self.before) + np.abs(self.x)))) + (16 * U + self.v) * np.abs(gg) + self.w
+        if self.form != "constant":
+            out["gate"] = (self.turn(gg), self.turn(bound))
+        return out
+
+
+def assert_within(got, expected, bound, what):
+    got, expected, bound = (np.asarray(a, np.float64) for a in (got, expected, bound))
+    assert got.shape == expected.shape, (what, got.shape, expected.shape)
+    off = np.abs(got - expected) - bound - 1e-37  # (subnormal results: the hardware's exponential flushes them)
+    if off.size:
+        worst = np.unravel_index(np.argmax(np.where(np.isnan(off), np.inf, off)), off.shape)
+        assert off[worst] <= 0.0, (what, worst, got[worst], expected[worst], bound[worst])

@@ -1,0 +1,359 @@
+"""mbt_gym_amd.learning: the gated linear recurrence, its backward pass and its single step against their definitions in float64."""
+import numpy as np
+import pytest
+
+from tests.learning_oracle import HALF_STEP, U, Recurrence, assert_within, sigmoid_pair
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
+
+
+def learning():
+    from mbt_gym_amd import learning as module
+
+    return module
+
+
+def to64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def make(shape, form, dtype, seed, reset=False, initial=True, layout="time_first"):
+    """time-first tensors whose memory lies as `layout` says"""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+
+    def place(t):
+        if layout == "time_last":
+            return t.movedim(0, -1).contiguous().movedim(-1, 0)
+        if layout == "padded":  # rows of a wider recording
+            wide = torch.zeros((t.shape[0], t.shape[1] + 5) + t.shape[2:], dtype=t.dtype, device=t.device)
+            wide[:, :t.shape[1]] = t
+            return wide[:, :t.shape[1]]
+        if layout == "batch_first":
+            return t.transpose(0, 1).contiguous().transpose(0, 1) if t.dim() > 1 else t
+        return t
+
+    x = place(torch.randn(shape, generator=gen, device="cuda").to(DTYPES[dtype]))
+    gate = torch.randn(shape, generator=gen, device="cuda") * 1.5 + 1.5
+    gate = 0.97 if form == "constant" else place((gate if form == "logit" else torch.sigmoid(gate) * torch.sign(torch.randn(shape, generator=gen, device="cuda") + 2.0)).to(DTYPES[dtype]))
+    h0 = torch.randn(shape[1:], generator=gen, device="cuda") if initial else None
+    cut = place(torch.rand(shape, generator=gen, device="cuda") < 0.05) if reset else None
+    return x, gate, h0, cut
+
+
+def run_case(shape, form, dtype, reverse, reset, initial, layout, seed=0):
+    x, gate, h0, cut = make(shape, form, dtype, seed, reset, initial, layout)
+    leaves = [t for t in (x, gate, h0) if isinstance(t, torch.Tensor)]
+    for t in leaves:
+        t.requires_grad_(True)
+    states, final = learning().linear_recurrence(x, gate, h0, dim=0, reverse=reverse, reset=cut, gate_is_logit=form == "logit", return_final=True)
+    assert states.shape == x.shape and states.dtype == x.dtype and final.dtype == torch.float32 and tuple(final.shape) == tuple(shape[1:])
+    up = torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(seed + 1), device="cuda").to(DTYPES[dtype])
+    up_final = torch.randn(shape[1:], generator=torch.Generator(device="cuda").manual_seed(seed + 2), device="cuda")
+    grads = torch.autograd.grad([states, final], leaves, [up, up_final])
+    ref = Recurrence(to64(x), gate if form == "constant" else to64(gate), form, None if h0 is None else to64(h0), None if cut is None else cut.cpu().numpy(), reverse, dtype)
+    what = (shape, form, dtype, reverse, reset, initial, layout)
+    assert_within(to64(states), *ref.states(), ("states",) + what)
+    assert_within(to64(final), ref.final, ref.final_bound, ("final",) + what)
+    expected = ref.gradients(to64(up), to64(up_final))
+    names = ["inputs"] + (["gate"] if form != "constant" else []) + (["initial"] if initial else [])
+    for name, grad in zip(names, grads):
+        assert_within(to64(grad), *expected[name], ("grad " + name,) + what)
+
+
+SIZES = [(1, 1), (1, 700), (2, 3), (7, 1), (15, 64), (16, 65), (17, 130), (50, 16, 3), (200, 33), (257, 8), (1000, 5), (1001, 7, 5), (4100, 2), (9000, 66)]
+
+
+@pytest.mark.parametrize("shape", SIZES, ids=str)
+@pytest.mark.parametrize("form", ["constant", "value", "logit"])
+@pytest.mark.parametrize("layout", ["time_first", "time_last"])
+def test_forward_and_backward_float32(shape, form, layout):
+    print(shape, form, layout, flush=True)
+    run_case(shape, form, "float32", reverse=False, reset=True, initial=True, layout=layout)
+    run_case(shape, form, "float32", reverse=True, reset=False, initial=False, layout=layout, seed=5)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("shape", [(1, 9), (3, 17), (33, 64, 4), (129, 40), (1001, 24), (5000, 8)], ids=str)
+@pytest.mark.parametrize("form", ["constant", "value", "logit"])
+@pytest.mark.parametrize("layout", ["time_first", "time_last"])
+def test_forward_and_backward_16_bit(shape, form, dtype, layout):
+    print(shape, form, dtype, layout, flush=True)
+    run_case(shape, form, dtype, reverse=True, reset=True, initial=True, layout=layout)
+    run_case(shape, form, dtype, reverse=False, reset=False, initial=False, layout=layout, seed=9)
+
+
+@pytest.mark.parametrize("layout", ["padded", "batch_first"])
+@pytest.mark.parametrize("shape", [(40, 37), (300, 12, 7)], ids=str)
+def test_strided_operands(shape, layout):
+    for form in ("value", "logit"):
+        run_case(shape, form, "float32", reverse=False, reset=True, initial=True, layout=layout)
+        run_case(shape, form, "bfloat16", reverse=True, reset=True, initial=True, layout=layout)
+
+
+@pytest.mark.parametrize("shape", [(20, 1 << 18), (70, 1 << 16), (1 << 17, 3)], ids=str)
+def test_many_columns_and_many_steps(shape):
+    run_case(shape, "value", "float32", reverse=False, reset=False, initial=True, layout="time_first")
+    run_case(shape, "logit", "bfloat16", reverse=True, reset=True, initial=True, layout="time_first")
+
+
+def test_operands_of_different_layouts_and_expanded_ones():
+    x, _, h0, _ = make((60, 20, 6), "value", "float32", 3)
+    gate = torch.sigmoid(torch.randn(6, device="cuda")).expand(60, 20, 6)             # one gate per channel
+    cut = (torch.rand(60, 20, 1, device="cuda") < 0.1).expand(60, 20, 6)              # one flag per lane
+    turned = x.permute(2, 1, 0).contiguous().permute(2, 1, 0)
+    for inputs in (x, turned):
+        states = learning().linear_recurrence(inputs, gate, h0, reset=cut)
+        ref = Recurrence(to64(x), to64(gate), "value", to64(h0), cut.cpu().numpy())
+        assert_within(to64(states), *ref.states(), "expanded")
+    leaf = torch.sigmoid(torch.randn(6, device="cuda")).requires_grad_(True)
+    learning().linear_recurrence(x, leaf.expand(60, 20, 6), h0).sum().backward()       # (an expanded gradient comes back too)
+    ref = Recurrence(to64(x), to64(leaf.detach().expand(60, 20, 6)), "value", to64(h0))
+    value, bound = ref.gradients(np.ones((60, 20, 6)))["gate"]
+    total = bound.sum(axis=(0, 1)) + 1200 * U * np.abs(value).sum(axis=(0, 1))
+    assert_within(to64(leaf.grad), value.sum(axis=(0, 1)), total, "shared gate")
+
+
+@pytest.mark.parametrize("steps", [1, 5, 40, 300, 3000])
+@pytest.mark.parametrize("layout", ["time_first", "time_last"])
+def test_a_reset_and_a_zero_gate_stop_infinities_and_nans(steps, layout):
+    x, gate, h0, _ = make((steps, 70), "value", "float32", 1, layout=layout)
+    x, gate = x.clone(memory_format=torch.preserve_format), gate.clone(memory_format=torch.preserve_format)
+    h0[0], h0[1] = float("nan"), float("inf")
+    cut = torch.zeros(x.shape, dtype=torch.bool, device="cuda")
+    cut[0, 0] = True
+    gate[0, 1] = 0.0
+    if steps > 3:
+        x[steps // 2, 2] = float("inf")
+        cut[steps // 2 + 1, 2] = True
+        x[steps // 2, 3] = float("nan")
+        gate[steps // 2 + 1, 3] = 0.0
+    ref = Recurrence(to64(x), to64(gate), "value", to64(h0), cut.cpu().numpy())
+    states, final = learning().linear_recurrence(x, gate, h0, reset=cut, return_final=True)
+    expected, bound = ref.states()
+    finite = np.isfinite(expected)
+    assert np.array_equal(np.isfinite(to64(states)), finite) and finite[:, :2].all()
+    assert_within(np.where(finite, to64(states), 0.0), np.where(finite, expected, 0.0), np.where(finite, bound, 0.0), "dropped")
+    # and a state that is not dropped stays what it is, however small the product of the gates gets
+    x[0, 4] = float("nan")
+    gate[:, 4] = 0.3
+    states = learning().linear_recurrence(x, gate, torch.zeros_like(h0))
+    assert torch.isnan(states[:, 4]).all()
+
+
+@pytest.mark.parametrize("steps", [4, 90, 2500])
+@pytest.mark.parametrize("layout", ["time_first", "time_last"])
+def test_gradients_do_not_pass_a_reset(steps, layout):
+    """what stands behind a reset - an episode that blew up - leaves the gradients in front of it finite and equal to those of the first piece alone"""
+    x, gate, h0, _ = make((steps, 6), "value", "float32", 2, layout=layout)
+    cut = torch.zeros(x.shape, dtype=torch.bool, device="cuda")
+    cut[steps // 2] = True
+    up = torch.randn(steps, 6, device="cuda")
+    up[steps // 2:] = float("nan")
+    a, g, h = (t.clone(memory_format=torch.preserve_format).requires_grad_(True) for t in (x, gate, h0))
+    grads = torch.autograd.grad(learning().linear_recurrence(a, g, h, reset=cut), [a, g, h], up)
+    first = Recurrence(to64(x[:steps // 2]), to64(gate[:steps // 2]), "value", to64(h0))
+    expected = first.gradients(to64(up[:steps // 2]))
+    assert_within(to64(grads[0][:steps // 2]), *expected["inputs"], "inputs")
+    assert_within(to64(grads[1][:steps // 2]), *expected["gate"], "gate")
+    assert_within(to64(grads[2]), *expected["initial"], "initial")
+
+
+def test_gates_at_their_limits():
+    logits = torch.tensor([-200.0, -110.5, -90.0, -20.0, -1e-3, 0.0, 1e-3, 20.0, 90.0, 200.0, float("inf"), float("-inf")], device="cuda")
+    x, h0 = torch.full((1, 12), 2.0, device="cuda"), torch.full((12,), -3.0, device="cuda")
+    states = learning().linear_recurrence(x, logits[None], h0, gate_is_logit=True)
+    f, i = sigmoid_pair(to64(logits))
+    assert_within(to64(states)[0], -3.0 * f + 2.0 * i, 16 * U * (3.0 * f + 2.0 * i), "logits")
+    nan = learning().linear_recurrence(x[:, :1], torch.full((1, 1), float("nan"), device="cuda"), h0[:1], gate_is_logit=True)
+    assert torch.isnan(nan).all()
+
+
+def test_gradients_agree_with_differences():
+    """central differences of a scalar of the float64 definition, at a float32 point; the step 2^-10 leaves h^2 / 6 times the third derivative"""
+    x, gate, h0, cut = make((9, 4), "logit", "float32", 8, reset=True)
+    up = torch.randn(9, 4, device="cuda")
+    a, g, h = (t.clone().requires_grad_(True) for t in (x, gate, h0))
+    grads = torch.autograd.grad(learning().linear_recurrence(a, g, h, reset=cut, gate_is_logit=True), [a, g, h], up)
+
+    def value(xs, gs, hs):
+        return float((Recurrence(xs, gs, "logit", hs, cut.cpu().numpy()).h * to64(up)).sum())
+
+    point = [to64(x), to64(gate), to64(h0)]
+    step = 2.0 ** -10
+    for which, grad in enumerate(grads):
+        for at in np.ndindex(point[which].shape):
+            moved = []
+            for sign in (1, -1):
+                q = [p.copy() for p in point]
+                q[which][at] += sign * step
+                moved.append(value(*q))
+            difference = (moved[0] - moved[1]) / (2 * step)
+            # third derivatives of a sigmoid are at most 1/8, of the sum over nine steps at most 9 |up| (|x| + |h|) < 9 * 4 * 8
+            assert abs(float(grad[at]) - difference) <= step ** 2 / 6 * 9 * 32 / 8 + 1e-5, (which, at)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("shape", [(1,), (3, 5), (1000, 64), (4099, 257)], ids=str)
+@pytest.mark.parametrize("logit", [False, True])
+def test_a_single_step(shape, dtype, logit):
+    x, gate, h0, _ = make((1,) + shape, "logit" if logit else "value", dtype, 4)
+    cut = (torch.rand(shape[:-1] + (1,), device="cuda") < 0.3).expand(shape)
+    before = h0.clone()
+    ref = Recurrence(to64(x), to64(gate), "logit" if logit else "value", to64(h0), cut.cpu().numpy()[None], dtype=dtype)
+    with torch.no_grad():
+        out, new = learning().linear_recurrence_step(h0, x[0], gate[0], reset=cut, gate_is_logit=logit)
+        assert torch.equal(h0, before) and out.dtype == DTYPES[dtype] and new.dtype == torch.float32
+        assert_within(to64(out), ref.states()[0][0], ref.states()[1][0], "out")
+        assert_within(to64(new), ref.final, ref.final_bound, "new")
+        again, same = learning().linear_recurrence_step(h0, x[0], gate[0], reset=cut, gate_is_logit=logit, new_state=h0)  # in place
+        assert same is h0 and torch.equal(h0, new) and torch.equal(again, out)
+
+
+def test_steps_repeat_the_sequence_and_pieces_join():
+    x, gate, h0, cut = make((37, 50, 3), "logit", "float32", 6, reset=True)
+    states, final = learning().linear_recurrence(x, gate, h0, reset=cut, gate_is_logit=True, return_final=True)
+    ref = Recurrence(to64(x), to64(gate), "logit", to64(h0), cut.cpu().numpy())
+    carry = h0
+    for t in range(37):
+        out, carry = learning().linear_recurrence_step(carry, x[t], gate[t], reset=cut[t], gate_is_logit=True)
+        assert_within(to64(out), ref.h[t], ref.bound[t] + U * np.abs(ref.h[t]), t)
+    front, middle = learning().linear_recurrence(x[:20], gate[:20], h0, reset=cut[:20], gate_is_logit=True, return_final=True)
+    back, end = learning().linear_recurrence(x[20:], gate[20:], middle, reset=cut[20:], gate_is_logit=True, return_final=True)
+    assert_within(to64(torch.cat([front, back])), *ref.states(), "pieces")
+    assert_within(to64(end), ref.final, ref.final_bound, "end")
+
+
+def test_a_sequence_without_steps_or_lanes():
+    x = torch.empty(0, 5, device="cuda", requires_grad=True)
+    h0 = torch.randn(5, device="cuda", requires_grad=True)
+    states, final = learning().linear_recurrence(x, 0.5, h0, return_final=True)
+    assert states.shape == (0, 5) and torch.equal(final, h0)
+    final.sum().backward()
+    assert torch.equal(h0.grad, torch.ones_like(h0))
+    assert learning().linear_recurrence(torch.empty(7, 0, device="cuda"), 0.5).shape == (7, 0)
+    assert learning().linear_recurrence(torch.empty(0, 5, device="cuda"), 0.5, return_final=True)[1].tolist() == [0.0] * 5
+
+
+def test_only_the_final_state_is_used():
+    x, gate, h0, _ = make((11, 8), "value", "bfloat16", 2)
+    for g in (gate.requires_grad_(True), 0.9):
+        a, h = x.clone().requires_grad_(True), h0.clone().requires_grad_(True)
+        final = learning().linear_recurrence(a, g, h, return_final=True)[1]
+        grads = torch.autograd.grad(final.sum(), [a, h])
+        ref = Recurrence(to64(x), to64(g) if isinstance(g, torch.Tensor) else g, "value" if isinstance(g, torch.Tensor) else "constant", to64(h0), dtype="bfloat16")
+        expected = ref.gradients(np.zeros((11, 8)), np.ones(8))
+        assert_within(to64(grads[0]), *expected["inputs"], "inputs")
+        assert_within(to64(grads[1]), *expected["initial"], "initial")
+
+
+@pytest.mark.parametrize("lanes, steps", [(1, 1), (1000, 200), (513, 50), (3, 4000), (70000, 5)])
+@pytest.mark.parametrize("discount", [1.0, 0.99, 0.0])
+def test_rewards_to_go_of_a_recording(lanes, steps, discount):
+    """(N, 1, T) views of time-major recordings with padded lanes, as the learner has them, and contiguous ones as generate_trajectory returns them"""
+    padded = -(-lanes // 512) * 512
+    recorded = torch.randn(steps, padded, device="cuda")
+    rewards = recorded[:, :lanes].t().unsqueeze(1)
+    done = torch.rand(lanes, 1, steps, device="cuda") < 0.02
+    for given, flags in ((rewards, None), (rewards.contiguous(), None), (rewards, done)):
+        got = learning().rewards_to_go(given, discount, done=flags)
+        ref = Recurrence(to64(given).transpose(2, 0, 1), discount, "constant", reset=None if flags is None else flags.cpu().numpy().transpose(2, 0, 1), reverse=True)
+        value, bound = ref.states()
+        assert_within(to64(got).transpose(2, 0, 1), value, bound, (lanes, steps, discount))
+    assert torch.equal(recorded[:, lanes:], recorded[:, lanes:].clone())
+
+
+def test_a_captured_graph_replays_and_two_graphs_have_their_own_workspaces():
+    shape = (70000, 4)  # (long enough that the walk is split over workgroups and needs a workspace)
+    x, gate, h0, _ = make(shape, "value", "float32", 11)
+    other = make(shape, "value", "float32", 12)
+    for t in (x, gate, h0):
+        t.requires_grad_(True)
+    up = torch.randn(shape, device="cuda")
+
+    def step(a, g, h):
+        states = learning().linear_recurrence(a, g, h)
+        return [states.detach()] + list(torch.autograd.grad(states, [a, g, h], up))
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(x, gate, h0)
+    torch.cuda.current_stream().wait_stream(stream)
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs.append(step(x, gate, h0))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for round_ in range(4):
+        with torch.no_grad():
+            source = other if round_ % 2 else make(shape, "value", "float32", 20 + round_)
+            for t, s in zip((x, gate, h0), source):
+                t.copy_(s)
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):  # at the same time, on two streams
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        eager = step(x, gate, h0)
+        for out in outs:
+            for a, b in zip(out, eager):
+                assert torch.equal(a, b), round_
+
+
+def test_two_streams_at_once_and_repeated_calls_give_the_same_bits():
+    x, gate, h0, _ = make((20000, 12), "logit", "float32", 13)
+    with torch.no_grad():
+        expected = learning().linear_recurrence(x, gate, h0, gate_is_logit=True)
+        torch.cuda.synchronize()
+        streams, results = [torch.cuda.Stream(), torch.cuda.Stream()], []
+        for k in range(6):
+            with torch.cuda.stream(streams[k % 2]):
+                results.append(learning().linear_recurrence(x, gate, h0, gate_is_logit=True))
+        torch.cuda.synchronize()
+    assert all(torch.equal(r, expected) for r in results)
+
+
+def test_the_loss_of_a_small_actor_goes_through_autograd():
+    """the operator inside an ordinary torch network: second use of the same leaf, gradients accumulate, second derivatives are refused"""
+    layer = torch.nn.Linear(3, 8).cuda()
+    obs = torch.randn(12, 5, 3, device="cuda")
+    out = layer(obs)
+    h = learning().linear_recurrence(out[..., :4], out[..., 4:], gate_is_logit=True)
+    h2 = learning().linear_recurrence(h, 0.5, reverse=True)
+    (h2 * h).sum().backward()
+    assert all(torch.isfinite(p.grad).all() and p.grad.abs().sum() > 0 for p in layer.parameters())
+    x = torch.randn(4, 3, device="cuda", requires_grad=True)
+    grad, = torch.autograd.grad(learning().linear_recurrence(x, 0.5).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(grad.sum(), x)
+
+
+def test_refusals_on_the_device():
+    call = learning().linear_recurrence
+    x = torch.randn(5, 3, device="cuda")
+    for arguments, error, text in [
+        ((x.double(), 0.5), TypeError, "float64"), ((x[0, 0], 0.5), ValueError, "scalar"), ((x, x[:4]), ValueError, "shape"),
+        ((x, x.half()), TypeError, "float16"), ((x, float("inf")), ValueError, "finite"), ((x, x.cpu()), ValueError, "no CPU path"),
+        ((x, 0.5, torch.zeros(4, device="cuda")), ValueError, "shape"), ((x, 0.5, torch.zeros(3, device="cuda", dtype=torch.float16)), TypeError, "float16"),
+    ]:
+        with pytest.raises(error, match=text):
+            call(*arguments)
+    with pytest.raises(TypeError, match="gate tensor"):
+        call(x, 0.5, gate_is_logit=True)
+    with pytest.raises(IndexError):
+        call(x, 0.5, dim=2)
+    with pytest.raises(TypeError, match="reset"):
+        call(x, 0.5, reset=x)
+    with pytest.raises(ValueError, match="reset"):
+        call(x, 0.5, reset=torch.zeros(5, dtype=torch.bool, device="cuda"))
+    step = learning().linear_recurrence_step
+    with pytest.raises(TypeError, match="state"):
+        step(x.half(), x, x)
+    with pytest.raises(ValueError, match="contiguous"):
+        step(torch.randn(3, 5, device="cuda").t(), x, x)
+    with pytest.raises(ValueError, match="not differentiable"):
+        step(x, x, x.clone().requires_grad_(True))

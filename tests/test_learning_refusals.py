@@ -1,0 +1,123 @@
+"""What the learner's operators refuse, without a device: the Python side's checks of its tensors and the C side's checks of its arguments (which
+come before any device is touched)."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+
+from mbt_gym_amd import _native
+
+torch = pytest.importorskip("torch")
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HEADER = os.path.join(ROOT, "include", "mbt_env.h")
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _native.load_library()
+
+
+def refused(lib, rc, text):
+    assert rc == -1 and text.encode() in lib.mbt_last_error(), (rc, lib.mbt_last_error())
+
+
+def offsets_match(struct, name, tmp_path):
+    """sizeof / offsetof from a C compiler on the header == the ctypes binding"""
+    fields = [f for f, _ in struct._fields_]
+    body = "".join(f'  printf("{f} %zu\\n", offsetof({name}, {f}));\n' for f in fields)
+    source = tmp_path / f"{name}.c"
+    source.write_text(f'#include <stdio.h>\n#include <stddef.h>\n#include "{HEADER}"\nint main(void) {{\n  printf("sizeof %zu\\n", sizeof({name}));\n{body}  return 0; }}\n')
+    exe = tmp_path / name
+    subprocess.run(["gcc", "-std=c11", "-Wall", "-Werror", str(source), "-o", str(exe)], check=True)
+    out = dict(line.split() for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines())
+    assert int(out.pop("sizeof")) == C.sizeof(struct)
+    for field, offset in out.items():
+        assert getattr(struct, field).offset == int(offset), field
+
+
+# ---- the recurrence --------------------------------------------------------------------------------------------------------------------
+def test_recurrence_struct_layout(tmp_path):
+    offsets_match(_native.MbtArray3, "mbt_array3", tmp_path)
+    offsets_match(_native.MbtRecurrence, "mbt_recurrence", tmp_path)
+
+
+def recurrence_struct(**changes):
+    """valid arguments over addresses that nothing reads: a refusal comes first, and without a device so does the lack of one"""
+    r = _native.MbtRecurrence(outer=2, steps=3, inner=4, dtype=_native.FLOAT32, form=_native.GATE_VALUE, workspace_bytes=0)
+    for name in ("inputs", "gate", "states", "grad_states", "grad_inputs", "grad_gate"):
+        array = getattr(r, name)
+        array.data = 4096
+        array.stride[0], array.stride[1], array.stride[2] = 12, 4, 1
+    for name, value in changes.items():
+        setattr(r, name, value)
+    return r
+
+
+def test_the_library_refuses_a_malformed_recurrence(lib):
+    def forward(r):
+        return lib.mbt_recurrence_forward(0, C.byref(r), None)
+
+    refused(lib, lib.mbt_recurrence_forward(0, None, None), "null argument")
+    refused(lib, forward(recurrence_struct(dtype=7)), "dtype 7")
+    refused(lib, forward(recurrence_struct(form=3)), "form 3")
+    for name in ("outer", "steps", "inner"):
+        refused(lib, forward(recurrence_struct(**{name: 0})), "at least 1")
+        refused(lib, forward(recurrence_struct(**{name: 1 << 41})), "beyond 2^40")
+    refused(lib, forward(recurrence_struct(outer=1 << 30, inner=1 << 30)), "beyond 2^40")
+    missing = recurrence_struct()
+    missing.gate.data = None
+    refused(lib, forward(missing), "needs a gate")
+    missing = recurrence_struct()
+    missing.states.data = None
+    refused(lib, forward(missing), "inputs and states")
+    missing = recurrence_struct()
+    missing.grad_states.data = None
+    refused(lib, lib.mbt_recurrence_backward(0, C.byref(missing), None), "needs grad_states")
+    constant = recurrence_struct(form=_native.GATE_CONSTANT, constant=float("nan"))
+    constant.grad_gate.data = None
+    refused(lib, forward(constant), "not finite")
+    constant = recurrence_struct(form=_native.GATE_CONSTANT, constant=0.5)
+    refused(lib, lib.mbt_recurrence_backward(0, C.byref(constant), None), "no gradient array")
+
+
+def test_a_long_walk_needs_its_workspace(lib):
+    r = recurrence_struct(outer=1, steps=1 << 16, inner=4)
+    size = lib.mbt_recurrence_workspace(C.byref(r), 0)
+    assert size > 0
+    refused(lib, lib.mbt_recurrence_forward(0, C.byref(r), None), f"{size} are needed")
+    r.workspace, r.workspace_bytes = 4096, size - 1
+    refused(lib, lib.mbt_recurrence_forward(0, C.byref(r), None), f"{size} are needed")
+    r.workspace, r.workspace_bytes = 4100, size
+    refused(lib, lib.mbt_recurrence_forward(0, C.byref(r), None), "aligned")
+    assert lib.mbt_recurrence_workspace(C.byref(recurrence_struct()), 0) == 0
+
+
+def test_the_library_refuses_a_malformed_step(lib):
+    args = dict(device=0, dtype=0, form=_native.GATE_VALUE, rows=3, columns=4, state=4096, inputs=4096, gate=4096, reset=None, rs=0, cs=0, out=4096, new=4096)
+
+    def step(**changes):
+        return lib.mbt_recurrence_step(*{**args, **changes}.values(), None)
+
+    refused(lib, step(dtype=3), "dtype 3")
+    refused(lib, step(form=_native.GATE_CONSTANT), "MBT_GATE_VALUE or MBT_GATE_LOGIT")
+    for name in ("state", "inputs", "gate", "out", "new"):
+        refused(lib, step(**{name: None}), "null argument")
+    for sizes in ((0, 1), (1, 0), (1 << 20, 1 << 20)):
+        refused(lib, step(rows=sizes[0], columns=sizes[1]), "2^38")
+
+
+def test_tensors_that_are_not_on_the_device_are_refused():
+    from mbt_gym_amd import learning
+
+    x = torch.randn(5, 3)
+    with pytest.raises(ValueError, match="no CPU path"):
+        learning.linear_recurrence(x, 0.5)
+    with pytest.raises(ValueError, match="no CPU path"):
+        learning.linear_recurrence_step(x, x, x)
+    with pytest.raises(ValueError, match="no CPU path"):
+        learning.rewards_to_go(x)
+    with pytest.raises(TypeError, match="torch tensor"):
+        learning.linear_recurrence([1.0, 2.0], 0.5)
+    with pytest.raises(ValueError, match="discount"):
+        learning.rewards_to_go(x, 1.5)
