@@ -92,8 +92,14 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
   P.steps = steps;
   P.outer = static_cast<int64_t>(swap ? r->inner : r->outer);
   P.inner = static_cast<int64_t>(swap ? r->outer : r->inner);
-  P.batch_initial_swapped = swap ? 1 : 0;
+  P.batch_swapped = swap ? 1 : 0;
   P.constant = static_cast<float>(r->constant);
+  P.constant_rest = static_cast<float>(r->constant - static_cast<double>(P.constant));
+  double power = 1.0;
+  for (int k = 0; k <= kMostSteps; ++k) {
+    P.power[k] = static_cast<float>(power);
+    power *= r->constant;
+  }
   P.segments = 1;
   P.segment = steps;
   plan.lds = 0;
@@ -122,25 +128,25 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
     return MBT_OK;
   }
 
-  const bool wide = inner_contiguous && P.inner >= vector;
-  const int v = wide ? vector : 1;
-  const int base = wide ? kColumnsVector : kColumnsScalar;
+  // Columns per thread: one float32 or two 16-bit elements, so that a wave's row is 256 bytes and the time axis can be cut finely; a recording with
+  // columns enough for every wave of the chip to have 64 x 16 bytes of its own is walked forwards in such vectors, alone.
+  const int pair = inner_contiguous && size == 2 && P.inner >= 2 ? 2 : 1;
+  const bool wide = !backward && inner_contiguous && P.outer * (P.inner / vector) >= chip;
+  const int v = wide ? vector : pair;
+  const int base = wide ? kColumnsWide : pair == 2 ? kColumnsPair : kColumnsScalar;
   P.vectors_per_outer = ceil_div(P.inner, v);
   P.vectors = P.outer * P.vectors_per_outer;
-  const int chunk = v == 1 ? 16 : 16 / v;  // (recurrence_launch.hpp: kChunk<V, kJoined>)
+  const int chunk = chunk_steps(r->form, backward, v, false);
   int64_t parallel = ceil_div(chip, P.vectors);
   if (parallel > ceil_div(steps, chunk)) parallel = ceil_div(steps, chunk);
-  if (parallel <= 2) {
+  if (wide || parallel <= 2) {
     plan.which = base + kAlone;
     plan.threads = 256;
     plan.blocks = ceil_div(P.vectors, 256);
     return MBT_OK;
   }
-  // columns of a workgroup: at most what LDS holds, at least a 128-byte line's worth, fewer when that buys chunks of time
-  int columns_log2 = v == 1 ? 6 : log2_ceil(256 / v);
-  if (columns_log2 > 6) columns_log2 = 6;
-  const int least = log2_ceil(128 / (v * static_cast<int>(size)));
-  while (columns_log2 > least && (1024 >> columns_log2) < parallel) --columns_log2;
+  // a workgroup takes 64 column vectors (256 bytes of a row), fewer only when there are fewer
+  int columns_log2 = 6;
   while (columns_log2 > 0 && (int64_t{1} << (columns_log2 - 1)) >= P.vectors) --columns_log2;
   int chunks_log2 = log2_ceil(parallel);
   if (chunks_log2 > 10 - columns_log2) chunks_log2 = 10 - columns_log2;
@@ -162,7 +168,7 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
   plan.which = base + kJoined;
   plan.threads = static_cast<unsigned>(chunks * columns);
   plan.blocks = P.column_blocks * P.segments;
-  plan.lds = static_cast<size_t>(plan.threads / 64) * v * columns * sizeof(float2);
+  plan.lds = static_cast<size_t>(plan.threads / 64 + 1) * v * columns * sizeof(float2);
   if (P.segments > 1) plan.workspace = static_cast<uint64_t>(P.vectors) * v * P.segments * sizeof(float2);
   return MBT_OK;
 }

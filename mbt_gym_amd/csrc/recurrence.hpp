@@ -26,6 +26,8 @@ namespace mbt_learning {
 
 constexpr int kGateConstant = MBT_GATE_CONSTANT, kGateValue = MBT_GATE_VALUE, kGateLogit = MBT_GATE_LOGIT;
 
+constexpr int kMostSteps = 16;  // steps of a chunk that one thread holds in registers
+
 struct Axis {  // one operand: address at the first step in walking order, element strides (time signed: reversed walks go down)
   void* p;
   int64_t so, st, si;
@@ -42,22 +44,30 @@ struct RecurrenceParams {
   int64_t vectors_per_outer, vectors;  // column vectors (V columns each)
   int64_t segment;                     // steps per segment
   int32_t segments;
-  int32_t lanes_log2;  // columns: column vectors per workgroup; rows: lanes per row
-  int32_t batch_initial_swapped;  // initial / final are (outer, inner) of the CALLER; 1 when the kernel's axes are exchanged
+  int32_t lanes_log2;     // columns: column vectors per workgroup; rows: lanes per row
+  int32_t batch_swapped;  // initial / final are (outer, inner) of the CALLER: 1 when the kernel's axes are exchanged
   int64_t column_blocks;
-  float constant;
+  // the constant gate as a float32 pair (0.99 is not a float32 number, and its error would be made at every step), and the powers of the
+  // double that a chunk of n steps composes to
+  float constant, constant_rest;
+  float power[kMostSteps + 1];
 };
-
-__device__ __forceinline__ float apply_step(float keep, float h, float b) { return keep == 0.0f ? b : __builtin_fmaf(keep, h, b); }
 
 struct Composite {
   float a, b;
 };
-// first, then second.  The product of two non-zero gates must not underflow to the zero that means "dropped".
+__device__ __forceinline__ float apply_step(float keep, float h, float b) { return keep == 0.0f ? b : __builtin_fmaf(keep, h, b); }
+// first, then second.  The product of two non-zero gates must not underflow to the zero that means "dropped".  A state is the composite (0, h).
 __device__ __forceinline__ Composite then(Composite first, Composite second) {
   float a = first.a * second.a;
   if (a == 0.0f && first.a != 0.0f && second.a != 0.0f) a = 1.4e-45f;
   return {a, apply_step(second.a, first.b, second.b)};
+}
+// one step of the walk
+template <int FORM>
+__device__ __forceinline__ float advance(const RecurrenceParams& P, float keep, float h, float b) {
+  if (FORM != kGateConstant) return apply_step(keep, h, b);
+  return keep == 0.0f ? b : __builtin_fmaf(keep, h, __builtin_fmaf(P.constant_rest, h, b));
 }
 
 // f = sigmoid(k) and 1 - f, each to about an ulp: e = exp(-|k|) with the rounding of the exponent's product carried along, r = 1 / (1 + e) by one
@@ -77,12 +87,24 @@ __device__ __forceinline__ void sigmoid_pair(float k, float& f, float& i) {
   if (k != k) f = i = k;
 }
 
+// what multiplies the state (unless a reset drops it) and what multiplies the input; g is turned in place into the former
 template <int FORM>
-__device__ __forceinline__ void gates(float g, bool reset, float constant, float& keep, float& f, float& i) {
-  if (FORM == kGateConstant) f = constant, i = 1.0f;
-  if (FORM == kGateValue) f = g, i = 1.0f;
-  if (FORM == kGateLogit) sigmoid_pair(g, f, i);
-  keep = reset ? 0.0f : f;
+__device__ __forceinline__ void gate(const RecurrenceParams& P, float& g, float& inject) {
+  inject = 1.0f;
+  if (FORM == kGateConstant) g = P.constant;
+  if (FORM == kGateLogit) {
+    float f;
+    sigmoid_pair(g, f, inject);
+    g = f;
+  }
+}
+
+// Steps of a chunk, held in registers: 16 elements of each array, so that a thread of a 1024-thread workgroup stays within its 128 registers - the
+// backward pass of the logit form holds four arrays over the join and takes half of that - and twice as many for a thread that walks alone
+// forwards with whole vectors.
+constexpr int chunk_steps(int form, bool backward, int v, bool alone) {
+  if (v > 2) return 32 / v;
+  return (backward && form == kGateLogit && !alone ? 8 : 16) / v;
 }
 
 // ---- columns -----------------------------------------------------------------------------------------------------------------------
@@ -94,8 +116,9 @@ struct Column {
   int64_t o, i;
   int nv;  // valid columns of the V (0: a lane without work)
 
-  __device__ __forceinline__ void load(const Axis& t, int64_t s, float (&out)[V]) const {
-    const E* p = static_cast<const E*>(t.p) + o * t.so + s * t.st + i * t.si;
+  // address at step s; the next step's is t.st further (walked, not recomputed: an address per step and array would not fit the registers)
+  __device__ __forceinline__ E* at(const Axis& t, int64_t s) const { return static_cast<E*>(t.p) + o * t.so + s * t.st + i * t.si; }
+  __device__ __forceinline__ void load(const E* p, float (&out)[V]) const {
     if (nv == V) {
       const Pack<E, V> v = load_pack<E, V>(p);
 #pragma unroll
@@ -105,8 +128,7 @@ struct Column {
       for (int j = 0; j < V; ++j) out[j] = j < nv ? static_cast<float>(p[j]) : 0.0f;
     }
   }
-  __device__ __forceinline__ void store(const Axis& t, int64_t s, const float (&in)[V]) const {
-    E* p = static_cast<E*>(t.p) + o * t.so + s * t.st + i * t.si;
+  __device__ __forceinline__ void store(E* p, const float (&in)[V]) const {
     if (nv == V) {
       Pack<E, V> v;
 #pragma unroll
@@ -123,7 +145,7 @@ struct Column {
   }
   // (outer, inner) float32 of the caller
   __device__ __forceinline__ int64_t batch(const RecurrenceParams& P, int j) const {
-    return P.batch_initial_swapped ? (i + j) * P.outer + o : o * P.inner + i + j;
+    return P.batch_swapped ? (i + j) * P.outer + o : o * P.inner + i + j;
   }
   __device__ __forceinline__ void load_batch(const RecurrenceParams& P, const float* p, float (&out)[V]) const {
 #pragma unroll
@@ -131,11 +153,12 @@ struct Column {
   }
 };
 
-// Joins the composites of a workgroup's chunks, thread order = walking order for each column: on return `mine` is the composite of
-// everything BEFORE this thread's chunk, `total` of the whole workgroup.  Within a wave by shuffles over the chunks (lane = chunk * C + column
-// with C = 2^lanes_log2 columns), across waves through LDS.
+// Joins the composites of a workgroup's chunks, thread order = walking order for each column: on return `mine` is everything BEFORE this thread's
+// chunk, the carry included, and the carry has moved behind the last chunk if `more` is to come.  Within a wave by shuffles over its chunks
+// (lane = chunk * C + column with C = 2^lanes_log2 columns), across waves through LDS: a wave folds only the waves in front of it, the last one
+// folds the carry on.
 template <int V>
-__device__ __forceinline__ void join_chunks(Composite (&mine)[V], Composite (&total)[V], int lanes_log2, float2* lds) {
+__device__ __forceinline__ void join_chunks(Composite (&mine)[V], Composite (&carry)[V], bool more, int lanes_log2, float2* lds) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int columns = 1 << lanes_log2, column = lane & (columns - 1);
 #pragma unroll
@@ -144,27 +167,38 @@ __device__ __forceinline__ void join_chunks(Composite (&mine)[V], Composite (&to
       const Composite before = {__shfl_up(mine[j].a, d), __shfl_up(mine[j].b, d)};
       if (lane >= d) mine[j] = then(before, mine[j]);
     }
-    if (lane >= 64 - columns) lds[(wave * V + j) * columns + column] = make_float2(mine[j].a, mine[j].b);
+    if (lane >= 64 - columns) lds[((wave + 1) * V + j) * columns + column] = make_float2(mine[j].a, mine[j].b);
     const Composite before = {__shfl_up(mine[j].a, columns & 63), __shfl_up(mine[j].b, columns & 63)};
     mine[j] = lane >= columns ? before : Composite{1.0f, 0.0f};
   }
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    Composite all = {1.0f, 0.0f}, front = {1.0f, 0.0f};
-    for (int w = 0; w < waves; ++w) {
-      if (w == wave) front = all;
-      const float2 c = lds[(w * V + j) * columns + column];
-      all = then(all, {c.x, c.y});
+    Composite front = carry[j];
+    for (int w = 0; w < wave; ++w) {
+      const float2 c = lds[((w + 1) * V + j) * columns + column];
+      front = then(front, {c.x, c.y});
     }
-    total[j] = all;
     mine[j] = then(front, mine[j]);
+    if (more && wave == waves - 1 && lane >= 64 - columns) {
+      const float2 c = lds[(waves * V + j) * columns + column];
+      const Composite all = then(front, {c.x, c.y});
+      lds[j * columns + column] = make_float2(all.a, all.b);
+    }
   }
-  __syncthreads();
+  if (more) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float2 c = lds[j * columns + column];
+      carry[j] = {c.x, c.y};
+    }
+  }
 }
 
 template <typename E, int FORM, int V, int K, bool BACKWARD, int MODE>
 __global__ __launch_bounds__(MODE == kAlone ? 256 : 1024) void recurrence_columns(const RecurrenceParams P) {
+  static_assert(K <= kMostSteps, "the powers of a constant gate");
   extern __shared__ float2 lds[];
   const int columns = MODE == kAlone ? blockDim.x : 1 << P.lanes_log2;
   const int chunk = MODE == kAlone ? 0 : threadIdx.x >> P.lanes_log2;
@@ -178,11 +212,17 @@ __global__ __launch_bounds__(MODE == kAlone ? 256 : 1024) void recurrence_column
   col.nv = vector >= P.vectors ? 0 : static_cast<int>(P.inner - col.i < V ? P.inner - col.i : V);
   if (MODE == kAlone && col.nv == 0) return;
   const int64_t begin = segment * P.segment, end = begin + P.segment < P.steps ? begin + P.segment : P.steps;
+  constexpr bool kStates = !BACKWARD || (MODE != kComposites && FORM != kGateConstant);  // x and the states are looked at
 
-  float carry[V];
-  col.load_batch(P, BACKWARD ? P.dfinal : P.initial, carry);
+  Composite carry[V];  // a state (0, h), or - composites only - what the walk so far composes to
+  {
+    float h[V];
+    col.load_batch(P, BACKWARD ? P.dfinal : P.initial, h);
+#pragma unroll
+    for (int j = 0; j < V; ++j) carry[j] = MODE == kComposites ? Composite{1.0f, 0.0f} : Composite{0.0f, h[j]};
+  }
   if (MODE == kJoined && segment > 0) {  // the segments in front of this one: their composites, a contiguous run of them per chunk
-    Composite mine[V], total[V];
+    Composite mine[V];
     const int64_t run = (segment + chunks - 1) / chunks, from = chunk * run, to = from + run < segment ? from + run : segment;
 #pragma unroll
     for (int j = 0; j < V; ++j) mine[j] = {1.0f, 0.0f};
@@ -195,94 +235,98 @@ __global__ __launch_bounds__(MODE == kAlone ? 256 : 1024) void recurrence_column
         }
       }
     }
-    join_chunks<V>(mine, total, P.lanes_log2, lds);
-#pragma unroll
-    for (int j = 0; j < V; ++j) carry[j] = apply_step(total[j].a, carry[j], total[j].b);
+    join_chunks<V>(mine, carry, true, P.lanes_log2, lds);
   }
-  Composite whole[V];  // (kComposites)
-#pragma unroll
-  for (int j = 0; j < V; ++j) whole[j] = {1.0f, 0.0f};
 
-  for (int64_t base = begin; base < end; base += static_cast<int64_t>(chunks) * K) {
+  const int64_t tile = static_cast<int64_t>(chunks) * K;
+  for (int64_t base = begin; base < end; base += tile) {
     const int64_t s0 = base + static_cast<int64_t>(chunk) * K;
     const int n = col.nv == 0 || s0 >= end ? 0 : static_cast<int>(end - s0 < K ? end - s0 : K);
-    float x[K][V], f[K][V], inject[K][V], keep[K][V], up[BACKWARD ? K : 1][V], front[V];
+    float x[K][V], f[K][V], inject[K][V], up[BACKWARD ? K : 1][V], front[V], edge[V];
+    uint32_t cut[V];  // bit k: a reset at step k of the chunk
     // every load of the chunk first, then the arithmetic: K independent rows in flight
+    {
+      const E *px = col.at(P.x, s0), *pg = col.at(P.g, s0), *pd = col.at(P.dh, s0);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
+      for (int k = 0; k < K; ++k, px += P.x.st, pg += P.g.st, pd += P.dh.st) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[k][j] = f[k][j] = 0.0f;
-      if (k < n) {
-        if (!(BACKWARD && (MODE == kComposites || FORM == kGateConstant))) col.load(P.x, s0 + k, x[k]);
-        if (FORM != kGateConstant) col.load(P.g, s0 + k, f[k]);
-        if (BACKWARD) col.load(P.dh, s0 + k, up[k]);
-      }
-    }
-    float edge[V];  // the state in front of the chunk's last step (walking order of the backward pass: the one behind it)
-#pragma unroll
-    for (int j = 0; j < V; ++j) front[j] = 1.0f, edge[j] = 0.0f;
-    if (BACKWARD && n > 0) {
-      if (s0 > 0) {  // the gate that carries d into the chunk belongs to the step before
-        float g0[V] = {};
-        if (FORM != kGateConstant) col.load(P.g, s0 - 1, g0);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          float unused_f, unused_i;
-          gates<FORM>(g0[j], P.reset.p != nullptr && col.flag(P.reset, s0 - 1, j), P.constant, front[j], unused_f, unused_i);
+        for (int j = 0; j < V; ++j) x[k][j] = f[k][j] = 0.0f;
+        if (k < n) {
+          if (kStates) col.load(px, x[k]);
+          if (FORM != kGateConstant) col.load(pg, f[k]);
+          if (BACKWARD) col.load(pd, up[k]);
         }
       }
-      if (MODE != kComposites && FORM != kGateConstant) {
-        if (s0 + n < P.steps) col.load(P.h, s0 + n, edge);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) front[j] = 1.0f, edge[j] = 0.0f, cut[j] = 0;
+    if (BACKWARD && n > 0) {
+      // the gate that carries d into the chunk belongs to the step before it, the state in front of its last step to the step behind it
+      // (the backward pass walks from the end)
+      if (s0 > 0 && FORM != kGateConstant) col.load(col.at(P.g, s0 - 1), front);
+      if (kStates) {
+        if (s0 + n < P.steps) col.load(col.at(P.h, s0 + n), edge);
         else col.load_batch(P, P.initial, edge);
       }
     }
+    if (P.reset.p != nullptr) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (k < n && col.flag(P.reset, s0 + k, j)) cut[j] |= 1u << k;
+    }
+    if (BACKWARD && n > 0 && s0 > 0) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const bool reset = P.reset.p != nullptr && k < n && col.flag(P.reset, s0 + k, j);
-        gates<FORM>(f[k][j], reset, P.constant, keep[k][j], f[k][j], inject[k][j]);
+        float unused;
+        gate<FORM>(P, front[j], unused);
+        if (P.reset.p != nullptr && col.flag(P.reset, s0 - 1, j)) front[j] = 0.0f;
       }
     }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) gate<FORM>(P, f[k][j], inject[k][j]);
+    auto keep = [&](int k, int j) { return cut[j] >> k & 1 ? 0.0f : f[k][j]; };
+    auto factor = [&](int k, int j) { return !BACKWARD ? keep(k, j) : k == 0 ? front[j] : keep(k - 1, j); };  // what multiplies the carried value at step k
+    auto term = [&](int k, int j) { return BACKWARD ? up[k][j] : FORM == kGateLogit ? inject[k][j] * x[k][j] : x[k][j]; };
     float start[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) start[j] = carry[j];
+    for (int j = 0; j < V; ++j) start[j] = carry[j].b;
     if (MODE != kAlone) {
-      Composite mine[V], total[V];
+      Composite mine[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         mine[j] = {1.0f, 0.0f};
+        if (FORM == kGateConstant) {
+          bool dropped = false;
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const float m = BACKWARD ? (k == 0 ? front[j] : keep[k - 1][j]) : keep[k][j];
-          const float b = BACKWARD ? up[k][j] : inject[k][j] * x[k][j];
-          if (k < n) mine[j] = then(mine[j], {m, b});
-        }
-      }
-      join_chunks<V>(mine, total, P.lanes_log2, lds);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (MODE == kComposites) {
-          whole[j] = then(whole[j], total[j]);
+          for (int k = 0; k < K; ++k) {
+            if (k < n) mine[j].b = advance<FORM>(P, factor(k, j), mine[j].b, term(k, j));
+            if (k < n && factor(k, j) == 0.0f) dropped = true;
+          }
+          mine[j].a = dropped ? 0.0f : P.power[BACKWARD && s0 == 0 && n > 0 ? n - 1 : n];
         } else {
-          start[j] = apply_step(mine[j].a, carry[j], mine[j].b);
-          carry[j] = apply_step(total[j].a, carry[j], total[j].b);
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+            if (k < n) mine[j] = then(mine[j], {factor(k, j), term(k, j)});
         }
       }
+      join_chunks<V>(mine, carry, MODE == kComposites || base + tile < end, P.lanes_log2, lds);
+#pragma unroll
+      for (int j = 0; j < V; ++j) start[j] = mine[j].b;
     }
     if (MODE == kComposites) continue;
     if (!BACKWARD) {
+      E* ph = col.at(P.h, s0);
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
+      for (int k = 0; k < K; ++k, ph += P.h.st) {
         if (k < n) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) start[j] = apply_step(keep[k][j], start[j], inject[k][j] * x[k][j]);
-          col.store(P.h, s0 + k, start);
+          for (int j = 0; j < V; ++j) start[j] = advance<FORM>(P, keep(k, j), start[j], term(k, j));
+          col.store(ph, start);
         }
-      }
-      if (MODE == kAlone) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) carry[j] = start[j];
       }
       if (P.final_state != nullptr && n > 0 && s0 + n == P.steps) {
 #pragma unroll
@@ -290,53 +334,52 @@ __global__ __launch_bounds__(MODE == kAlone ? 256 : 1024) void recurrence_column
           if (j < col.nv) P.final_state[col.batch(P, j)] = start[j];
       }
     } else {
-      if (FORM != kGateConstant) {  // the states once more, in the order of the forward pass; `up` of step k keeps dh, x becomes what dg multiplies
+      if (kStates) {  // the states once more, in the order of the forward pass: x turns into what dg multiplies
 #pragma unroll
         for (int k = K - 1; k >= 0; --k) {
           if (k < n) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-              const bool dropped = P.reset.p != nullptr && col.flag(P.reset, s0 + k, j);
-              const float before = dropped ? 0.0f : edge[j];
-              const float value = x[k][j];
-              edge[j] = apply_step(keep[k][j], edge[j], inject[k][j] * value);
+              const float before = cut[j] >> k & 1 ? 0.0f : edge[j], value = x[k][j];
+              edge[j] = apply_step(keep(k, j), edge[j], inject[k][j] * value);
               x[k][j] = FORM == kGateLogit ? f[k][j] * inject[k][j] * (before - value) : before;
             }
           }
         }
       }
+      E *pdx = col.at(P.dx, s0), *pdg = col.at(P.dg, s0);
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
+      for (int k = 0; k < K; ++k, pdx += P.dx.st, pdg += P.dg.st) {
         if (k < n) {
           float out[V];
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            start[j] = apply_step(k == 0 ? front[j] : keep[k - 1][j], start[j], up[k][j]);
+            start[j] = advance<FORM>(P, factor(k, j), start[j], up[k][j]);
             out[j] = inject[k][j] * start[j];
           }
-          if (P.dx.p != nullptr) col.store(P.dx, s0 + k, out);
-          if (FORM != kGateConstant && P.dg.p != nullptr) {
+          if (P.dx.p != nullptr) col.store(pdx, out);
+          if (kStates && P.dg.p != nullptr) {
 #pragma unroll
             for (int j = 0; j < V; ++j) out[j] = x[k][j] * start[j];
-            col.store(P.dg, s0 + k, out);
+            col.store(pdg, out);
           }
           if (s0 + k + 1 == P.steps && P.dinitial != nullptr) {
 #pragma unroll
             for (int j = 0; j < V; ++j)
-              if (j < col.nv) P.dinitial[col.batch(P, j)] = keep[k][j] == 0.0f ? 0.0f : keep[k][j] * start[j];
+              if (j < col.nv) P.dinitial[col.batch(P, j)] = advance<FORM>(P, keep(k, j), start[j], 0.0f);
           }
         }
       }
-      if (MODE == kAlone) {
+    }
+    if (MODE == kAlone) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) carry[j] = start[j];
-      }
+      for (int j = 0; j < V; ++j) carry[j].b = start[j];
     }
   }
   if (MODE == kComposites && chunk == 0) {
 #pragma unroll
     for (int j = 0; j < V; ++j)
-      if (j < col.nv) P.composites[(segment * P.vectors + vector) * V + j] = make_float2(whole[j].a, whole[j].b);
+      if (j < col.nv) P.composites[(segment * P.vectors + vector) * V + j] = make_float2(carry[j].a, carry[j].b);
   }
 }
 
@@ -379,6 +422,16 @@ __device__ __forceinline__ void store_steps(E* row, int64_t st, int64_t s, int64
   }
 }
 
+// n steps of a constant gate without a reset, the power from the table
+template <int V>
+__device__ __forceinline__ Composite constant_run(const RecurrenceParams& P, int n, const float (&term)[V]) {
+  float b = 0.0f;
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    if (j < n) b = advance<kGateConstant>(P, P.constant, b, term[j]);
+  return {P.power[n], b};
+}
+
 // inclusive prefix of the composites over a group of 2^log2 lanes (UP: towards higher lanes), then the exclusive one; `total`: the whole group's
 template <bool UP>
 __device__ __forceinline__ void group_scan(Composite mine, int log2, Composite& exclusive, Composite& total) {
@@ -413,11 +466,12 @@ __global__ __launch_bounds__(256) void recurrence_rows(const RecurrenceParams P)
   const int64_t last = begin + P.segment < P.steps ? begin + P.segment : P.steps;  // (loop bound: the same for every group of a wave when segments == 1)
   auto at = [&](const Axis& t) { return static_cast<E*>(t.p) + o * t.so + i * t.si; };
   const uint8_t* reset = P.reset.p == nullptr ? nullptr : static_cast<const uint8_t*>(P.reset.p) + o * P.reset.so + i * P.reset.si;
-  const int64_t batch = P.batch_initial_swapped ? i * P.outer + o : o * P.inner + i;
+  const int64_t batch = P.batch_swapped ? i * P.outer + o : o * P.inner + i;
   const E *px = at(P.x), *pg = at(P.g), *ph = at(P.h), *pd = at(P.dh);
 
   const float* entering = BACKWARD ? P.dfinal : P.initial;
-  float carry = entering != nullptr && active ? entering[batch] : 0.0f;
+  constexpr bool kStates = !BACKWARD || (!COMPOSITES && FORM != kGateConstant);
+  Composite carry = COMPOSITES ? Composite{1.0f, 0.0f} : Composite{0.0f, entering != nullptr && active ? entering[batch] : 0.0f};
   if (!COMPOSITES && segment > 0) {  // (segments > 1: a group is a whole wave, so every lane takes the same way)
     Composite before = {1.0f, 0.0f};
     for (int64_t q = 0; q < segment; q += 64) {
@@ -429,102 +483,117 @@ __global__ __launch_bounds__(256) void recurrence_rows(const RecurrenceParams P)
       group_scan<true>(mine, log2, exclusive, total);
       before = then(before, total);
     }
-    carry = apply_step(before.a, carry, before.b);
+    carry = then(carry, before);
   }
   float keep_before = 1.0f;  // backward: the gate that carries d into this tile
   if (BACKWARD && begin > 0 && active) {
-    float f, in;
-    gates<FORM>(FORM == kGateConstant ? 0.0f : static_cast<float>(pg[(begin - 1) * P.g.st]), reset != nullptr && reset[(begin - 1) * P.reset.st] != 0, P.constant,
-                keep_before, f, in);
+    float unused;
+    if (FORM != kGateConstant) keep_before = static_cast<float>(pg[(begin - 1) * P.g.st]);
+    gate<FORM>(P, keep_before, unused);
+    if (reset != nullptr && reset[(begin - 1) * P.reset.st] != 0) keep_before = 0.0f;
   }
-  Composite whole = {1.0f, 0.0f};
 
-  for (int64_t base = begin; base < last; base += static_cast<int64_t>(width) * V) {
+  // what one tile reads; the next tile's is requested before this one is worked on
+  struct Tile {
+    float x[V], g[V], up[V], edge;
+    uint32_t cut;
+  };
+  const int64_t tile = static_cast<int64_t>(width) * V;
+  auto fetch = [&](int64_t base, Tile& t) {
     const int64_t s = base + static_cast<int64_t>(lane) * V;
-    float x[V], g[V] = {}, up[V] = {}, keep[V], inject[V];
-    if (!(BACKWARD && (COMPOSITES || FORM == kGateConstant))) load_steps<E, V>(px, P.x.st, s, end, x);
-    if (FORM != kGateConstant) load_steps<E, V>(pg, P.g.st, s, end, g);
-    if (BACKWARD) load_steps<E, V>(pd, P.dh.st, s, end, up);
-    bool dropped[V];
-    float edge = 0.0f;
-    const int64_t tile_end = base + static_cast<int64_t>(width) * V < end ? base + static_cast<int64_t>(width) * V : end;
-    if (BACKWARD && !COMPOSITES && FORM != kGateConstant && active && base < end) {
-      if (tile_end < P.steps) edge = static_cast<float>(ph[tile_end * P.h.st]);
-      else if (P.initial != nullptr) edge = P.initial[batch];
+    t.cut = 0;
+    t.edge = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) t.x[j] = t.g[j] = t.up[j] = 0.0f;
+    if (kStates) load_steps<E, V>(px, P.x.st, s, end, t.x);
+    if (FORM != kGateConstant) load_steps<E, V>(pg, P.g.st, s, end, t.g);
+    if (BACKWARD) load_steps<E, V>(pd, P.dh.st, s, end, t.up);
+    if (BACKWARD && kStates && base < end) {  // the state behind the tile (in front of it, for the forward order)
+      const int64_t behind = base + tile < end ? base + tile : end;
+      if (behind < P.steps) t.edge = static_cast<float>(ph[behind * P.h.st]);
+      else if (P.initial != nullptr) t.edge = P.initial[batch];
     }
+    if (reset != nullptr) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (s + j < end && reset[(s + j) * P.reset.st] != 0) t.cut |= 1u << j;
+    }
+  };
+  Tile t, next;
+  fetch(begin, t);
+  for (int64_t base = begin; base < last; base += tile, t = next) {
+    if (base + tile < last) fetch(base + tile, next);
+    const int64_t s = base + static_cast<int64_t>(lane) * V;
+    float keep[V], inject[V], term[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      dropped[j] = reset != nullptr && s + j < end && reset[(s + j) * P.reset.st] != 0;
-      float f;
-      gates<FORM>(g[j], dropped[j], P.constant, keep[j], f, inject[j]);
-      g[j] = f;
+      gate<FORM>(P, t.g[j], inject[j]);
+      keep[j] = t.cut >> j & 1 ? 0.0f : t.g[j];
       if (s + j >= end) keep[j] = 1.0f, inject[j] = 0.0f;  // steps behind the end change nothing
+      term[j] = FORM == kGateLogit ? inject[j] * t.x[j] : s + j < end ? t.x[j] : 0.0f;
     }
     if (!BACKWARD) {
       Composite mine = {1.0f, 0.0f}, exclusive, total;
 #pragma unroll
-      for (int j = 0; j < V; ++j) mine = then(mine, {keep[j], s + j < end ? inject[j] * x[j] : 0.0f});
+      for (int j = 0; j < V; ++j) mine = then(mine, {keep[j], term[j]});
+      if (FORM == kGateConstant && t.cut == 0 && s < end) mine = constant_run(P, s + V <= end ? V : static_cast<int>(end - s), term);
       group_scan<true>(mine, log2, exclusive, total);
-      if (COMPOSITES) {
-        whole = then(whole, total);
-        continue;
-      }
-      float h = apply_step(exclusive.a, carry, exclusive.b), out[V];
+      if (!COMPOSITES) {
+        float h = then(carry, exclusive).b, out[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (s + j < end) h = apply_step(keep[j], h, inject[j] * x[j]);
-        out[j] = h;
+        for (int j = 0; j < V; ++j) {
+          if (s + j < end) h = advance<FORM>(P, keep[j], h, term[j]);
+          out[j] = h;
+        }
+        store_steps<E, V>(at(P.h), P.h.st, s, end, out);
+        if (P.final_state != nullptr && s < P.steps && s + V >= P.steps && end == P.steps) P.final_state[batch] = h;
       }
-      store_steps<E, V>(at(P.h), P.h.st, s, end, out);
-      if (P.final_state != nullptr && s < P.steps && s + V >= P.steps && end == P.steps) P.final_state[batch] = h;
-      carry = apply_step(total.a, carry, total.b);
+      carry = then(carry, total);
     } else {
       // d: the gate in front of each step is its left neighbour's
       const float left = __shfl_up(keep[V - 1], 1, width);
       const float front = lane == 0 ? keep_before : left;
       Composite mine = {1.0f, 0.0f}, exclusive, total;
 #pragma unroll
-      for (int j = 0; j < V; ++j) mine = then(mine, s + j < end ? Composite{j == 0 ? front : keep[j - 1], up[j]} : Composite{1.0f, 0.0f});
+      for (int j = 0; j < V; ++j) mine = then(mine, s + j < end ? Composite{j == 0 ? front : keep[j - 1], t.up[j]} : Composite{1.0f, 0.0f});
       group_scan<true>(mine, log2, exclusive, total);
       keep_before = __shfl(keep[V - 1], width - 1, width);  // (read only when another tile follows, and then this one was full)
-      if (COMPOSITES) {
-        whole = then(whole, total);
-        continue;
-      }
-      float scale[V];
+      if (!COMPOSITES) {
+        float scale[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) scale[j] = 0.0f;
-      if (FORM != kGateConstant) {  // the states once more: forward order runs towards lower lanes
-        Composite states = {1.0f, 0.0f}, behind, unused;
+        for (int j = 0; j < V; ++j) scale[j] = 0.0f;
+        if (FORM != kGateConstant) {  // the states once more: forward order runs towards lower lanes
+          Composite states = {1.0f, 0.0f}, behind, unused;
 #pragma unroll
-        for (int j = V - 1; j >= 0; --j) states = then(states, {keep[j], s + j < end ? inject[j] * x[j] : 0.0f});
-        group_scan<false>(states, log2, behind, unused);
-        float h = apply_step(behind.a, edge, behind.b);
+          for (int j = V - 1; j >= 0; --j) states = then(states, {keep[j], term[j]});
+          group_scan<false>(states, log2, behind, unused);
+          float h = apply_step(behind.a, t.edge, behind.b);
 #pragma unroll
-        for (int j = V - 1; j >= 0; --j) {
-          if (s + j < end) {
-            const float before = dropped[j] ? 0.0f : h;
-            scale[j] = FORM == kGateLogit ? g[j] * inject[j] * (before - x[j]) : before;
-            h = apply_step(keep[j], h, inject[j] * x[j]);
+          for (int j = V - 1; j >= 0; --j) {
+            if (s + j < end) {
+              const float before = t.cut >> j & 1 ? 0.0f : h;
+              scale[j] = FORM == kGateLogit ? t.g[j] * inject[j] * (before - t.x[j]) : before;
+              h = apply_step(keep[j], h, term[j]);
+            }
           }
         }
-      }
-      float d = apply_step(exclusive.a, carry, exclusive.b), out[V], gate_out[V];
+        float d = then(carry, exclusive).b, out[V], gate_out[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (s + j < end) {
-          d = apply_step(j == 0 ? front : keep[j - 1], d, up[j]);
-          if (s + j + 1 == P.steps && P.dinitial != nullptr) P.dinitial[batch] = keep[j] == 0.0f ? 0.0f : keep[j] * d;
+        for (int j = 0; j < V; ++j) {
+          if (s + j < end) {
+            d = advance<FORM>(P, j == 0 ? front : keep[j - 1], d, t.up[j]);
+            if (s + j + 1 == P.steps && P.dinitial != nullptr) P.dinitial[batch] = advance<FORM>(P, keep[j], d, 0.0f);
+          }
+          out[j] = inject[j] * d;
+          gate_out[j] = scale[j] * d;
         }
-        out[j] = inject[j] * d;
-        gate_out[j] = scale[j] * d;
+        if (P.dx.p != nullptr) store_steps<E, V>(at(P.dx), P.dx.st, s, end, out);
+        if (FORM != kGateConstant && P.dg.p != nullptr) store_steps<E, V>(at(P.dg), P.dg.st, s, end, gate_out);
       }
-      if (P.dx.p != nullptr) store_steps<E, V>(at(P.dx), P.dx.st, s, end, out);
-      if (FORM != kGateConstant && P.dg.p != nullptr) store_steps<E, V>(at(P.dg), P.dg.st, s, end, gate_out);
-      carry = apply_step(total.a, carry, total.b);
+      carry = then(carry, total);
     }
   }
-  if (COMPOSITES && lane == 0 && active) P.composites[row * P.segments + segment] = make_float2(whole.a, whole.b);
+  if (COMPOSITES && lane == 0 && active) P.composites[row * P.segments + segment] = make_float2(carry.a, carry.b);
 }
 
 // ---- one step ----------------------------------------------------------------------------------------------------------------------
@@ -557,9 +626,9 @@ __global__ __launch_bounds__(256) void recurrence_step(const float* state, const
   for (int j = 0; j < V; ++j) {
     bool dropped = false;
     if (reset != nullptr && j < nv) dropped = reset[(at + j) / reset_columns * rs + (at + j) % reset_columns * rc] != 0;
-    float keep, f, inject;
-    gates<FORM>(gs[j], dropped, 0.0f, keep, f, inject);
-    const float next = apply_step(keep, h[j], inject * xs[j]);
+    float f = gs[j], inject = 1.0f;
+    if (FORM == kGateLogit) sigmoid_pair(gs[j], f, inject);
+    const float next = apply_step(dropped ? 0.0f : f, h[j], inject * xs[j]);
     sv.e[j] = next;
     ov.e[j] = static_cast<E>(next);
   }
@@ -576,6 +645,6 @@ __global__ __launch_bounds__(256) void recurrence_step(const float* state, const
 // one translation unit per element type (kernels_recurrence_*.hip): picks the instantiation and launches it
 template <typename E>
 int launch_recurrence(const RecurrenceParams& P, int form, bool backward, int which, unsigned blocks, unsigned threads, size_t lds, hipStream_t stream);
-enum : int { kColumnsScalar = 0, kColumnsVector = 4, kRows = 8 };  // + kAlone / kJoined / kComposites (rows: 1 = with, 2 = composites only)
+enum : int { kColumnsScalar = 0, kColumnsPair = 4, kColumnsWide = 8, kRows = 12 };  // + kAlone / kJoined / kComposites
 
 }  // namespace mbt_learning

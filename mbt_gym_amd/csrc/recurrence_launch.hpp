@@ -7,16 +7,12 @@ namespace mbt_learning {
 template <typename E>
 constexpr int kVector = 16 / static_cast<int>(sizeof(E));  // columns (or steps) of one 16-byte access
 
-// Rows of a chunk held in registers.  A thread of a 1024-thread workgroup has 128 registers: 16 elements of each of the four or five arrays it
-// keeps fit; a thread that walks alone (256-thread workgroups) takes twice as many, which is what keeps enough bytes in flight.
-template <int V, int MODE>
-constexpr int kChunk = V == 1 ? 16 : (MODE == kAlone ? 32 : 16) / V;
-
 template <typename E, int FORM, int V, bool BACKWARD>
 void (*columns_kernel(int mode))(RecurrenceParams) {
-  if (mode == kAlone) return recurrence_columns<E, FORM, V, kChunk<V, kAlone>, BACKWARD, kAlone>;
-  if (mode == kJoined) return recurrence_columns<E, FORM, V, kChunk<V, kJoined>, BACKWARD, kJoined>;
-  return recurrence_columns<E, FORM, V, kChunk<V, kJoined>, BACKWARD, kComposites>;
+  constexpr int kJoinedSteps = chunk_steps(FORM, BACKWARD, V, false), kAloneSteps = chunk_steps(FORM, BACKWARD, V, true);
+  if (mode == kAlone) return recurrence_columns<E, FORM, V, kAloneSteps, BACKWARD, kAlone>;
+  if (mode == kJoined) return recurrence_columns<E, FORM, V, kJoinedSteps, BACKWARD, kJoined>;
+  return recurrence_columns<E, FORM, V, kJoinedSteps, BACKWARD, kComposites>;
 }
 
 template <typename E, int FORM, bool BACKWARD>
@@ -25,7 +21,12 @@ void (*pick_recurrence(int which))(RecurrenceParams) {
     if (which - kRows == kComposites) return recurrence_rows<E, FORM, kVector<E>, BACKWARD, true>;
     return recurrence_rows<E, FORM, kVector<E>, BACKWARD, false>;
   }
-  if (which >= kColumnsVector) return columns_kernel<E, FORM, kVector<E>, BACKWARD>(which - kColumnsVector);
+  if constexpr (!BACKWARD) {
+    if (which == kColumnsWide + kAlone) return recurrence_columns<E, FORM, kVector<E>, chunk_steps(FORM, false, kVector<E>, true), false, kAlone>;
+  }
+  if constexpr (sizeof(E) == 2) {
+    if (which >= kColumnsPair) return columns_kernel<E, FORM, 2, BACKWARD>(which - kColumnsPair);
+  }
   return columns_kernel<E, FORM, 1, BACKWARD>(which - kColumnsScalar);
 }
 
