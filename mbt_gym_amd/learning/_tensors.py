@@ -23,16 +23,19 @@ def require(tensor, name, device=None, dtypes=None, shape=None):
     return tensor
 
 
-def where(device):
-    """(device ordinal, handle of torch's current stream there)"""
-    return device.index, torch.cuda.current_stream(device).cuda_stream
+def current_stream(index):
+    """The handle of torch's current stream on this device."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def dense_like(tensor):
     """An empty tensor of the same shape whose axes lie in memory in the same order, without gaps."""
-    order = sorted(range(tensor.dim()), key=lambda d: (-tensor.stride(d), d))
-    out = torch.empty([tensor.shape[d] for d in order], dtype=tensor.dtype, device=tensor.device)
-    back = [0] * tensor.dim()
-    for position, d in enumerate(order):
-        back[d] = position
-    return out.permute(back)
+    if tensor.is_contiguous():
+        return torch.empty_like(tensor)
+    strides = tensor.stride()
+    order = sorted(range(len(strides)), key=lambda d: (-strides[d], d))
+    shape, dense, run = tensor.shape, [0] * len(strides), 1
+    for d in reversed(order):
+        dense[d] = run
+        run *= shape[d]
+    return torch.empty_strided(shape, dense, dtype=tensor.dtype, device=tensor.device)

@@ -2,7 +2,6 @@
 
 The rewards-to-go of the reference's learner (mbt_gym/agents/PolicyGradientAgent.py:69-73) are the recurrence walked backwards with a constant
 gate; the state of a recurrent actor is the one with learnt gates.  Kernels, splits and what bounds them: csrc/recurrence.hpp."""
-import ctypes
 import math
 from typing import Optional, Union
 
@@ -10,77 +9,86 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from mbt_gym_amd import _native
-from mbt_gym_amd.learning._tensors import DTYPES, dense_like, require, where
+from mbt_gym_amd.learning._tensors import DTYPES, current_stream, dense_like, require
 
 
-def _batch_axes(tensors, axis):
+def _batch_groups(shape, axis, strides):
     """The batch dimensions (all but `axis`) as at most two groups of neighbours that are one stride apart in EVERY tensor: [(size, last dim)]
     ordered outer, inner; or None when they do not fold into two."""
-    shape = tensors[0].shape
     groups = []
-    for d in range(len(shape)):
-        if d == axis or shape[d] == 1:
+    for d, size in enumerate(shape):
+        if d == axis or size == 1:
             continue
-        if groups and all(t.stride(groups[-1][1]) == t.stride(d) * shape[d] for t in tensors):
-            groups[-1] = (groups[-1][0] * shape[d], d)
-        else:
-            groups.append((shape[d], d))
+        if groups:
+            before, last = groups[-1]
+            if all(s[last] == s[d] * size for s in strides):
+                groups[-1] = (before * size, d)
+                continue
+        groups.append((size, d))
     return groups if len(groups) <= 2 else None
 
 
-class _Call:
-    """One call's tensors as struct mbt_recurrence sees them: arrays of (outer, time, inner)."""
+def _array(tensor, axis, groups):
+    """struct mbt_array3 of a tensor: its address and its strides along (outer, time, inner)"""
+    s = tensor.stride()
+    outer, inner = (s[groups[0][1]], s[groups[1][1]]) if len(groups) == 2 else (0, s[groups[0][1]] if groups else 0)
+    return _native.MbtArray3(tensor.data_ptr(), (outer, s[axis], inner))
 
-    def __init__(self, tensors, axis):
+
+def _launch(entry, struct, backward, index):
+    """The call itself, with the workspace it asks for (torch's, on the stream the call works on)."""
+    lib = _native.load_library()
+    size = lib.mbt_recurrence_workspace(struct, backward)
+    if size:
+        workspace = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", index))
+        struct.workspace, struct.workspace_bytes = workspace.data_ptr(), size
+    code = entry(index, struct, current_stream(index))
+    if code < 0:
+        _native.check(code)
+
+
+class _Plan:
+    """One call's operands in the order the library sees them: (outer, time, inner).  The forward call builds it, the backward call fills it on."""
+
+    def __init__(self, inputs, gate, initial, reset, axis, form, constant, reverse):
         self.axis = axis
-        self.groups = _batch_axes(list(tensors.values()), axis)
-        if self.groups is None:  # (batch axes that do not fold: copies that do)
-            tensors = {name: t.contiguous() for name, t in tensors.items()}
-            self.groups = _batch_axes(list(tensors.values()), axis)
-        self.tensors = tensors  # (kept: the copies live until the launch)
-        first = next(iter(tensors.values()))
-        sizes = [1] * (2 - len(self.groups)) + [size for size, _ in self.groups]
-        self.struct = _native.MbtRecurrence(outer=sizes[0], steps=first.shape[axis], inner=sizes[1], dtype=DTYPES[first.dtype])
-        for name, t in tensors.items():
-            array = getattr(self.struct, name)
-            array.data = t.data_ptr()
-            strides = [0] * (2 - len(self.groups)) + [t.stride(d) for _, d in self.groups]
-            array.stride[0], array.stride[1], array.stride[2] = strides[0], t.stride(axis), strides[1]
+        states = dense_like(inputs)
+        given = [t for t in (inputs, gate, reset) if t is not None]
+        groups = _batch_groups(inputs.shape, axis, [t.stride() for t in given + [states]])
+        if groups is None:  # (batch axes that do not fold: copies that do)
+            inputs, gate, reset = (None if t is None else t.contiguous() for t in (inputs, gate, reset))
+            states = torch.empty_like(inputs)
+            groups = _batch_groups(inputs.shape, axis, [states.stride()])
+        self.inputs, self.gate, self.initial, self.reset, self.states, self.groups = inputs, gate, initial, reset, states, groups
+        self.final = torch.empty([n for d, n in enumerate(inputs.shape) if d != axis], dtype=torch.float32, device=inputs.device)
+        r = self.struct = _native.MbtRecurrence(groups[0][0] if len(groups) == 2 else 1, inputs.shape[axis], groups[-1][0] if groups else 1,
+                                                DTYPES[inputs.dtype], form, reverse, 0, constant)
+        r.inputs, r.states = _array(inputs, axis, groups), _array(states, axis, groups)
+        if gate is not None:
+            r.gate = _array(gate, axis, groups)
+        if reset is not None:
+            r.reset = _array(reset, axis, groups)
+        if initial is not None:
+            r.initial = initial.data_ptr()
+        r.final_state = self.final.data_ptr()
 
-    def run(self, entry, backward, device):
-        lib = _native.load_library()
-        size = lib.mbt_recurrence_workspace(ctypes.byref(self.struct), int(backward))
-        workspace = None
-        if size:
-            workspace = torch.empty(size, dtype=torch.uint8, device=device)
-            self.struct.workspace, self.struct.workspace_bytes = workspace.data_ptr(), size
-        index, stream = where(device)
-        _native.check(getattr(lib, entry)(index, ctypes.byref(self.struct), stream))
+    def forward(self):
+        _launch(_native.load_library().mbt_recurrence_forward, self.struct, 0, self.states.device.index)
+        return self.states, self.final
 
 
-def _forward(inputs, gate, initial, reset, axis, form, constant, reverse):
-    states = dense_like(inputs)
-    final = torch.empty([n for d, n in enumerate(inputs.shape) if d != axis], dtype=torch.float32, device=inputs.device)
-    tensors = {"inputs": inputs, "states": states}
-    if gate is not None:
-        tensors["gate"] = gate
-    if reset is not None:
-        tensors["reset"] = reset
-    call = _Call(tensors, axis)
-    call.struct.form, call.struct.constant, call.struct.reverse = form, constant, int(reverse)
-    call.struct.initial = None if initial is None else initial.data_ptr()
-    call.struct.final_state = final.data_ptr()
-    call.run("mbt_recurrence_forward", False, inputs.device)
-    return call.tensors["states"], final
+def _forward(*arguments):
+    return _Plan(*arguments).forward()
 
 
 class _LinearRecurrence(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, inputs, gate, initial, reset, axis, form, constant, reverse):
-        states, final = _forward(inputs, gate, initial, reset, axis, form, constant, reverse)
-        ctx.save_for_backward(*((None, None, initial, reset, None) if gate is None else (inputs, gate, initial, reset, states)))
-        ctx.settings = (axis, form, constant, reverse)
-        ctx.shape, ctx.dtype = inputs.shape, inputs.dtype
+    def forward(ctx, *arguments):
+        plan = _Plan(*arguments)
+        states, final = plan.forward()
+        ctx.save_for_backward(*((None, None, plan.initial, plan.reset, None) if plan.gate is None else (plan.inputs, plan.gate, plan.initial, plan.reset, states)))
+        ctx.axis, ctx.groups, ctx.struct = plan.axis, plan.groups, plan.struct
+        ctx.shape, ctx.strides, ctx.dtype, ctx.device = states.shape, states.stride(), states.dtype, states.device
         ctx.set_materialize_grads(False)
         return states, final
 
@@ -88,40 +96,40 @@ class _LinearRecurrence(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_states, grad_final):
         inputs, gate, initial, reset, states = ctx.saved_tensors
-        axis, form, constant, reverse = ctx.settings
         if grad_states is None and grad_final is None:
             return (None,) * 8
-        if grad_states is None:
-            grad_states = torch.zeros(ctx.shape, dtype=ctx.dtype, device=grad_final.device) if states is None else torch.zeros_like(states)
-        layout = inputs if inputs is not None else grad_states
-        if states is not None and grad_states.stride() != states.stride():  # (an expanded or transposed gradient: one copy, then the fast layout)
-            grad_states = torch.empty_like(states).copy_(grad_states)
-        elif states is None and not (grad_states.is_contiguous() or grad_states.stride(axis) == 1):
-            grad_states = grad_states.contiguous()
-        tensors = {"grad_states": grad_states}
+        axis, groups = ctx.axis, ctx.groups
+        if grad_states is None or grad_states.stride() != ctx.strides:  # (an expanded or transposed gradient: one copy, then the states' layout)
+            given, grad_states = grad_states, torch.empty_strided(ctx.shape, ctx.strides, dtype=ctx.dtype, device=ctx.device)
+            grad_states.zero_() if given is None else grad_states.copy_(given)
+        # a struct of this call's own - a graph may be walked more than once - with the addresses of what autograd kept: hooks may have moved it
+        r = _native.MbtRecurrence.from_buffer_copy(ctx.struct)
+        r.workspace, r.workspace_bytes, r.final_state = None, 0, None
+        dense = r.states
         if gate is not None:
-            tensors.update(inputs=inputs, gate=gate, states=states)
+            r.inputs, r.gate, r.states = _array(inputs, axis, groups), _array(gate, axis, groups), _array(states, axis, groups)
         if reset is not None:
-            tensors["reset"] = reset
+            r.reset = _array(reset, axis, groups)
+        if initial is not None:
+            r.initial = initial.data_ptr()
+        r.grad_states = dense
+        r.grad_states.data = grad_states.data_ptr()
         grads = [None, None, None]
         if ctx.needs_input_grad[0]:
-            grads[0] = tensors["grad_inputs"] = dense_like(layout)
-        if gate is not None and ctx.needs_input_grad[1]:
-            grads[1] = tensors["grad_gate"] = dense_like(layout)
-        if initial is not None and ctx.needs_input_grad[2]:
+            grads[0] = torch.empty_like(grad_states)
+            r.grad_inputs = dense
+            r.grad_inputs.data = grads[0].data_ptr()
+        if ctx.needs_input_grad[1]:
+            grads[1] = torch.empty_like(grad_states)
+            r.grad_gate = dense
+            r.grad_gate.data = grads[1].data_ptr()
+        if ctx.needs_input_grad[2]:
             grads[2] = torch.empty_like(initial)
-        call = _Call(tensors, axis)
-        call.struct.form, call.struct.constant, call.struct.reverse = form, constant, int(reverse)
-        call.struct.initial = None if initial is None else initial.data_ptr()
+            r.grad_initial = grads[2].data_ptr()
         if grad_final is not None:
             grad_final = grad_final.contiguous()
-            call.struct.grad_final = grad_final.data_ptr()
-        if grads[2] is not None:
-            call.struct.grad_initial = grads[2].data_ptr()
-        call.run("mbt_recurrence_backward", True, grad_states.device)
-        for position, name in ((0, "grad_inputs"), (1, "grad_gate")):
-            if grads[position] is not None:
-                grads[position] = call.tensors[name]
+            r.grad_final = grad_final.data_ptr()
+        _launch(_native.load_library().mbt_recurrence_backward, r, 1, ctx.device.index)
         return (grads[0], grads[1], grads[2], None, None, None, None, None)
 
 
@@ -169,7 +177,7 @@ def linear_recurrence(inputs: torch.Tensor, gate: Union[float, torch.Tensor], in
         return (states, final) if return_final else states
     tracked = torch.is_grad_enabled() and (inputs.requires_grad or (gate is not None and gate.requires_grad) or (initial is not None and initial.requires_grad))
     run = _LinearRecurrence.apply if tracked else _forward
-    states, final = run(inputs, gate, initial, reset, axis, form, constant, bool(reverse))
+    states, final = run(inputs, gate, initial, reset, axis, form, constant, int(bool(reverse)))
     return (states, final) if return_final else states
 
 
@@ -202,10 +210,10 @@ def linear_recurrence_step(state: torch.Tensor, inputs: torch.Tensor, gate: torc
         folded = reset.reshape(rows, columns)
         flags, row_stride, column_stride = folded.data_ptr(), folded.stride(0), folded.stride(1)
     inputs, gate = inputs.contiguous(), gate.contiguous()
-    index, stream = where(inputs.device)
+    index = inputs.device.index
     _native.check(_native.load_library().mbt_recurrence_step(
         index, DTYPES[inputs.dtype], _native.GATE_LOGIT if gate_is_logit else _native.GATE_VALUE, rows, columns, state.data_ptr(), inputs.data_ptr(),
-        gate.data_ptr(), flags or None, row_stride, column_stride, out.data_ptr(), new_state.data_ptr(), stream))
+        gate.data_ptr(), flags or None, row_stride, column_stride, out.data_ptr(), new_state.data_ptr(), current_stream(index)))
     return out, new_state
 
 
