@@ -731,6 +731,42 @@ int mbt_recurrence_backward(int device, const mbt_recurrence* r, void* stream);
 int mbt_recurrence_step(int device, int dtype, int form, uint64_t rows, uint64_t columns, const float* state, const void* inputs, const void* gate,
                         const uint8_t* reset, int64_t reset_row_stride, int64_t reset_column_stride, void* out, float* new_state, void* stream);
 
+/* The policy-gradient loss of recorded actions with its gradient (PG:49-62, where the entropy is left out):
+ *   loss = - mean over the rows that `mask` keeps and the components of  [ weight log N(action | mean, std) + entropy_weight H(std) ]
+ * with H(std) = log std + log(2 pi e) / 2.  Rows are (outer, inner); a row's `actions` (1 .. 8) components are contiguous.  A masked row counts for
+ * nothing whatever its values, NaN too, and has a gradient of zero; without any row the loss and the gradients are zero. */
+enum { MBT_STD_NUMBER = 0, MBT_STD_COMPONENT = 1, MBT_STD_FULL = 2 };
+typedef struct mbt_array2 {
+  void* data;         /* NULL = absent, where that is allowed */
+  int64_t stride[2];  /* in elements, along (outer, inner) */
+} mbt_array2;
+typedef struct mbt_policy_loss {
+  uint64_t outer, inner;    /* both at least 1 */
+  int32_t actions;          /* components of a row */
+  int32_t dtype;            /* of mean, grad_mean, and of std and grad_std when there is one per row */
+  int32_t std_kind;         /* one number / float32 per component / one per row and component */
+  int32_t gradients_ready;  /* backward: the gradient arrays hold what the forward call wrote, i.e. the gradients for *grad_loss == 1 */
+  double std;               /* MBT_STD_NUMBER */
+  double entropy_weight;
+  mbt_array2 mean;
+  mbt_array2 action;        /* float32 */
+  mbt_array2 weight;        /* float32, one per row */
+  mbt_array2 mask;          /* bytes, one per row; absent = every row counts */
+  mbt_array2 std_array;     /* MBT_STD_COMPONENT: `actions` float32 (strides ignored), MBT_STD_FULL: as mean */
+  float* loss;              /* forward output: one float32 */
+  double* sums;             /* MBT_POLICY_LOSS_SUMS doubles: forward output, backward input */
+  mbt_array2 grad_mean;     /* outputs of both calls, each may be absent: the forward call writes the gradients for a loss gradient of one */
+  mbt_array2 grad_std;      /* MBT_STD_COMPONENT: `actions` float32, MBT_STD_FULL: as mean */
+  const float* grad_loss;   /* backward input: one float32 ON THE DEVICE */
+  void* workspace;
+  uint64_t workspace_bytes; /* forward: at least what mbt_policy_loss_workspace says */
+} mbt_policy_loss;
+#define MBT_POLICY_LOSS_SUMS 10
+uint64_t mbt_policy_loss_workspace(const mbt_policy_loss* p);
+int mbt_policy_loss_forward(int device, const mbt_policy_loss* p, void* stream);
+/* Writes the gradients for *grad_loss.  With gradients_ready and *grad_loss == 1 - decided on the device - it touches nothing. */
+int mbt_policy_loss_backward(int device, const mbt_policy_loss* p, void* stream);
+
 /* ---- timing on the environment's stream (HIP events) ------------------------------------------- */
 int mbt_env_timer_begin(mbt_env* env);
 int mbt_env_timer_end(mbt_env* env, float* elapsed_ms); /* = stop + elapsed: synchronises */

@@ -212,6 +212,26 @@ class MbtRecurrence(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
 
 
+STD_NUMBER, STD_COMPONENT, STD_FULL = 0, 1, 2
+POLICY_LOSS_SUMS = 10
+
+
+class MbtArray2(C.Structure):
+    """struct mbt_array2 (include/mbt_env.h): strides in elements along (outer, inner)."""
+
+    _fields_ = [("data", C.c_void_p), ("stride", C.c_int64 * 2)]
+
+
+class MbtPolicyLoss(C.Structure):
+    """struct mbt_policy_loss (include/mbt_env.h)."""
+
+    _fields_ = [("outer", C.c_uint64), ("inner", C.c_uint64), ("actions", C.c_int32), ("dtype", C.c_int32), ("std_kind", C.c_int32),
+                ("gradients_ready", C.c_int32), ("std", C.c_double), ("entropy_weight", C.c_double),
+                ("mean", MbtArray2), ("action", MbtArray2), ("weight", MbtArray2), ("mask", MbtArray2), ("std_array", MbtArray2),
+                ("loss", C.c_void_p), ("sums", C.c_void_p), ("grad_mean", MbtArray2), ("grad_std", MbtArray2), ("grad_loss", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
 class NativeError(RuntimeError):
     """A libmbtenv call returned a negative status."""
 
@@ -312,6 +332,9 @@ SIGNATURES = {
     "mbt_recurrence_backward": (C.c_int, [C.c_int, C.POINTER(MbtRecurrence), C.c_void_p]),
     "mbt_recurrence_step": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_uint64, C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                       C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "mbt_policy_loss_workspace": (C.c_uint64, [C.POINTER(MbtPolicyLoss)]),
+    "mbt_policy_loss_forward": (C.c_int, [C.c_int, C.POINTER(MbtPolicyLoss), C.c_void_p]),
+    "mbt_policy_loss_backward": (C.c_int, [C.c_int, C.POINTER(MbtPolicyLoss), C.c_void_p]),
     "mbt_env_timer_begin": (C.c_int, [_ENV]),
     "mbt_env_timer_end": (C.c_int, [_ENV, C.POINTER(C.c_float)]),
     "mbt_env_timer_stop": (C.c_int, [_ENV]),

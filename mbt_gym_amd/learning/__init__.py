@@ -2,9 +2,11 @@
 neighbours, behind the C ABI of include/mbt_env.h):
 
   linear_recurrence, linear_recurrence_step, rewards_to_go     the gated linear recurrence along the time axis of a recording
+  policy_gradient_loss                                         the loss of recorded actions, with its gradient
 
 Every function takes CUDA tensors only (there is no CPU path), works on the current stream of the tensors' device, allocates its outputs and
 workspaces from torch and never synchronises, so it may be captured into a `torch.cuda.graph`."""
+from mbt_gym_amd.learning.policy_loss import policy_gradient_loss
 from mbt_gym_amd.learning.recurrence import linear_recurrence, linear_recurrence_step, rewards_to_go
 
-__all__ = ["linear_recurrence", "linear_recurrence_step", "rewards_to_go"]
+__all__ = ["linear_recurrence", "linear_recurrence_step", "policy_gradient_loss", "rewards_to_go"]

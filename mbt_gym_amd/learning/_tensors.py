@@ -39,3 +39,19 @@ def dense_like(tensor):
         dense[d] = run
         run *= shape[d]
     return torch.empty_strided(shape, dense, dtype=tensor.dtype, device=tensor.device)
+
+
+def batch_groups(shape, axis, strides):
+    """The batch dimensions (all but `axis`) as at most two groups of neighbours that are one stride apart in EVERY tensor: [(size, last dim)]
+    ordered outer, inner; or None when they do not fold into two."""
+    groups = []
+    for d, size in enumerate(shape):
+        if d == axis or size == 1:
+            continue
+        if groups:
+            before, last = groups[-1]
+            if all(s[last] == s[d] * size for s in strides):
+                groups[-1] = (before * size, d)
+                continue
+        groups.append((size, d))
+    return groups if len(groups) <= 2 else None

@@ -9,23 +9,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from mbt_gym_amd import _native
-from mbt_gym_amd.learning._tensors import DTYPES, current_stream, dense_like, require
-
-
-def _batch_groups(shape, axis, strides):
-    """The batch dimensions (all but `axis`) as at most two groups of neighbours that are one stride apart in EVERY tensor: [(size, last dim)]
-    ordered outer, inner; or None when they do not fold into two."""
-    groups = []
-    for d, size in enumerate(shape):
-        if d == axis or size == 1:
-            continue
-        if groups:
-            before, last = groups[-1]
-            if all(s[last] == s[d] * size for s in strides):
-                groups[-1] = (before * size, d)
-                continue
-        groups.append((size, d))
-    return groups if len(groups) <= 2 else None
+from mbt_gym_amd.learning._tensors import DTYPES, batch_groups, current_stream, dense_like, require
 
 
 def _array(tensor, axis, groups):
@@ -54,11 +38,11 @@ class _Plan:
         self.axis = axis
         states = dense_like(inputs)
         given = [t for t in (inputs, gate, reset) if t is not None]
-        groups = _batch_groups(inputs.shape, axis, [t.stride() for t in given + [states]])
+        groups = batch_groups(inputs.shape, axis, [t.stride() for t in given + [states]])
         if groups is None:  # (batch axes that do not fold: copies that do)
             inputs, gate, reset = (None if t is None else t.contiguous() for t in (inputs, gate, reset))
             states = torch.empty_like(inputs)
-            groups = _batch_groups(inputs.shape, axis, [states.stride()])
+            groups = batch_groups(inputs.shape, axis, [states.stride()])
         self.inputs, self.gate, self.initial, self.reset, self.states, self.groups = inputs, gate, initial, reset, states, groups
         self.final = torch.empty([n for d, n in enumerate(inputs.shape) if d != axis], dtype=torch.float32, device=inputs.device)
         r = self.struct = _native.MbtRecurrence(groups[0][0] if len(groups) == 2 else 1, inputs.shape[axis], groups[-1][0] if groups else 1,

@@ -96,3 +96,39 @@ def assert_within(got, expected, bound, what):
     if off.size:
         worst = np.unravel_index(np.argmax(np.where(np.isnan(off), np.inf, off)), off.shape)
         assert off[worst] <= 0.0, (what, worst, got[worst], expected[worst], bound[worst])
+
+
+class PolicyLoss:
+    """rows x components in float64; std a number, (A,) or rows x components; mask bool over rows or None.  Bounds: z = (a - mean) / std carries four
+    roundings, its square nine, the logarithm two ulps; a row is summed in float32, the rows in float64; one rounding at the end."""
+
+    def __init__(self, mean, actions, weights, std, mask=None, entropy_weight=0.0, dtype="float32", grad_loss=1.0):
+        mean, actions = np.asarray(mean, np.float64), np.asarray(actions, np.float64)
+        keep = np.ones(mean.shape[:-1], bool) if mask is None else np.asarray(mask, bool)
+        clean = lambda a, fill: np.where(keep[..., None], a, fill)  # noqa: E731
+        w = clean(np.asarray(weights, np.float64)[..., None], 0.0)
+        mean, actions = clean(mean, 0.0), clean(actions, 0.0)
+        full = np.ndim(std) > 1
+        sigma = np.broadcast_to(np.asarray(std, np.float64), mean.shape)
+        sigma = clean(sigma, 1.0) if full else sigma
+        n = keep.sum() * mean.shape[-1]
+        c = float(np.float32(entropy_weight))
+        v, tiny = HALF_STEP[dtype], HALF_SUBNORMAL[dtype]
+        z = (actions - mean) / sigma
+        log_prob, entropy = -0.5 * z * z - np.log(sigma) - 0.5 * np.log(2 * np.pi), np.log(sigma) + 0.5 * np.log(2 * np.pi * np.e)
+        value = clean(w * log_prob + c * entropy, 0.0)
+        size = clean(np.abs(w) * (0.5 * z * z + np.abs(np.log(sigma)) + 1.0) + abs(c) * (np.abs(np.log(sigma)) + 1.5), 0.0)
+        scale = grad_loss / n if n else 0.0
+        self.loss = -value.sum() / n if n else 0.0
+        self.loss_bound = (16 + mean.shape[-1]) * U * size.sum() / max(n, 1) + U * abs(self.loss)
+        self.grad_mean = -scale * w * z / sigma
+        self.grad_mean_bound = (12 * U + v) * np.abs(self.grad_mean) + tiny
+        each = clean((w * (z * z - 1.0) + c) / sigma, 0.0)
+        each_bound = clean(16 * U * (np.abs(w) * (z * z + 1.0) + abs(c)) / sigma, 0.0)
+        if full:
+            self.grad_std = -scale * each
+            self.grad_std_bound = abs(scale) * each_bound + (4 * U + v) * np.abs(self.grad_std) + tiny
+        else:
+            axes = tuple(range(mean.ndim - 1))
+            self.grad_std = -scale * each.sum(axis=axes)
+            self.grad_std_bound = abs(scale) * each_bound.sum(axis=axes) + 4 * U * np.abs(self.grad_std)

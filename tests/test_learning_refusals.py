@@ -121,3 +121,58 @@ def test_tensors_that_are_not_on_the_device_are_refused():
         learning.linear_recurrence([1.0, 2.0], 0.5)
     with pytest.raises(ValueError, match="discount"):
         learning.rewards_to_go(x, 1.5)
+
+
+# ---- the policy-gradient loss ------------------------------------------------------------------------------------------------------------
+def loss_struct(**changes):
+    p = _native.MbtPolicyLoss(outer=3, inner=5, actions=2, dtype=_native.FLOAT32, std_kind=_native.STD_NUMBER, std=0.1, loss=4096, sums=4096, grad_loss=4096)
+    for name in ("mean", "action", "weight"):
+        array = getattr(p, name)
+        array.data, array.stride[0], array.stride[1] = 4096, 10, 2
+    for name, value in changes.items():
+        setattr(p, name, value)
+    return p
+
+
+def test_policy_loss_struct_layout(tmp_path):
+    offsets_match(_native.MbtArray2, "mbt_array2", tmp_path)
+    offsets_match(_native.MbtPolicyLoss, "mbt_policy_loss", tmp_path)
+
+
+def test_the_library_refuses_a_malformed_policy_loss(lib):
+    def forward(**changes):
+        return lib.mbt_policy_loss_forward(0, C.byref(loss_struct(**changes)), None)
+
+    refused(lib, lib.mbt_policy_loss_forward(0, None, None), "null argument")
+    refused(lib, forward(dtype=5), "dtype 5")
+    refused(lib, forward(std_kind=3), "std_kind 3")
+    for n in (0, 9):
+        refused(lib, forward(actions=n), f"{n} action components")
+    for sizes in ((0, 1), (1, 0), (1 << 41, 1), (1 << 30, 1 << 30)):
+        refused(lib, forward(outer=sizes[0], inner=sizes[1]), "2^40")
+    for name in ("mean", "action", "weight"):
+        p = loss_struct()
+        getattr(p, name).data = None
+        refused(lib, lib.mbt_policy_loss_forward(0, C.byref(p), None), "are needed")
+    refused(lib, forward(sums=None), "sums")
+    refused(lib, forward(loss=None), "needs loss")
+    refused(lib, forward(std_kind=_native.STD_FULL), "std_array")
+    for std in (0.0, -1.0, float("nan"), float("inf")):
+        refused(lib, forward(std=std), "positive")
+    refused(lib, forward(entropy_weight=float("nan")), "entropy_weight")
+    p = loss_struct()
+    p.grad_std.data = 4096
+    refused(lib, lib.mbt_policy_loss_forward(0, C.byref(p), None), "no gradient array")
+    size = lib.mbt_policy_loss_workspace(C.byref(loss_struct()))
+    assert size > 0
+    refused(lib, forward(), f"{size} are needed")
+    refused(lib, forward(workspace=4096, workspace_bytes=size - 1), f"{size} are needed")
+    refused(lib, forward(workspace=4100, workspace_bytes=size), "aligned")
+    refused(lib, lib.mbt_policy_loss_backward(0, C.byref(loss_struct(grad_loss=None)), None), "needs grad_loss")
+
+
+def test_a_policy_loss_off_the_device_is_refused():
+    from mbt_gym_amd import learning
+
+    with pytest.raises(ValueError, match="no CPU path"):
+        learning.policy_gradient_loss(torch.randn(3, 2), torch.randn(3, 2), torch.randn(3), 0.1)
