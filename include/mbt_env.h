@@ -767,6 +767,21 @@ int mbt_policy_loss_forward(int device, const mbt_policy_loss* p, void* stream);
 /* Writes the gradients for *grad_loss.  With gradients_ready and *grad_loss == 1 - decided on the device - it touches nothing. */
 int mbt_policy_loss_backward(int device, const mbt_policy_loss* p, void* stream);
 
+/* Orthogonalised updates, for a learner that steps along them instead of along the gradient (the Muon optimiser): with X = G / (|G| + eps), |G| the
+ * Frobenius norm, `steps` Newton-Schulz products X <- a X + (b X X^T + c (X X^T)^2) X (a matrix with more rows than columns is turned).
+ * float32 accuracy for every element type.  The coefficients have to keep singular values that start within [0, 1] below 1.9. */
+typedef struct mbt_matrix {
+  const void* in;
+  void* out;                       /* may be `in` itself with the same strides */
+  uint32_t rows, columns;          /* 1 .. 32768 */
+  uint64_t batch;                  /* matrices of this shape, at least 1 */
+  int64_t in_stride[3];            /* in elements, along (batch, row, column) */
+  int64_t out_stride[3];
+} mbt_matrix;
+uint64_t mbt_orthogonalise_workspace(uint32_t count, const mbt_matrix* matrices);
+int mbt_orthogonalise(int device, int dtype, uint32_t count, const mbt_matrix* matrices, int steps, const double coefficients[3], double eps,
+                      void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* ---- timing on the environment's stream (HIP events) ------------------------------------------- */
 int mbt_env_timer_begin(mbt_env* env);
 int mbt_env_timer_end(mbt_env* env, float* elapsed_ms); /* = stop + elapsed: synchronises */

@@ -232,6 +232,13 @@ class MbtPolicyLoss(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
 
 
+class MbtMatrix(C.Structure):
+    """struct mbt_matrix (include/mbt_env.h): strides in elements along (batch, row, column)."""
+
+    _fields_ = [("in_", C.c_void_p), ("out", C.c_void_p), ("rows", C.c_uint32), ("columns", C.c_uint32), ("batch", C.c_uint64),
+                ("in_stride", C.c_int64 * 3), ("out_stride", C.c_int64 * 3)]
+
+
 class NativeError(RuntimeError):
     """A libmbtenv call returned a negative status."""
 
@@ -335,6 +342,9 @@ SIGNATURES = {
     "mbt_policy_loss_workspace": (C.c_uint64, [C.POINTER(MbtPolicyLoss)]),
     "mbt_policy_loss_forward": (C.c_int, [C.c_int, C.POINTER(MbtPolicyLoss), C.c_void_p]),
     "mbt_policy_loss_backward": (C.c_int, [C.c_int, C.POINTER(MbtPolicyLoss), C.c_void_p]),
+    "mbt_orthogonalise_workspace": (C.c_uint64, [C.c_uint32, C.POINTER(MbtMatrix)]),
+    "mbt_orthogonalise": (C.c_int, [C.c_int, C.c_int, C.c_uint32, C.POINTER(MbtMatrix), C.c_int, C.POINTER(C.c_double), C.c_double, C.c_void_p,
+                                    C.c_uint64, C.c_void_p]),
     "mbt_env_timer_begin": (C.c_int, [_ENV]),
     "mbt_env_timer_end": (C.c_int, [_ENV, C.POINTER(C.c_float)]),
     "mbt_env_timer_stop": (C.c_int, [_ENV]),

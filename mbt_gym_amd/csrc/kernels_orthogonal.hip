@@ -1,0 +1,236 @@
+// The C entry point of the Newton-Schulz orthogonalisation: argument checks, how a list of matrices is cut into launches (kernels: orthogonal.hpp).
+#include <atomic>
+#include <cmath>
+
+#include "orthogonal.hpp"
+
+namespace mbt_learning {
+namespace {
+
+constexpr uint32_t kMostSize = 32768;
+
+int64_t padded(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+bool is_small(const mbt_matrix& m) { return m.rows <= kSmall && m.columns <= kSmall; }
+
+// 128 x 128 tiles read every operand half as often as 64 x 64 ones and need four times as large a matrix to occupy the chip
+int tile_of(const mbt_matrix& m) {
+  const int64_t small = m.rows < m.columns ? m.rows : m.columns, large = m.rows < m.columns ? m.columns : m.rows;
+  return (padded(small, 128) / 128) * (padded(large, 128) / 128) * static_cast<int64_t>(m.batch) >= 192 ? 128 : 64;
+}
+
+MatrixGroup group_of(const mbt_matrix& m, int tile) {
+  MatrixGroup g{};
+  const bool turn = m.rows > m.columns;
+  g.in = m.in;
+  g.out = m.out;
+  g.in_batch = m.in_stride[0];
+  g.in_row = m.in_stride[turn ? 2 : 1];
+  g.in_column = m.in_stride[turn ? 1 : 2];
+  g.out_batch = m.out_stride[0];
+  g.out_row = m.out_stride[turn ? 2 : 1];
+  g.out_column = m.out_stride[turn ? 1 : 2];
+  g.m = static_cast<int32_t>(turn ? m.columns : m.rows);
+  g.n = static_cast<int32_t>(turn ? m.rows : m.columns);
+  g.mp = static_cast<int32_t>(padded(g.m, tile));
+  g.np = static_cast<int32_t>(padded(g.n, tile));
+  g.batch = static_cast<int64_t>(m.batch);
+  g.stride = 6 * static_cast<int64_t>(g.mp) * g.np + 4 * static_cast<int64_t>(g.mp) * g.mp;  // (orthogonal.hpp: Planes)
+  return g;
+}
+
+int check_matrices(uint32_t count, const mbt_matrix* matrices) {
+  if (count < 1 || matrices == nullptr) return mbt_set_error(MBT_ERR_INVALID, "no matrices");
+  uint64_t total = 0;
+  for (uint32_t k = 0; k < count; ++k) {
+    const mbt_matrix& m = matrices[k];
+    if (m.in == nullptr || m.out == nullptr) return mbt_set_error(MBT_ERR_INVALID, "matrix %u: null argument", k);
+    if (m.rows < 1 || m.columns < 1 || m.rows > kMostSize || m.columns > kMostSize)
+      return mbt_set_error(MBT_ERR_INVALID, "matrix %u is %u x %u: rows and columns lie within 1 .. %u", k, m.rows, m.columns, kMostSize);
+    if (m.batch < 1 || m.batch > (uint64_t{1} << 24)) return mbt_set_error(MBT_ERR_INVALID, "matrix %u: a batch of %llu lies outside 1 .. 2^24", k, (unsigned long long)m.batch);
+    const MatrixGroup g = group_of(m, 128);
+    total += m.batch * static_cast<uint64_t>(g.mp) * g.np / 4096;
+    if (total > (uint64_t{1} << 28)) return mbt_set_error(MBT_ERR_INVALID, "more elements than one call takes (2^40)");
+  }
+  return MBT_OK;
+}
+
+// the tile that the large matrices of the call share (one launch works on all of them), and the halfs and partial sums they need
+int common_tile(uint32_t count, const mbt_matrix* matrices) {
+  int tile = 64;
+  for (uint32_t k = 0; k < count; ++k)
+    if (!is_small(matrices[k]) && tile_of(matrices[k]) > tile) tile = 128;
+  return tile;
+}
+uint64_t workspace_of(uint32_t count, const mbt_matrix* matrices) {
+  uint64_t bytes = 0;
+  const int tile = common_tile(count, matrices);
+  for (uint32_t k = 0; k < count; ++k) {
+    if (is_small(matrices[k])) continue;
+    const MatrixGroup g = group_of(matrices[k], tile);
+    bytes += matrices[k].batch * (static_cast<uint64_t>(g.stride) * sizeof(_Float16) + kNormBlocks * sizeof(double));
+  }
+  return bytes;
+}
+
+// Singular values start within [0, 1]: what the largest can become, step by step (a grid fine enough for a polynomial of degree five, and 1 % on top).
+bool bounded(int steps, const double c[3]) {
+  double top = 1.0;
+  for (int s = 0; s < steps; ++s) {
+    double next = 0.0;
+    for (int k = 0; k <= 2048; ++k) {
+      const double x = top * k / 2048, y = x * x, q = c[0] + c[1] * y + c[2] * y * y;
+      if (!(std::fabs(q) < 7.9)) return false;
+      if (std::fabs(x * q) > next) next = std::fabs(x * q);
+    }
+    top = next * 1.01;
+    if (!(top < 1.9)) return false;
+  }
+  return true;
+}
+
+template <typename E, int T>
+int run_products(OrthogonaliseParams& P, int64_t gram_tiles, int64_t apply_tiles, const int64_t (&gram_first)[kMostGroups], const int64_t (&apply_first)[kMostGroups],
+                 hipStream_t stream) {
+  constexpr size_t lds = 2 * 4 * T * 40 * sizeof(_Float16);
+  auto launch = [&](auto kernel, int64_t tiles, const int64_t (&first)[kMostGroups]) {
+    for (int g = 0; g < P.groups; ++g) P.group[g].first = first[g];
+    P.blocks = tiles;
+    kernel<<<static_cast<unsigned>((tiles + 7) / 8 * 8), 256, lds, stream>>>(P);
+  };
+  P.odd = 0;
+  for (int step = 0; step < P.steps; ++step) {
+    P.last = step + 1 == P.steps;
+    launch(orthogonalise_product<E, T, kGram>, gram_tiles, gram_first);
+    launch(orthogonalise_product<E, T, kPolynomial>, gram_tiles, gram_first);
+    launch(orthogonalise_product<E, T, kApply>, apply_tiles, apply_first);
+    P.odd ^= 1;
+  }
+  return launch_status("orthogonalise");
+}
+
+template <typename E>
+int run(uint32_t count, const mbt_matrix* matrices, OrthogonaliseParams& P, void* workspace, hipStream_t stream) {
+  // small ones: kMostGroups shapes a launch
+  P.groups = 0;
+  P.odd = 0;
+  int64_t blocks = 0;
+  auto flush_small = [&]() {
+    if (P.groups == 0) return static_cast<int>(MBT_OK);
+    orthogonalise_small<E><<<static_cast<unsigned>(blocks), 256, kSmallLds, stream>>>(P);
+    P.groups = 0;
+    blocks = 0;
+    return launch_status("orthogonalise");
+  };
+  for (uint32_t k = 0; k < count; ++k) {
+    if (!is_small(matrices[k])) continue;
+    MatrixGroup& g = P.group[P.groups++];
+    g = group_of(matrices[k], 32);
+    g.first = blocks;
+    blocks += g.batch;
+    if (P.groups == kMostGroups) {
+      const int rc = flush_small();
+      if (rc != MBT_OK) return rc;
+    }
+  }
+  int rc = flush_small();
+  if (rc != MBT_OK) return rc;
+
+  const int tile = common_tile(count, matrices);
+  char* next = static_cast<char*>(workspace);
+  uint32_t k = 0;
+  while (k < count) {
+    int64_t matrices_in = 0, split_tiles = 0, gram_tiles = 0, apply_tiles = 0, halfs = 0;
+    int64_t norm_first[kMostGroups] = {}, split_first[kMostGroups] = {}, gram_first[kMostGroups] = {}, apply_first[kMostGroups] = {};
+    P.groups = 0;
+    P.odd = 0;
+    for (; k < count && P.groups < kMostGroups; ++k) {
+      if (is_small(matrices[k])) continue;
+      const int at = P.groups++;
+      MatrixGroup& g = P.group[at];
+      g = group_of(matrices[k], tile);
+      g.planes = halfs;
+      halfs += g.batch * g.stride;
+      const int64_t rows = g.mp / tile, columns = g.np / tile;
+      norm_first[at] = matrices_in;
+      split_first[at] = split_tiles;
+      gram_first[at] = gram_tiles;
+      apply_first[at] = apply_tiles;
+      matrices_in += g.batch;
+      split_tiles += g.batch * (g.mp / 64) * (g.np / 64);
+      gram_tiles += g.batch * (rows * (rows + 1) / 2);
+      apply_tiles += g.batch * rows * columns;
+    }
+    if (P.groups == 0) break;
+    if (split_tiles > 0x7fffff00 || matrices_in * kNormBlocks > 0x7fffff00) return mbt_set_error(MBT_ERR_INVALID, "more matrices than one launch takes");
+    P.partials = reinterpret_cast<double*>(next);
+    next += matrices_in * kNormBlocks * sizeof(double);
+    P.planes = reinterpret_cast<_Float16*>(next);
+    next += halfs * sizeof(_Float16);
+    for (int g = 0; g < P.groups; ++g) P.group[g].first = norm_first[g];
+    orthogonalise_norms<E><<<static_cast<unsigned>(matrices_in * kNormBlocks), 256, 0, stream>>>(P);
+    for (int g = 0; g < P.groups; ++g) P.group[g].first = split_first[g];
+    orthogonalise_split<E><<<static_cast<unsigned>(split_tiles), 256, 0, stream>>>(P);
+    rc = tile == 128 ? run_products<E, 128>(P, gram_tiles, apply_tiles, gram_first, apply_first, stream)
+                     : run_products<E, 64>(P, gram_tiles, apply_tiles, gram_first, apply_first, stream);
+    if (rc != MBT_OK) return rc;
+  }
+  return MBT_OK;
+}
+
+// the kernels' shared memory is beyond the 64 KB that a launch gets unasked; set once per device
+template <typename E>
+int allow_lds(int device) {
+  static std::atomic<uint64_t> done{0};
+  if (device < 64 && (done.load(std::memory_order_relaxed) >> device & 1)) return MBT_OK;
+  LEARNING_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(orthogonalise_small<E>), hipFuncAttributeMaxDynamicSharedMemorySize, kSmallLds));
+  const int lds = 2 * 4 * 128 * 40 * static_cast<int>(sizeof(_Float16));
+  LEARNING_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(orthogonalise_product<E, 128, kGram>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  LEARNING_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(orthogonalise_product<E, 128, kPolynomial>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  LEARNING_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(orthogonalise_product<E, 128, kApply>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  if (device < 64) done.fetch_or(1ull << device, std::memory_order_relaxed);
+  return MBT_OK;
+}
+
+}  // namespace
+}  // namespace mbt_learning
+
+extern "C" {
+
+uint64_t mbt_orthogonalise_workspace(uint32_t count, const mbt_matrix* matrices) {
+  using namespace mbt_learning;
+  return check_matrices(count, matrices) == MBT_OK ? workspace_of(count, matrices) : 0;
+}
+
+int mbt_orthogonalise(int device, int dtype, uint32_t count, const mbt_matrix* matrices, int steps, const double coefficients[3], double eps, void* workspace,
+                      uint64_t workspace_bytes, void* stream) {
+  using namespace mbt_learning;
+  if (!dtype_known(dtype)) return mbt_set_error(MBT_ERR_INVALID, "dtype %d: float32, bfloat16 and float16 are known", dtype);
+  int rc = check_matrices(count, matrices);
+  if (rc != MBT_OK) return rc;
+  if (steps < 1 || steps > 64) return mbt_set_error(MBT_ERR_INVALID, "%d steps: 1 .. 64 are taken", steps);
+  if (coefficients == nullptr || !bounded(steps, coefficients))
+    return mbt_set_error(MBT_ERR_INVALID, "the coefficients let singular values grow beyond 1.9 (or are not numbers)");
+  if (!(eps >= 0.0 && std::isfinite(eps))) return mbt_set_error(MBT_ERR_INVALID, "eps = %g: it has to be a finite number, not negative", eps);
+  const uint64_t needed = workspace_of(count, matrices);
+  if (needed > 0 && (workspace == nullptr || workspace_bytes < needed))
+    return mbt_set_error(MBT_ERR_INVALID, "the workspace has %llu bytes; %llu are needed (mbt_orthogonalise_workspace)",
+                         (unsigned long long)(workspace == nullptr ? 0 : workspace_bytes), (unsigned long long)needed);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return mbt_set_error(MBT_ERR_INVALID, "the workspace is not aligned to 16 bytes");
+  DeviceScope scope;
+  rc = scope.enter(device);
+  if (rc != MBT_OK) return rc;
+  rc = dtype == MBT_FLOAT32 ? allow_lds<float>(device) : dtype == MBT_BFLOAT16 ? allow_lds<bfloat16>(device) : allow_lds<float16>(device);
+  if (rc != MBT_OK) return rc;
+  OrthogonaliseParams P{};
+  P.steps = steps;
+  P.a = static_cast<float>(coefficients[0]);
+  P.b = static_cast<float>(coefficients[1]);
+  P.c = static_cast<float>(coefficients[2]);
+  P.eps = eps;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == MBT_FLOAT32) return run<float>(count, matrices, P, workspace, s);
+  if (dtype == MBT_BFLOAT16) return run<bfloat16>(count, matrices, P, workspace, s);
+  return run<float16>(count, matrices, P, workspace, s);
+}
+
+}  // extern "C"

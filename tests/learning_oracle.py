@@ -132,3 +132,36 @@ class PolicyLoss:
             axes = tuple(range(mean.ndim - 1))
             self.grad_std = -scale * each.sum(axis=axes)
             self.grad_std_bound = abs(scale) * each_bound.sum(axis=axes) + 4 * U * np.abs(self.grad_std)
+
+
+def orthogonalise(g, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """(the formula in float64, a bound on the Frobenius norm of a float32-accurate evaluation's error).
+
+    The bound follows the errors through the products.  Operands are good to 2^-21 (two float16 numbers and the product of their low parts that is left
+    out), sums of k terms are float32: a product L R^T is off by at most e_k |L|_F |R|_F with e_k = 2^-20 + k U in Frobenius norm (the classical bound, k
+    the terms of a sum).  One step maps singular values by f(s) = a s + b s^3 + c s^5; in the singular vectors' basis its derivative multiplies the entries of
+    an error by the divided differences (f(s) - f(t)) / (s - t) and (f(s) + f(t)) / (s + t), all at most max |f'| over [0, |X|_2], so an error is passed on
+    at most that many times in Frobenius norm, and the step adds those of its three products and of the split results.  The classical bound takes
+    every rounding at its worst and all of one sign; a sum of k terms is off by a random walk, sqrt(k) instead of k, with overwhelming probability,
+    and that is used here: e_k = 2^-20 + 4 sqrt(k) U."""
+    a, b, c = coefficients
+    x = np.asarray(g, np.float64)
+    turned = x.shape[0] > x.shape[1]
+    x = x.T if turned else x
+    m, n = x.shape
+    x = x / (np.sqrt((x * x).sum()) + eps)
+    frob = np.linalg.norm
+    en, em = 2.0 ** -20 + 4 * np.sqrt(n) * U, 2.0 ** -20 + 4 * np.sqrt(m) * U
+    error = 4 * U * frob(x)
+    for _ in range(steps):
+        gram = x @ x.T
+        q = a * np.eye(m) + b * gram + c * (gram @ gram)
+        s = np.linalg.norm(x, 2)
+        gram_error = en * frob(x) * s + 2 * U * frob(gram)
+        square_error = em * frob(gram) * s * s
+        q_error = (abs(b) + 2 * abs(c) * s * s) * gram_error + abs(c) * square_error + 4 * U * (frob(b * gram) + frob(c * gram @ gram) + abs(a) * np.sqrt(m))
+        apply_error = em * frob(q @ x) + em * frob(x) * np.linalg.norm(q, 2)
+        grid = np.linspace(0.0, s, 2001) ** 2
+        error = error * np.abs(a + 3 * b * grid + 5 * c * grid * grid).max() + q_error * s + apply_error
+        x = q @ x
+    return (x.T if turned else x), error

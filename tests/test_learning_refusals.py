@@ -176,3 +176,63 @@ def test_a_policy_loss_off_the_device_is_refused():
 
     with pytest.raises(ValueError, match="no CPU path"):
         learning.policy_gradient_loss(torch.randn(3, 2), torch.randn(3, 2), torch.randn(3), 0.1)
+
+
+# ---- the orthogonalisation --------------------------------------------------------------------------------------------------------------
+def test_matrix_struct_layout(tmp_path):
+    source = {"in_": "in"}
+    fields = [f for f, _ in _native.MbtMatrix._fields_]
+    body = "".join(f'  printf("{f} %zu\\n", offsetof(mbt_matrix, {source.get(f, f)}));\n' for f in fields)
+    path = tmp_path / "matrix.c"
+    path.write_text(f'#include <stdio.h>\n#include <stddef.h>\n#include "{HEADER}"\nint main(void) {{\n  printf("sizeof %zu\\n", sizeof(mbt_matrix));\n{body}  return 0; }}\n')
+    subprocess.run(["gcc", "-std=c11", "-Wall", "-Werror", str(path), "-o", str(tmp_path / "matrix")], check=True)
+    out = dict(line.split() for line in subprocess.run([str(tmp_path / "matrix")], check=True, capture_output=True, text=True).stdout.splitlines())
+    assert int(out.pop("sizeof")) == C.sizeof(_native.MbtMatrix)
+    assert all(getattr(_native.MbtMatrix, f).offset == int(o) for f, o in out.items())
+
+
+def matrix(rows=100, columns=90, batch=1, given=4096, out=4096):
+    m = _native.MbtMatrix(in_=given, out=out, rows=rows, columns=columns, batch=batch)
+    m.in_stride[:] = m.out_stride[:] = (rows * columns, columns, 1)
+    return m
+
+
+def test_the_library_refuses_malformed_matrices(lib):
+    good = (C.c_double * 3)(3.4445, -4.7750, 2.0315)
+
+    def call(*matrices, dtype=0, steps=5, coefficients=good, eps=1e-7, workspace=None, size=0, count=None):
+        array = (_native.MbtMatrix * max(1, len(matrices)))(*matrices)
+        return lib.mbt_orthogonalise(0, dtype, len(matrices) if count is None else count, array, steps, coefficients, eps, workspace, size, None)
+
+    refused(lib, call(matrix(), dtype=9), "dtype 9")
+    refused(lib, call(), "no matrices")
+    refused(lib, lib.mbt_orthogonalise(0, 0, 1, None, 5, good, 1e-7, None, 0, None), "no matrices")
+    refused(lib, call(matrix(), matrix(given=None)), "matrix 1: null argument")
+    refused(lib, call(matrix(out=None)), "null argument")
+    for bad in (matrix(rows=0), matrix(columns=0), matrix(rows=32769)):
+        refused(lib, call(bad), "1 .. 32768")
+    refused(lib, call(matrix(batch=0)), "batch of 0")
+    refused(lib, call(matrix(rows=32768, columns=32768, batch=1 << 20)), "more elements")
+    for steps in (0, -1, 65):
+        refused(lib, call(matrix(), steps=steps), f"{steps} steps")
+    for c in ((4.5, 0.0, 0.0), (1.0, 2.0, 0.0), (float("inf"), 0.0, 0.0), (0.0, float("nan"), 0.0)):
+        refused(lib, call(matrix(), coefficients=(C.c_double * 3)(*c)), "1.9")
+    refused(lib, call(matrix(), coefficients=None), "1.9")
+    for eps in (-1.0, float("nan"), float("inf")):
+        refused(lib, call(matrix(), eps=eps), "eps")
+    size = lib.mbt_orthogonalise_workspace(1, matrix())
+    assert size > 0 and lib.mbt_orthogonalise_workspace(1, matrix(64, 64)) == 0
+    refused(lib, call(matrix()), f"{size} are needed")
+    refused(lib, call(matrix(), workspace=4096, size=size - 1), f"{size} are needed")
+    refused(lib, call(matrix(), workspace=4104, size=size), "aligned")
+
+
+def test_updates_off_the_device_are_refused():
+    from mbt_gym_amd import learning
+
+    with pytest.raises(ValueError, match="no CPU path"):
+        learning.orthogonalise(torch.randn(3, 2))
+    parameter = torch.nn.Parameter(torch.randn(3, 2))
+    parameter.grad = torch.ones(3, 2)
+    with pytest.raises(ValueError, match="no CPU path"):
+        learning.Muon([parameter]).step()
