@@ -10,7 +10,11 @@ namespace {
 constexpr uint32_t kMostSize = 32768;
 
 int64_t padded(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
-bool is_small(const mbt_matrix& m) { return m.rows <= kSmall && m.columns <= kSmall; }
+enum Kind { kSmallMatrix, kFlatMatrix, kLargeMatrix };
+Kind kind_of(const mbt_matrix& m) {
+  const uint32_t small = m.rows < m.columns ? m.rows : m.columns, large = m.rows < m.columns ? m.columns : m.rows;
+  return large <= kSmall ? kSmallMatrix : small <= kSmall ? kFlatMatrix : kLargeMatrix;
+}
 
 // 128 x 128 tiles read every operand half as often as 64 x 64 ones and need four times as large a matrix to occupy the chip
 int tile_of(const mbt_matrix& m) {
@@ -31,10 +35,18 @@ MatrixGroup group_of(const mbt_matrix& m, int tile) {
   g.out_column = m.out_stride[turn ? 1 : 2];
   g.m = static_cast<int32_t>(turn ? m.columns : m.rows);
   g.n = static_cast<int32_t>(turn ? m.rows : m.columns);
-  g.mp = static_cast<int32_t>(padded(g.m, tile));
-  g.np = static_cast<int32_t>(padded(g.n, tile));
   g.batch = static_cast<int64_t>(m.batch);
-  g.stride = 6 * static_cast<int64_t>(g.mp) * g.np + 4 * static_cast<int64_t>(g.mp) * g.mp;  // (orthogonal.hpp: Planes)
+  const Kind kind = kind_of(m);
+  if (kind == kLargeMatrix) {
+    g.mp = static_cast<int32_t>(padded(g.m, tile));
+    g.np = static_cast<int32_t>(padded(g.n, tile));
+    g.stride = 6 * static_cast<int64_t>(g.mp) * g.np + 4 * static_cast<int64_t>(g.mp) * g.mp;  // halfs (orthogonal.hpp: Planes)
+  } else {
+    g.mp = static_cast<int32_t>(padded(g.m, 16));
+    g.np = static_cast<int32_t>(padded(g.n, kind == kSmallMatrix ? 16 : 64));
+    g.shares = g.np / 64 < kMostShares ? g.np / 64 : kMostShares;
+    g.stride = 64 * static_cast<int64_t>(g.np) + 2 * kMostShares * 4096;  // floats (orthogonal.hpp: orthogonalise_flat)
+  }
   return g;
 }
 
@@ -48,7 +60,7 @@ int check_matrices(uint32_t count, const mbt_matrix* matrices) {
       return mbt_set_error(MBT_ERR_INVALID, "matrix %u is %u x %u: rows and columns lie within 1 .. %u", k, m.rows, m.columns, kMostSize);
     if (m.batch < 1 || m.batch > (uint64_t{1} << 24)) return mbt_set_error(MBT_ERR_INVALID, "matrix %u: a batch of %llu lies outside 1 .. 2^24", k, (unsigned long long)m.batch);
     const MatrixGroup g = group_of(m, 128);
-    total += m.batch * static_cast<uint64_t>(g.mp) * g.np / 4096;
+    total += m.batch * (static_cast<uint64_t>(g.mp) * g.np / 4096 + 1);
     if (total > (uint64_t{1} << 28)) return mbt_set_error(MBT_ERR_INVALID, "more elements than one call takes (2^40)");
   }
   return MBT_OK;
@@ -58,16 +70,17 @@ int check_matrices(uint32_t count, const mbt_matrix* matrices) {
 int common_tile(uint32_t count, const mbt_matrix* matrices) {
   int tile = 64;
   for (uint32_t k = 0; k < count; ++k)
-    if (!is_small(matrices[k]) && tile_of(matrices[k]) > tile) tile = 128;
+    if (kind_of(matrices[k]) == kLargeMatrix && tile_of(matrices[k]) > tile) tile = 128;
   return tile;
 }
 uint64_t workspace_of(uint32_t count, const mbt_matrix* matrices) {
   uint64_t bytes = 0;
   const int tile = common_tile(count, matrices);
   for (uint32_t k = 0; k < count; ++k) {
-    if (is_small(matrices[k])) continue;
+    const Kind kind = kind_of(matrices[k]);
+    if (kind == kSmallMatrix) continue;
     const MatrixGroup g = group_of(matrices[k], tile);
-    bytes += matrices[k].batch * (static_cast<uint64_t>(g.stride) * sizeof(_Float16) + kNormBlocks * sizeof(double));
+    bytes += matrices[k].batch * (static_cast<uint64_t>(g.stride) * (kind == kFlatMatrix ? sizeof(float) : sizeof(_Float16)) + kNormBlocks * sizeof(double));
   }
   return bytes;
 }
@@ -109,72 +122,96 @@ int run_products(OrthogonaliseParams& P, int64_t gram_tiles, int64_t apply_tiles
 }
 
 template <typename E>
-int run(uint32_t count, const mbt_matrix* matrices, OrthogonaliseParams& P, void* workspace, hipStream_t stream) {
-  // small ones: kMostGroups shapes a launch
+int run_small(uint32_t count, const mbt_matrix* matrices, OrthogonaliseParams& P, hipStream_t stream) {
   P.groups = 0;
-  P.odd = 0;
   int64_t blocks = 0;
-  auto flush_small = [&]() {
-    if (P.groups == 0) return static_cast<int>(MBT_OK);
-    orthogonalise_small<E><<<static_cast<unsigned>(blocks), 256, kSmallLds, stream>>>(P);
-    P.groups = 0;
-    blocks = 0;
-    return launch_status("orthogonalise");
-  };
-  for (uint32_t k = 0; k < count; ++k) {
-    if (!is_small(matrices[k])) continue;
-    MatrixGroup& g = P.group[P.groups++];
-    g = group_of(matrices[k], 32);
-    g.first = blocks;
-    blocks += g.batch;
-    if (P.groups == kMostGroups) {
-      const int rc = flush_small();
+  for (uint32_t k = 0; k <= count; ++k) {
+    if (k < count) {
+      if (kind_of(matrices[k]) != kSmallMatrix) continue;
+      MatrixGroup& g = P.group[P.groups++];
+      g = group_of(matrices[k], 0);
+      g.first = blocks;
+      blocks += g.batch;
+    }
+    if (P.groups == kMostGroups || (k == count && P.groups > 0)) {
+      if (blocks > 0x7fffff00) return mbt_set_error(MBT_ERR_INVALID, "more matrices than one launch takes");
+      orthogonalise_small<E><<<static_cast<unsigned>(blocks), 1024, kSmallLds, stream>>>(P);
+      const int rc = launch_status("orthogonalise");
       if (rc != MBT_OK) return rc;
+      P.groups = 0;
+      blocks = 0;
     }
   }
-  int rc = flush_small();
-  if (rc != MBT_OK) return rc;
+  return MBT_OK;
+}
 
-  const int tile = common_tile(count, matrices);
-  char* next = static_cast<char*>(workspace);
+// Flat and large matrices, kMostGroups shapes at a time; `next` walks through the workspace.
+template <typename E>
+int run_kind(Kind kind, uint32_t count, const mbt_matrix* matrices, int tile, OrthogonaliseParams& P, char*& next, hipStream_t stream) {
   uint32_t k = 0;
   while (k < count) {
-    int64_t matrices_in = 0, split_tiles = 0, gram_tiles = 0, apply_tiles = 0, halfs = 0;
-    int64_t norm_first[kMostGroups] = {}, split_first[kMostGroups] = {}, gram_first[kMostGroups] = {}, apply_first[kMostGroups] = {};
+    int64_t matrices_in = 0, split_tiles = 0, gram_tiles = 0, apply_tiles = 0, elements = 0, shares = 0;
+    int64_t norm_first[kMostGroups] = {}, split_first[kMostGroups] = {}, gram_first[kMostGroups] = {}, apply_first[kMostGroups] = {}, share_first[kMostGroups] = {};
     P.groups = 0;
     P.odd = 0;
+    P.last = 0;
     for (; k < count && P.groups < kMostGroups; ++k) {
-      if (is_small(matrices[k])) continue;
+      if (kind_of(matrices[k]) != kind) continue;
       const int at = P.groups++;
       MatrixGroup& g = P.group[at];
       g = group_of(matrices[k], tile);
-      g.planes = halfs;
-      halfs += g.batch * g.stride;
+      g.planes = elements;
+      elements += g.batch * g.stride;
       const int64_t rows = g.mp / tile, columns = g.np / tile;
       norm_first[at] = matrices_in;
       split_first[at] = split_tiles;
       gram_first[at] = gram_tiles;
       apply_first[at] = apply_tiles;
+      share_first[at] = shares;
       matrices_in += g.batch;
       split_tiles += g.batch * (g.mp / 64) * (g.np / 64);
       gram_tiles += g.batch * (rows * (rows + 1) / 2);
       apply_tiles += g.batch * rows * columns;
+      shares += g.batch * g.shares;
     }
     if (P.groups == 0) break;
-    if (split_tiles > 0x7fffff00 || matrices_in * kNormBlocks > 0x7fffff00) return mbt_set_error(MBT_ERR_INVALID, "more matrices than one launch takes");
+    if (split_tiles > 0x7fffff00 || shares > 0x7fffff00 || matrices_in > 0x7fffff00 / kNormBlocks) return mbt_set_error(MBT_ERR_INVALID, "more matrices than one launch takes");
     P.partials = reinterpret_cast<double*>(next);
     next += matrices_in * kNormBlocks * sizeof(double);
     P.planes = reinterpret_cast<_Float16*>(next);
-    next += halfs * sizeof(_Float16);
-    for (int g = 0; g < P.groups; ++g) P.group[g].first = norm_first[g];
+    next += elements * (kind == kFlatMatrix ? sizeof(float) : sizeof(_Float16));
+    auto place = [&](const int64_t (&first)[kMostGroups]) {
+      for (int g = 0; g < P.groups; ++g) P.group[g].first = first[g];
+    };
+    place(norm_first);
     orthogonalise_norms<E><<<static_cast<unsigned>(matrices_in * kNormBlocks), 256, 0, stream>>>(P);
-    for (int g = 0; g < P.groups; ++g) P.group[g].first = split_first[g];
-    orthogonalise_split<E><<<static_cast<unsigned>(split_tiles), 256, 0, stream>>>(P);
-    rc = tile == 128 ? run_products<E, 128>(P, gram_tiles, apply_tiles, gram_first, apply_first, stream)
-                     : run_products<E, 64>(P, gram_tiles, apply_tiles, gram_first, apply_first, stream);
+    int rc;
+    if (kind == kFlatMatrix) {
+      place(share_first);
+      for (int launch = 0; launch <= P.steps; ++launch) {
+        P.last = launch == P.steps;
+        orthogonalise_flat<E><<<static_cast<unsigned>(shares), 1024, kSmallLds, stream>>>(P, launch);
+      }
+      rc = launch_status("orthogonalise");
+    } else {
+      place(split_first);
+      orthogonalise_split<E><<<static_cast<unsigned>(split_tiles), 256, 0, stream>>>(P);
+      rc = tile == 128 ? run_products<E, 128>(P, gram_tiles, apply_tiles, gram_first, apply_first, stream)
+                       : run_products<E, 64>(P, gram_tiles, apply_tiles, gram_first, apply_first, stream);
+    }
     if (rc != MBT_OK) return rc;
   }
   return MBT_OK;
+}
+
+template <typename E>
+int run(uint32_t count, const mbt_matrix* matrices, OrthogonaliseParams& P, void* workspace, hipStream_t stream) {
+  const int tile = common_tile(count, matrices);
+  char* next = static_cast<char*>(workspace);
+  int rc = run_small<E>(count, matrices, P, stream);
+  if (rc == MBT_OK) rc = run_kind<E>(kFlatMatrix, count, matrices, tile, P, next, stream);
+  if (rc == MBT_OK) rc = run_kind<E>(kLargeMatrix, count, matrices, tile, P, next, stream);
+  return rc;
 }
 
 // the kernels' shared memory is beyond the 64 KB that a launch gets unasked; set once per device
@@ -183,6 +220,7 @@ int allow_lds(int device) {
   static std::atomic<uint64_t> done{0};
   if (device < 64 && (done.load(std::memory_order_relaxed) >> device & 1)) return MBT_OK;
   LEARNING_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(orthogonalise_small<E>), hipFuncAttributeMaxDynamicSharedMemorySize, kSmallLds));
+  LEARNING_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(orthogonalise_flat<E>), hipFuncAttributeMaxDynamicSharedMemorySize, kSmallLds));
   const int lds = 2 * 4 * 128 * 40 * static_cast<int>(sizeof(_Float16));
   LEARNING_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(orthogonalise_product<E, 128, kGram>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
   LEARNING_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(orthogonalise_product<E, 128, kPolynomial>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));

@@ -3,17 +3,23 @@
 //   X = G / (|G| + eps),   `steps` times:   A = X X^T,   Q = a I + b A + c A^2,   X <- Q X         (m x n with m <= n; taller matrices are turned)
 //
 // The first steps multiply small singular values by a (3.4 each time), and with them whatever a rounding left in their directions, so operands of 11 or 8
-// bits would show in the result.  The fast matrix instructions take 16-bit operands; the float32 ones run at a sixteenth of their rate.  So every
-// operand is kept as TWO float16 numbers, v = hi + lo with hi = float16(v) and lo = float16(v - hi): 22 bits, and a product of two such operands
-// is hi hi + hi lo + lo hi - three float16 products, summed in float32, with nothing lost beyond 2^-21.  Values are scaled by powers of two that put
-// the largest possible one just inside float16's range (|X| < 1.9, A < 3.61, |Q| < 8: the host checks the coefficients), which leaves lo's
-// subnormal steps far below what matters.
+// bits would show in the result.  The matrix instructions that take 16-bit operands are sixteen times as fast as the float32 ones, so
+//
+//   min(m, n) > 64   every operand is TWO float16 numbers, v = hi + lo with hi = float16(v) and lo = float16(v - hi): 22 bits, and a product of two such
+//                    operands is hi hi + hi lo + lo hi - three float16 products, summed in float32, with nothing lost beyond 2^-21.  Values are scaled by
+//                    powers of two that put the largest possible one just inside float16's range (|X| < 1.9, A < 3.61, |Q| < 8: the host checks the
+//                    coefficients), which leaves lo's subnormal steps far below what matters.  The errors of many entries average out: the
+//                    result is as far from the exact one as that of float32 products (256 x 256: 1.5e-6 both; 1024 x 1024: 2.8e-6 and 2.6e-6).
+//   min(m, n) <= 64  float32 operands and instructions: the few entries of A and Q are shared by a whole row, a rounding of theirs does not average
+//                    out (4 x 64 with split operands: twice the error), and the work is too small for its rate to matter.
 //
 // A, A^2 and Q are symmetric.  Every product is of the form C = L R^T with both operands stored along k: A = X X^T, A^2 = A A^T, and
 // Q X = Q (X^T)^T, for which X is kept in both orders.  The polynomial is the epilogue of the product in front of it, the split into hi and lo the
 // epilogue of all three; a X needs no pass of its own, it is the a on Q's diagonal.
 //
-//   up to 64 x 64      one workgroup per matrix, everything in LDS, one launch for a whole list: latency bound (15 dependent products of 64^3)
+//   up to 64 x 64      one workgroup per matrix, everything in LDS, one launch for a whole list: bound by the latency of 15 dependent products
+//   m <= 64 < n        workgroups take columns of X; each adds up everyone's share of A, works out Q for itself, and turns its columns, whose
+//                      share of the next A it leaves for the next launch: one launch per step
 //   larger             tiled products over all matrices of the list at once: one launch for the norms, one for the split, three per step
 #pragma once
 #include "learning_common.hpp"
@@ -25,6 +31,7 @@ typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 
 constexpr float kScaleX = 32768.0f, kScaleA = 16384.0f, kScaleQ = 8192.0f;
+constexpr int kNormBlocks = 64;  // workgroups that add up one matrix's squares
 constexpr int kMostGroups = 16;  // matrix shapes of one launch, by value in its arguments
 
 struct MatrixGroup {  // `batch` matrices of one shape
@@ -32,10 +39,12 @@ struct MatrixGroup {  // `batch` matrices of one shape
   void* out;
   int64_t in_batch, in_row, in_column, out_batch, out_row, out_column;  // strides of the matrix as the kernels see it: m <= n, turned if it was taller
   int32_t m, n, mp, np;        // sizes, padded to the tile
-  int64_t first;               // (large) first tile of this launch, (small) first workgroup
-  int64_t planes;              // (large) where its planes start in the workspace, in halfs; each matrix of the batch has `stride` of them
+  int64_t first;               // first tile or workgroup of this launch
+  int64_t planes;              // where its planes start in the workspace, in halfs (flat: floats); each matrix of the batch has `stride` of them
   int64_t stride;
   int64_t batch;
+  int32_t shares;              // (flat) workgroups per matrix
+  int32_t reserved;
 };
 struct OrthogonaliseParams {
   MatrixGroup group[kMostGroups];
@@ -78,157 +87,198 @@ __device__ __forceinline__ int find_group(const OrthogonaliseParams& P, int64_t 
   return g;
 }
 
-// ---- up to 64 x 64: one workgroup, four waves, a 32 x 32 quarter of every product each ----------------------------------------------
-constexpr int kSmall = 64, kPitch = kSmall + 8;  // halfs; rows 144 bytes apart put the 16 rows of an operand read into 64 different banks
+// ---- min(m, n) <= 64: float32, sixteen waves, a 16 x 16 tile of every product each ----------------------------------------------------
+constexpr int kSmall = 64, kPitch = kSmall + 4;  // floats; rows 272 bytes apart put the 16 rows of an operand read into 64 different banks
 constexpr int kSmallPlane = kSmall * kPitch;
-constexpr size_t kSmallLds = 8 * kSmallPlane * sizeof(_Float16);
+constexpr size_t kSmallLds = 4 * kSmallPlane * sizeof(float);  // X, X^T, A, Q
+constexpr int kMostShares = 32;                                // workgroups that share one flat matrix
 
-// 32 x 32 of L R^T at (row, column), k up to kp
-__device__ __forceinline__ void small_product(const _Float16* l, const _Float16* r, int row, int column, int kp, float4v (&acc)[2][2]) {
-  const int lane = threadIdx.x & 63, at = (lane & 15) * kPitch + 8 * (lane >> 4);
+// the 16 x 16 tile of L R^T at (row, column).  A lane holds four neighbours along k of its row; which k an instruction's four slots stand for does not
+// matter as long as both operands agree.
+__device__ __forceinline__ float4v tile_product(const float* l, const float* r, int row, int column, int kp) {
+  const int lane = threadIdx.x & 63, at = (lane & 15) * kPitch + 4 * (lane >> 4);
+  const float *lp = l + row * kPitch + at, *rp = r + column * kPitch + at;
+  float4v acc = {0.f, 0.f, 0.f, 0.f}, odd = {0.f, 0.f, 0.f, 0.f};  // (two chains: an instruction need not wait for the one before it)
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int k = 0; k < kSmall; k += 16) {
+    if (k >= kp) break;
+    const float4v a = *reinterpret_cast<const float4v*>(lp + k), b = *reinterpret_cast<const float4v*>(rp + k);
+    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.x, b.x, acc, 0, 0, 0);
+    odd = __builtin_amdgcn_mfma_f32_16x16x4f32(a.y, b.y, odd, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.z, b.z, acc, 0, 0, 0);
+    odd = __builtin_amdgcn_mfma_f32_16x16x4f32(a.w, b.w, odd, 0, 0, 0);
+  }
+  return acc + odd;
+}
+
+struct SmallTile {
+  int row, column;  // of this wave's tile
+  int r0, c0;       // an accumulator's element r of this lane is at (row + r0 + r, column + c0)
+  __device__ __forceinline__ SmallTile() {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    row = 16 * (wave >> 2);
+    column = 16 * (wave & 3);
+    r0 = 4 * (lane >> 4);
+    c0 = lane & 15;
+  }
+  // four rows of one column, stored as four neighbours of a row of the transpose
+  __device__ __forceinline__ void put_turned(float* plane, float4v v) const { *reinterpret_cast<float4v*>(plane + (column + c0) * kPitch + row + r0) = v; }
+  __device__ __forceinline__ void put(float* plane, float4v v) const {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = float4v{0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < kp; k += 32) {
-    half8 lh[2], ll[2], rh[2], rl[2];
+    for (int r = 0; r < 4; ++r) plane[(row + r0 + r) * kPitch + column + c0] = v[r];
+  }
+};
+
+// Q from A, both in LDS; every wave calls it, mp a multiple of 16
+__device__ __forceinline__ void small_polynomial(const OrthogonaliseParams& P, const SmallTile& T, const float* am, float* q, int mp) {
+  if (T.row < mp && T.column < mp) {
+    const float4v square = tile_product(am, am, T.row, T.column, mp);
+    const float4v av = *reinterpret_cast<const float4v*>(am + (T.column + T.c0) * kPitch + T.row + T.r0);
+    float4v v;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int lo = (row + 16 * i) * kPitch + k + at, ro = (column + 16 * i) * kPitch + k + at;
-      lh[i] = *reinterpret_cast<const half8*>(l + lo);
-      ll[i] = *reinterpret_cast<const half8*>(l + kSmallPlane + lo);
-      rh[i] = *reinterpret_cast<const half8*>(r + ro);
-      rl[i] = *reinterpret_cast<const half8*>(r + kSmallPlane + ro);
+    for (int r = 0; r < 4; ++r) {
+      v[r] = __builtin_fmaf(P.b, av[r], P.c * square[r]);
+      if (T.row + T.r0 + r == T.column + T.c0) v[r] += P.a;
     }
-    // (a tile's three products depend on each other: the four tiles take turns)
-#pragma unroll
-    for (int t = 0; t < 4; ++t) acc[t >> 1][t & 1] = mfma(lh[t >> 1], rl[t & 1], acc[t >> 1][t & 1]);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) acc[t >> 1][t & 1] = mfma(ll[t >> 1], rh[t & 1], acc[t >> 1][t & 1]);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) acc[t >> 1][t & 1] = mfma(lh[t >> 1], rh[t & 1], acc[t >> 1][t & 1]);
+    T.put_turned(q, v);
   }
 }
 
 template <typename E>
-__global__ __launch_bounds__(256) void orthogonalise_small(const OrthogonaliseParams P) {
-  extern __shared__ _Float16 lds_small[];
-  __shared__ double sums[4];
+__global__ __launch_bounds__(1024) void orthogonalise_small(const OrthogonaliseParams P) {
+  extern __shared__ float lds_small[];
+  __shared__ double sums[16];
   int64_t which;
   const MatrixGroup M = P.group[find_group(P, blockIdx.x, which)];
   const E* in = static_cast<const E*>(M.in) + which * M.in_batch;
   E* out = static_cast<E*>(M.out) + which * M.out_batch;
-  // planes: X (hi, lo), X^T, A, Q
-  _Float16 *x = lds_small, *xt = x + 2 * kSmallPlane, *am = xt + 2 * kSmallPlane, *q = am + 2 * kSmallPlane;
-  float v[16];
+  float *x = lds_small, *xt = x + kSmallPlane, *am = xt + kSmallPlane, *q = am + kSmallPlane;
+  float v[4];
   double sum = 0.0;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {  // (threads along the longer stride-1 axis would only matter for a matrix that is read once)
-    const int at = threadIdx.x + 256 * k, i = at >> 6, j = at & 63;
+  for (int k = 0; k < 4; ++k) {
+    const int at = threadIdx.x + 1024 * k, i = at >> 6, j = at & 63;
     v[k] = i < M.m && j < M.n ? static_cast<float>(in[i * M.in_row + j * M.in_column]) : 0.0f;
     sum += static_cast<double>(v[k]) * static_cast<double>(v[k]);
   }
   sum = block_sum(sum, sums);
-  const float inverse = static_cast<float>(1.0 / (sqrt(sum) + P.eps));
+  const double inverse = 1.0 / (sqrt(sum) + P.eps);
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    const int at = threadIdx.x + 256 * k, i = at >> 6, j = at & 63;
-    const Halves h = split(v[k] * inverse * kScaleX);
-    x[i * kPitch + j] = h.hi;
-    x[kSmallPlane + i * kPitch + j] = h.lo;
-    xt[j * kPitch + i] = h.hi;
-    xt[kSmallPlane + j * kPitch + i] = h.lo;
+  for (int k = 0; k < 4; ++k) {
+    const int at = threadIdx.x + 1024 * k, i = at >> 6, j = at & 63;
+    const float scaled = static_cast<float>(v[k] * inverse);
+    x[i * kPitch + j] = scaled;
+    xt[j * kPitch + i] = scaled;
   }
   __syncthreads();
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int row = 32 * (wave >> 1), column = 32 * (wave & 1);
-  const int r0 = 4 * (lane >> 4), c0 = lane & 15;  // an accumulator's element r of this lane is at (r0 + r, c0) of its 16 x 16 tile
-  const bool square = row < M.mp && column < M.mp, flat = row < M.mp && column < M.np;
-  float4v acc[2][2];
+  const SmallTile T;
+  const bool square = T.row < M.mp && T.column < M.mp, flat = T.row < M.mp && T.column < M.np;
+  float4v acc = {0.f, 0.f, 0.f, 0.f};
   for (int step = 0; step < P.steps; ++step) {
-    if (square) {  // A; symmetric, so a lane's four rows of one column are stored as four neighbours of a row
-      small_product(x, x, row, column, M.np, acc);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          half4 hi, lo;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const Halves h = split(acc[i][j][r] * (kScaleA / kScaleX / kScaleX));
-            hi[r] = h.hi;
-            lo[r] = h.lo;
-          }
-          const int at = (column + 16 * j + c0) * kPitch + row + 16 * i + r0;
-          *reinterpret_cast<half4*>(am + at) = hi;
-          *reinterpret_cast<half4*>(am + kSmallPlane + at) = lo;
-        }
-    }
+    if (square) T.put_turned(am, tile_product(x, x, T.row, T.column, M.np));  // (symmetric)
     __syncthreads();
-    if (square) {
-      small_product(am, am, row, column, M.mp, acc);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int at = (column + 16 * j + c0) * kPitch + row + 16 * i + r0;
-          const half4 ah = *reinterpret_cast<const half4*>(am + at), al = *reinterpret_cast<const half4*>(am + kSmallPlane + at);
-          half4 hi, lo;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float av = (static_cast<float>(ah[r]) + static_cast<float>(al[r])) * (kScaleQ / kScaleA);
-            float value = __builtin_fmaf(P.b, av, P.c * (acc[i][j][r] * (kScaleQ / kScaleA / kScaleA)));
-            if (row + 16 * i + r0 + r == column + 16 * j + c0) value += P.a * kScaleQ;
-            const Halves h = split(value);
-            hi[r] = h.hi;
-            lo[r] = h.lo;
-          }
-          *reinterpret_cast<half4*>(q + at) = hi;
-          *reinterpret_cast<half4*>(q + kSmallPlane + at) = lo;
-        }
-    }
+    small_polynomial(P, T, am, q, M.mp);
     __syncthreads();
-    if (flat) small_product(q, xt, row, column, M.mp, acc);
+    if (flat) acc = tile_product(q, xt, T.row, T.column, M.mp);
     if (step + 1 == P.steps) break;
     __syncthreads();  // X^T has been read
     if (flat) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          half4 hi, lo;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const Halves h = split(acc[i][j][r] * (1.0f / kScaleQ));
-            hi[r] = h.hi;
-            lo[r] = h.lo;
-            const int at = (row + 16 * i + r0 + r) * kPitch + column + 16 * j + c0;
-            x[at] = h.hi;
-            x[kSmallPlane + at] = h.lo;
-          }
-          const int at = (column + 16 * j + c0) * kPitch + row + 16 * i + r0;
-          *reinterpret_cast<half4*>(xt + at) = hi;
-          *reinterpret_cast<half4*>(xt + kSmallPlane + at) = lo;
-        }
+      T.put(x, acc);
+      T.put_turned(xt, acc);
     }
     __syncthreads();
   }
   if (flat) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int at = row + 16 * i + r0 + r, to = column + 16 * j + c0;
-          if (at < M.m && to < M.n) out[at * M.out_row + to * M.out_column] = static_cast<E>(acc[i][j][r] * (1.0f / kScaleQ / kScaleX));
-        }
+    for (int r = 0; r < 4; ++r) {
+      const int i = T.row + T.r0 + r, j = T.column + T.c0;
+      if (i < M.m && j < M.n) out[i * M.out_row + j * M.out_column] = static_cast<E>(acc[r]);
+    }
   }
 }
 
-// ---- larger ------------------------------------------------------------------------------------------------------------------------
-constexpr int kNormBlocks = 64;
+// One step of a flat matrix (m <= 64 < n), `shares` workgroups each, which take its blocks of 64 columns in turn.  Workspace per matrix, in floats:
+// X (64 x np, by blocks of 64 x 64), then the shares of A (64 x 64 each) of this step and the next.  Launch 0 brings X in and leaves the first shares;
+// launch s = 1 .. steps turns X, the last one into the output.
+template <typename E>
+__global__ __launch_bounds__(1024) void orthogonalise_flat(const OrthogonaliseParams P, int launch) {
+  extern __shared__ float lds_small[];
+  __shared__ double sums[16];
+  int64_t at;
+  const int group = find_group(P, blockIdx.x, at);
+  const MatrixGroup M = P.group[group];
+  const int shares = M.shares, share = static_cast<int>(at % shares), column_blocks = M.np / 64;
+  const int64_t which = at / shares;
+  float* xs = reinterpret_cast<float*>(P.planes) + M.planes + which * M.stride;
+  float* const all_shares = xs + 64 * static_cast<int64_t>(M.np);
+  const float* before = all_shares + (launch & 1 ? 0 : 1) * static_cast<int64_t>(kMostShares) * 4096;
+  float* after = all_shares + (launch & 1 ? 1 : 0) * static_cast<int64_t>(kMostShares) * 4096;
+  float *x = lds_small, *xt = x + kSmallPlane, *am = xt + kSmallPlane, *q = am + kSmallPlane;
+  const SmallTile T;
+  const int mp = M.mp;
+  const bool square = T.row < mp && T.column < mp, flat = T.row < mp;
+  double inverse = 0.0;
+  if (launch == 0) {
+    int64_t matrix = which;
+    for (int g = 0; g < group; ++g) matrix += P.group[g].batch;
+    const double norm = block_sum(threadIdx.x < kNormBlocks ? P.partials[matrix * kNormBlocks + threadIdx.x] : 0.0, sums);
+    inverse = 1.0 / (sqrt(norm) + P.eps);
+  } else {  // A: everyone's shares, in their order
+    float4v a = {0.f, 0.f, 0.f, 0.f};
+    const int i = threadIdx.x >> 4, j = 4 * (threadIdx.x & 15);
+#pragma unroll 8
+    for (int w = 0; w < shares; ++w) a += *reinterpret_cast<const float4v*>(before + w * 4096 + i * 64 + j);
+    *reinterpret_cast<float4v*>(am + i * kPitch + j) = a;
+    __syncthreads();
+    small_polynomial(P, T, am, q, mp);
+  }
+  const E* in = static_cast<const E*>(M.in) + which * M.in_batch;
+  E* out = static_cast<E*>(M.out) + which * M.out_batch;
+  const bool along_n = M.in_column <= M.in_row;
+  float4v gram = {0.f, 0.f, 0.f, 0.f};
+  for (int block = share; block < column_blocks; block += shares) {
+    const int j0 = 64 * block;
+    float* mine = xs + static_cast<int64_t>(block) * 4096;
+    __syncthreads();  // (the block before has been read, Q is written)
+    if (launch == 0) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int e = threadIdx.x + 1024 * k, i = along_n ? e >> 6 : e & 63, j = along_n ? e & 63 : e >> 6;
+        const float v = i < M.m && j0 + j < M.n ? static_cast<float>(static_cast<float>(in[i * M.in_row + (j0 + j) * M.in_column]) * inverse) : 0.0f;
+        x[i * kPitch + j] = v;
+        mine[i * 64 + j] = v;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int e = threadIdx.x + 1024 * k, i = e >> 6, j = e & 63;
+        xt[j * kPitch + i] = mine[e];
+      }
+      __syncthreads();
+      if (flat) {
+        const float4v acc = tile_product(q, xt, T.row, T.column, mp);
+        if (P.last) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int i = T.row + T.r0 + r, j = j0 + T.column + T.c0;
+            if (i < M.m && j < M.n) out[i * M.out_row + j * M.out_column] = static_cast<E>(acc[r]);
+          }
+        } else {
+          T.put(x, acc);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) mine[(T.row + T.r0 + r) * 64 + T.column + T.c0] = acc[r];
+        }
+      }
+    }
+    if (P.last) continue;
+    __syncthreads();
+    if (square) gram += tile_product(x, x, T.row, T.column, 64);
+  }
+  if (P.last) return;
+  *reinterpret_cast<float4v*>(after + share * 4096 + (T.column + T.c0) * 64 + T.row + T.r0) = gram;  // (zeros where there is no tile)
+}
 
+// ---- larger ------------------------------------------------------------------------------------------------------------------------
 // planes of one matrix, in halfs from its start: X hi, lo (mp x np); X^T hi, lo twice (np x mp); A hi, lo; Q hi, lo (mp x mp)
 struct Planes {
   _Float16 *x, *xt, *xt_next, *a, *q;  // (X^T of this step and of the next)

@@ -23,8 +23,8 @@ def orthogonalise(updates: Union[torch.Tensor, Sequence[torch.Tensor]], *, steps
                   what comes back has the same form.  The arithmetic is as accurate as float32 for every type: one rounding, at the end
     coefficients  (a, b, c); they have to keep singular values that start within [0, 1] below 1.9
 
-    A matrix of zeros stays zero; a NaN or an infinity anywhere in a matrix makes that matrix NaN.  Not differentiable.  Lists cost one launch for all
-    matrices up to 64 x 64 and seventeen for all larger ones, however many there are (per sixteen shapes)."""
+    A matrix of zeros stays zero; a NaN or an infinity anywhere in a matrix makes that matrix NaN.  Not differentiable.  A list costs one launch for all its
+    matrices up to 64 x 64, seven for those with one side longer and seventeen for the rest, however many there are (per sixteen shapes)."""
     single = isinstance(updates, torch.Tensor)
     given = [updates] if single else list(updates)
     if not given:
@@ -56,10 +56,7 @@ def orthogonalise(updates: Union[torch.Tensor, Sequence[torch.Tensor]], *, steps
             t = t.reshape(-1, rows, columns)  # (a copy only where the batch axes do not fold)
             batch, in_stride = t.shape[0], t.stride(0)
         kept.append(t)
-        m = matrices[count]
-        m.in_, m.out, m.rows, m.columns, m.batch = t.data_ptr(), out.data_ptr(), rows, columns, batch
-        m.in_stride[:] = (in_stride, t.stride(-2), t.stride(-1))
-        m.out_stride[:] = (out_stride, columns, 1)
+        matrices[count] = _native.MbtMatrix(t.data_ptr(), out.data_ptr(), rows, columns, batch, (in_stride,) + t.stride()[-2:], (out_stride, columns, 1))
         count += 1
     if count:
         lib = _native.load_library()
