@@ -5,10 +5,12 @@ include_log_probs)`, `train(num_epochs, reporting_freq) -> (losses, mean rewards
 of the sampled actions weighted by the rewards-to-go, PG:49-73).  What differs is where an epoch's data comes from: when the
 actor is a network the kernels can evaluate ([Linear, act, Linear, act, Linear], hidden width <= 64, tanh or relu) the whole
 episode is sampled by ONE fused rollout launch - the network on the matrix cores, a ~ N(mean, std) drawn from Philox in the
-kernel, observations / actions / rewards recorded straight into torch tensors - and PyTorch only computes what needs
-gradients: log N(a | policy(obs), std) of the recorded pairs.  Any other torch module takes the reference's loop
-(generate_trajectory with include_log_probs=True: one host forward pass and one env.step per time step).  PyTorch is the
-consumer here, not the product."""
+kernel, observations / actions / rewards recorded straight into torch tensors - and what is learnt from them is computed there
+too: the rewards-to-go, the loss log N(a | policy(obs), std) x reward-to-go and its gradient with respect to the network's
+answers are kernels (mbt_gym_amd/learning), PyTorch carries that gradient on through the network.  Any other torch module takes
+the reference's loop (generate_trajectory with include_log_probs=True: one host forward pass and one env.step per time step); a
+`learning.RecurrentPolicy` quotes step by step in that loop and is scored on the whole recording at once.  PyTorch is the consumer
+here, not the product."""
 from typing import Callable, Tuple, Union
 
 import numpy as np
@@ -37,9 +39,20 @@ def _actor_layers(policy):
 
 
 class PolicyGradientAgent(Agent):
-    def __init__(self, policy, action_std: Union[float, Callable] = 0.01, optimizer=None, env=None, lr_scheduler=None):
+    def __init__(self, policy, action_std: Union[float, Callable] = 0.01, optimizer=None, env=None, lr_scheduler=None, discount: float = 1.0):
+        """Beyond the reference's arguments: `discount` of the rewards-to-go (the reference's learner has none: 1), and `optimizer` may be the name
+        "muon" (mbt_gym_amd.learning.Muon over the policy's parameters)."""
         import torch
         from torch.optim.lr_scheduler import StepLR
+
+        if not 0.0 <= discount <= 1.0:
+            raise ValueError(f"discount = {discount}: it has to lie in [0, 1]")
+        if isinstance(optimizer, str):
+            if optimizer != "muon":
+                raise ValueError(f"optimizer = {optimizer!r}: an optimizer, or the name 'muon'")
+            from mbt_gym_amd.learning import Muon
+
+            optimizer = Muon(policy.parameters())
 
         if env is None:
             from mbt_gym_amd.gym.TradingEnvironment import TradingEnvironment
@@ -52,6 +65,7 @@ class PolicyGradientAgent(Agent):
         assert first is None or self.input_size == first.in_features
         self.policy_net = policy
         self.action_std = action_std
+        self.discount = float(discount)
         self.optimizer = optimizer or torch.optim.SGD(self.policy_net.parameters(), lr=1e-1)
         self.lr_scheduler = lr_scheduler or StepLR(self.optimizer, step_size=1, gamma=0.995)
         self.noise_dist = torch.distributions.Normal
@@ -70,7 +84,8 @@ class PolicyGradientAgent(Agent):
         import torch
 
         assert not (deterministic and include_log_probs), "include_log_probs is only an option for deterministic output"
-        mean_value = self.policy_net(torch.as_tensor(np.asarray(state), dtype=torch.float, device=self._module_device()))
+        observation = torch.as_tensor(np.asarray(state), dtype=torch.float, device=self._module_device())
+        mean_value = self.policy_net.step(observation) if self._is_recurrent else self.policy_net(observation)
         if deterministic:
             return mean_value.detach().cpu().numpy()
         action_dist = self.noise_dist(loc=mean_value, scale=self._std() * torch.ones_like(mean_value))
@@ -78,6 +93,17 @@ class PolicyGradientAgent(Agent):
         if include_log_probs:
             return action.detach().cpu().numpy(), action_dist.log_prob(action)
         return action.detach().cpu().numpy()
+
+    @property
+    def _is_recurrent(self) -> bool:
+        from mbt_gym_amd.learning import RecurrentPolicy
+
+        return isinstance(self.policy_net, RecurrentPolicy)
+
+    def begin_episode(self):
+        """What an actor carries from step to step starts anew (generate_trajectory calls this after env.reset())."""
+        if self._is_recurrent:
+            self.policy_net.begin_episode()
 
     @property
     def has_device_policy(self) -> bool:
@@ -117,8 +143,8 @@ class PolicyGradientAgent(Agent):
         return _native.mlp_policy(layers, activation, action_std=std, clip=False)
 
     # ---- one epoch of data ----------------------------------------------------------------------------------------------------
-    def _sample_on_device(self):
-        """(rewards (N, 1, T) tensor, log-probabilities (N, A, T) tensor with gradients), from one fused rollout launch."""
+    def _record_on_device(self):
+        """One fused rollout launch: (observations (T, N, D), actions (T, N, A), rewards (T, N)), views of the padded recording on the device."""
         import torch
 
         env = self.env
@@ -130,10 +156,34 @@ class PolicyGradientAgent(Agent):
         env.set_stream(torch.cuda.current_stream(cuda).cuda_stream)  # torch's allocator and the kernel share a stream
         env.reset_device()
         steps, _ = env.rollout_device(self.device_policy(), max_steps=horizon, obs_ptr=obs.data_ptr(), act_ptr=act.data_ptr(), rew_ptr=rew.data_ptr())
+        return obs[:steps, :n], act[:steps, :n], rew[:steps, :n]
+
+    def _sample_on_device(self):
+        """(rewards (N, 1, T) tensor, log-probabilities (N, A, T) tensor with gradients), from one fused rollout launch."""
         where = self._module_device()
-        o, a, r = obs[:steps, :n].to(where), act[:steps, :n].to(where), rew[:steps, :n].to(where)
+        o, a, r = (t.to(where) for t in self._record_on_device())
         log_prob = self.noise_dist(self.kernel_mean(o), self._std()).log_prob(a)  # of the actions the KERNEL sampled, around ITS mean: (T, N, A)
         return r.t().unsqueeze(1), log_prob.permute(1, 2, 0)
+
+    def _device_epoch(self):
+        """(rewards, loss) of one epoch whose data never leaves the device: - mean of log N(a | mean, std) x reward-to-go (PG:58-59) as kernels"""
+        from mbt_gym_amd.learning import policy_gradient_loss, rewards_to_go
+
+        if self._is_recurrent:
+            observations, actions, rewards, where = *generate_trajectory(self.env, self), self._module_device()
+            o, a = (self._time_first(t, where) for t in (observations[:, :, :-1], actions))
+            r, mean = self._time_first(rewards[:, 0], where), self.policy_net(o)
+        else:
+            o, a, r = self._record_on_device()
+            mean = self.kernel_mean(o)
+        return r, policy_gradient_loss(mean, a, rewards_to_go(r, self.discount, dim=0), self._std())
+
+    @staticmethod
+    def _time_first(array, where):
+        """(N, ..., T) on the host -> (T, N, ...) on the device"""
+        import torch
+
+        return torch.as_tensor(np.ascontiguousarray(np.moveaxis(array, -1, 0)), device=where)
 
     def train(self, num_epochs: int = 1, reporting_freq: int = 100):
         import torch
@@ -141,14 +191,18 @@ class PolicyGradientAgent(Agent):
         learning_losses, learning_rewards = [], []
         self.proportion_completed = 0.0
         for epoch in range(num_epochs):
-            if self.has_device_policy:
-                rewards, log_probs = self._sample_on_device()
+            if self._is_recurrent or (self.has_device_policy and self._module_device() == torch.device("cuda", self.env.device)):
+                rewards, loss = self._device_epoch()
+                learning_rewards.append(float(rewards.mean()))
             else:
-                _, _, rewards, log_probs = generate_trajectory(self.env, self, include_log_probs=True)
-                rewards = torch.as_tensor(rewards, device=log_probs.device)
-            learning_rewards.append(float(rewards.mean()))
-            future_rewards = self._calculate_future_rewards(rewards)
-            loss = -torch.mean(log_probs * future_rewards)  # PG:58-59
+                if self.has_device_policy:
+                    rewards, log_probs = self._sample_on_device()
+                else:
+                    _, _, rewards, log_probs = generate_trajectory(self.env, self, include_log_probs=True)
+                    rewards = torch.as_tensor(rewards, device=log_probs.device)
+                learning_rewards.append(float(rewards.mean()))
+                future_rewards = self._calculate_future_rewards(rewards, self.discount)
+                loss = -torch.mean(log_probs * future_rewards)  # PG:58-59
             self.optimizer.zero_grad()
             loss.backward()
             self.optimizer.step()
@@ -160,7 +214,18 @@ class PolicyGradientAgent(Agent):
         return learning_losses, learning_rewards
 
     @staticmethod
-    def _calculate_future_rewards(rewards):
+    def _calculate_future_rewards(rewards, discount: float = 1.0):
+        """Rewards-to-go along the last axis (PG:69-73): a kernel where the rewards live on the device, torch where they live on the host."""
         import torch
 
-        return torch.flip(torch.cumsum(torch.flip(rewards, dims=(-1,)), dim=-1), dims=(-1,))  # rewards-to-go (PG:69-73)
+        if rewards.is_cuda and rewards.dtype in (torch.float32, torch.bfloat16, torch.float16):
+            from mbt_gym_amd.learning import rewards_to_go
+
+            return rewards_to_go(rewards, discount)
+        if discount == 1.0:
+            return torch.flip(torch.cumsum(torch.flip(rewards, dims=(-1,)), dim=-1), dims=(-1,))
+        out, following = torch.empty_like(rewards), torch.zeros_like(rewards[..., 0])
+        for k in range(rewards.shape[-1] - 1, -1, -1):
+            following = rewards[..., k] + discount * following
+            out[..., k] = following
+        return out

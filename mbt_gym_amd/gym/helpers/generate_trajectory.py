@@ -65,6 +65,8 @@ def generate_trajectory(env, agent, seed: int = None, include_log_probs: bool = 
 
         log_probs = torch.zeros((n, env.action_space.shape[0], horizon))
     obs = env.reset()
+    if hasattr(agent, "begin_episode"):  # an actor with a memory starts its episode with the environment's
+        agent.begin_episode()
     observations[:, :, 0] = obs
     for k in range(horizon):
         if include_log_probs:
