@@ -28,17 +28,14 @@ def current_stream(index):
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-def dense_like(tensor):
-    """An empty tensor of the same shape whose axes lie in memory in the same order, without gaps."""
-    if tensor.is_contiguous():
-        return torch.empty_like(tensor)
-    strides = tensor.stride()
-    order = sorted(range(len(strides)), key=lambda d: (-strides[d], d))
-    shape, dense, run = tensor.shape, [0] * len(strides), 1
-    for d in reversed(order):
+def dense_strides(tensor):
+    """The strides of a tensor of the same shape whose axes lie in memory in the same order, without gaps."""
+    strides, shape = tensor.stride(), tensor.shape
+    dense, run = [0] * len(strides), 1
+    for d in sorted(range(len(strides)), key=lambda d: (strides[d], -d)):
         dense[d] = run
-        run *= shape[d]
-    return torch.empty_strided(shape, dense, dtype=tensor.dtype, device=tensor.device)
+        run *= max(1, shape[d])
+    return tuple(dense)
 
 
 def batch_groups(shape, axis, strides):

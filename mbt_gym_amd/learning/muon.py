@@ -37,28 +37,30 @@ def orthogonalise(updates: Union[torch.Tensor, Sequence[torch.Tensor]], *, steps
     coefficients = [float(c) for c in coefficients]
     if len(coefficients) != 3:
         raise ValueError(f"{len(coefficients)} coefficients: three (a, b, c) are needed")
-    matrices = (_native.MbtMatrix * len(given))()
-    outs, kept, count = [], [], 0
+    outs, kept, described = [], [], []
+    tracked = torch.is_grad_enabled()
     for t in given:
         require(t, "updates", device, (dtype,))
-        if t.dim() < 2:
-            raise ValueError(f"an update of the shape {tuple(t.shape)} is not a matrix")
-        if torch.is_grad_enabled() and t.requires_grad:
+        shape = t.shape
+        if len(shape) < 2:
+            raise ValueError(f"an update of the shape {tuple(shape)} is not a matrix")
+        if tracked and t.requires_grad:
             raise ValueError("orthogonalise is not differentiable: detach the updates")
-        out = torch.empty(t.shape, dtype=dtype, device=device)
+        out = torch.empty(shape, dtype=dtype, device=device)
         outs.append(out)
-        if t.numel() == 0:
-            continue
-        rows, columns = t.shape[-2:]
-        batch = 1
-        in_stride, out_stride = 0, rows * columns
-        if t.dim() > 2:
-            t = t.reshape(-1, rows, columns)  # (a copy only where the batch axes do not fold)
-            batch, in_stride = t.shape[0], t.stride(0)
-        kept.append(t)
-        matrices[count] = _native.MbtMatrix(t.data_ptr(), out.data_ptr(), rows, columns, batch, (in_stride,) + t.stride()[-2:], (out_stride, columns, 1))
-        count += 1
+        if len(shape) == 2:
+            rows, columns = shape
+            batch, strides = 1, (0,) + t.stride()
+        else:
+            rows, columns = shape[-2:]
+            t = t.reshape(-1, rows, columns) if t.numel() else t  # (a copy only where the batch axes do not fold)
+            batch, strides = t.shape[0], t.stride()[-3:]
+        if rows and columns and t.numel():
+            kept.append(t)
+            described.append((t.data_ptr(), out.data_ptr(), rows, columns, batch, strides, (rows * columns, columns, 1)))
+    count = len(described)
     if count:
+        matrices = (_native.MbtMatrix * count)(*described)
         lib = _native.load_library()
         size = lib.mbt_orthogonalise_workspace(count, matrices)
         workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
