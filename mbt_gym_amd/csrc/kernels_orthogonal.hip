@@ -16,7 +16,8 @@ Kind kind_of(const mbt_matrix& m) {
   return large <= kSmall ? kSmallMatrix : small <= kSmall ? kFlatMatrix : kLargeMatrix;
 }
 
-// 128 x 128 tiles read every operand half as often as 64 x 64 ones and need four times as large a matrix to occupy the chip
+// 128 x 128 tiles read every operand half as often as 64 x 64 ones, but there are a quarter as many: they win where they occupy three quarters of the
+// compute units (2048 x 2048: 41 and 50 us a product against 46 and 70), and lose below (1024 x 1024: 21 and 23 against 11 and 13)
 int tile_of(const mbt_matrix& m) {
   const int64_t small = m.rows < m.columns ? m.rows : m.columns, large = m.rows < m.columns ? m.columns : m.rows;
   return (padded(small, 128) / 128) * (padded(large, 128) / 128) * static_cast<int64_t>(m.batch) >= 192 ? 128 : 64;
@@ -101,21 +102,28 @@ bool bounded(int steps, const double c[3]) {
   return true;
 }
 
+// three buffers of two operands in two halves, 64 bytes a row
+template <int T>
+constexpr size_t kProductLds = 3 * 2 * 2 * T * 64;
+
+template <int T>
+constexpr int kWaves = T == 128 ? 8 : 4;
+
 template <typename E, int T>
 int run_products(OrthogonaliseParams& P, int64_t gram_tiles, int64_t apply_tiles, const int64_t (&gram_first)[kMostGroups], const int64_t (&apply_first)[kMostGroups],
                  hipStream_t stream) {
-  constexpr size_t lds = 2 * 4 * T * 40 * sizeof(_Float16);
+  constexpr size_t lds = kProductLds<T>;
   auto launch = [&](auto kernel, int64_t tiles, const int64_t (&first)[kMostGroups]) {
     for (int g = 0; g < P.groups; ++g) P.group[g].first = first[g];
     P.blocks = tiles;
-    kernel<<<static_cast<unsigned>((tiles + 7) / 8 * 8), 256, lds, stream>>>(P);
+    kernel<<<static_cast<unsigned>((tiles + 7) / 8 * 8), 64 * kWaves<T>, lds, stream>>>(P);
   };
   P.odd = 0;
   for (int step = 0; step < P.steps; ++step) {
     P.last = step + 1 == P.steps;
-    launch(orthogonalise_product<E, T, kGram>, gram_tiles, gram_first);
-    launch(orthogonalise_product<E, T, kPolynomial>, gram_tiles, gram_first);
-    launch(orthogonalise_product<E, T, kApply>, apply_tiles, apply_first);
+    launch(orthogonalise_product<E, T, kWaves<T>, kGram>, gram_tiles, gram_first);
+    launch(orthogonalise_product<E, T, kWaves<T>, kPolynomial>, gram_tiles, gram_first);
+    launch(orthogonalise_product<E, T, kWaves<T>, kApply>, apply_tiles, apply_first);
     P.odd ^= 1;
   }
   return launch_status("orthogonalise");
@@ -184,7 +192,7 @@ int run_kind(Kind kind, uint32_t count, const mbt_matrix* matrices, int tile, Or
       for (int g = 0; g < P.groups; ++g) P.group[g].first = first[g];
     };
     place(norm_first);
-    orthogonalise_norms<E><<<static_cast<unsigned>(matrices_in * kNormBlocks), 256, 0, stream>>>(P);
+    orthogonalise_norms<E><<<static_cast<unsigned>(matrices_in * kNormBlocks), 1024, 0, stream>>>(P);
     int rc;
     if (kind == kFlatMatrix) {
       place(share_first);
@@ -221,10 +229,10 @@ int allow_lds(int device) {
   if (device < 64 && (done.load(std::memory_order_relaxed) >> device & 1)) return MBT_OK;
   LEARNING_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(orthogonalise_small<E>), hipFuncAttributeMaxDynamicSharedMemorySize, kSmallLds));
   LEARNING_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(orthogonalise_flat<E>), hipFuncAttributeMaxDynamicSharedMemorySize, kSmallLds));
-  const int lds = 2 * 4 * 128 * 40 * static_cast<int>(sizeof(_Float16));
-  LEARNING_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(orthogonalise_product<E, 128, kGram>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-  LEARNING_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(orthogonalise_product<E, 128, kPolynomial>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-  LEARNING_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(orthogonalise_product<E, 128, kApply>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  const int lds = static_cast<int>(kProductLds<128>);
+  LEARNING_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(orthogonalise_product<E, 128, kWaves<128>, kGram>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  LEARNING_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(orthogonalise_product<E, 128, kWaves<128>, kPolynomial>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  LEARNING_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(orthogonalise_product<E, 128, kWaves<128>, kApply>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
   if (device < 64) done.fetch_or(1ull << device, std::memory_order_relaxed);
   return MBT_OK;
 }

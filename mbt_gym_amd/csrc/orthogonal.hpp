@@ -31,7 +31,7 @@ typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 
 constexpr float kScaleX = 32768.0f, kScaleA = 16384.0f, kScaleQ = 8192.0f;
-constexpr int kNormBlocks = 64;  // workgroups that add up one matrix's squares
+constexpr int kNormBlocks = 256;  // workgroups that add up one matrix's squares
 constexpr int kMostGroups = 16;  // matrix shapes of one launch, by value in its arguments
 
 struct MatrixGroup {  // `batch` matrices of one shape
@@ -67,6 +67,14 @@ __device__ __forceinline__ Halves split(float v) {
   return {hi, static_cast<_Float16>(v - static_cast<float>(hi))};
 }
 
+// A barrier over what the workgroup has in LDS: __syncthreads() also waits for every load from memory that is on its way, which is what a pipeline
+// that runs steps ahead must not do.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 __device__ __forceinline__ float4v mfma(half8 a, half8 b, float4v c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
 __device__ __forceinline__ double block_sum(double v, double* lds) {
@@ -88,21 +96,25 @@ __device__ __forceinline__ int find_group(const OrthogonaliseParams& P, int64_t 
 }
 
 // ---- min(m, n) <= 64: float32, sixteen waves, a 16 x 16 tile of every product each ----------------------------------------------------
-constexpr int kSmall = 64, kPitch = kSmall + 4;  // floats; rows 272 bytes apart put the 16 rows of an operand read into 64 different banks
-constexpr int kSmallPlane = kSmall * kPitch;
+constexpr int kSmall = 64, kSmallPlane = kSmall * kSmall;
 constexpr size_t kSmallLds = 4 * kSmallPlane * sizeof(float);  // X, X^T, A, Q
 constexpr int kMostShares = 32;                                // workgroups that share one flat matrix
+
+// where element (row, column) of a plane lies: the 16-byte pieces of a row are exchanged by its number, so that the lanes of a 16-byte read - the same piece
+// of sixteen rows, or neighbouring pieces of half of them - meet different banks
+__device__ __forceinline__ int small_at(int row, int column) { return row * kSmall + (((column >> 2) ^ row) & 15) * 4 + (column & 3); }
 
 // the 16 x 16 tile of L R^T at (row, column).  A lane holds four neighbours along k of its row; which k an instruction's four slots stand for does not
 // matter as long as both operands agree.
 __device__ __forceinline__ float4v tile_product(const float* l, const float* r, int row, int column, int kp) {
-  const int lane = threadIdx.x & 63, at = (lane & 15) * kPitch + 4 * (lane >> 4);
-  const float *lp = l + row * kPitch + at, *rp = r + column * kPitch + at;
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const float *lp = l + (row + i) * kSmall, *rp = r + (column + i) * kSmall;
   float4v acc = {0.f, 0.f, 0.f, 0.f}, odd = {0.f, 0.f, 0.f, 0.f};  // (two chains: an instruction need not wait for the one before it)
 #pragma unroll
   for (int k = 0; k < kSmall; k += 16) {
     if (k >= kp) break;
-    const float4v a = *reinterpret_cast<const float4v*>(lp + k), b = *reinterpret_cast<const float4v*>(rp + k);
+    const int piece = ((k >> 2) + g ^ i) * 4;  // (row and column are multiples of 16: i is the row's number as far as the exchange goes)
+    const float4v a = *reinterpret_cast<const float4v*>(lp + piece), b = *reinterpret_cast<const float4v*>(rp + piece);
     acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.x, b.x, acc, 0, 0, 0);
     odd = __builtin_amdgcn_mfma_f32_16x16x4f32(a.y, b.y, odd, 0, 0, 0);
     acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.z, b.z, acc, 0, 0, 0);
@@ -122,10 +134,10 @@ struct SmallTile {
     c0 = lane & 15;
   }
   // four rows of one column, stored as four neighbours of a row of the transpose
-  __device__ __forceinline__ void put_turned(float* plane, float4v v) const { *reinterpret_cast<float4v*>(plane + (column + c0) * kPitch + row + r0) = v; }
+  __device__ __forceinline__ void put_turned(float* plane, float4v v) const { *reinterpret_cast<float4v*>(plane + small_at(column + c0, row + r0)) = v; }
   __device__ __forceinline__ void put(float* plane, float4v v) const {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) plane[(row + r0 + r) * kPitch + column + c0] = v[r];
+    for (int r = 0; r < 4; ++r) plane[small_at(row + r0 + r, column + c0)] = v[r];
   }
 };
 
@@ -133,7 +145,7 @@ struct SmallTile {
 __device__ __forceinline__ void small_polynomial(const OrthogonaliseParams& P, const SmallTile& T, const float* am, float* q, int mp) {
   if (T.row < mp && T.column < mp) {
     const float4v square = tile_product(am, am, T.row, T.column, mp);
-    const float4v av = *reinterpret_cast<const float4v*>(am + (T.column + T.c0) * kPitch + T.row + T.r0);
+    const float4v av = *reinterpret_cast<const float4v*>(am + small_at(T.column + T.c0, T.row + T.r0));
     float4v v;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -167,8 +179,8 @@ __global__ __launch_bounds__(1024) void orthogonalise_small(const OrthogonaliseP
   for (int k = 0; k < 4; ++k) {
     const int at = threadIdx.x + 1024 * k, i = at >> 6, j = at & 63;
     const float scaled = static_cast<float>(v[k] * inverse);
-    x[i * kPitch + j] = scaled;
-    xt[j * kPitch + i] = scaled;
+    x[small_at(i, j)] = scaled;
+    xt[small_at(j, i)] = scaled;
   }
   __syncthreads();
   const SmallTile T;
@@ -228,7 +240,7 @@ __global__ __launch_bounds__(1024) void orthogonalise_flat(const OrthogonalisePa
     const int i = threadIdx.x >> 4, j = 4 * (threadIdx.x & 15);
 #pragma unroll 8
     for (int w = 0; w < shares; ++w) a += *reinterpret_cast<const float4v*>(before + w * 4096 + i * 64 + j);
-    *reinterpret_cast<float4v*>(am + i * kPitch + j) = a;
+    *reinterpret_cast<float4v*>(am + small_at(i, j)) = a;
     __syncthreads();
     small_polynomial(P, T, am, q, mp);
   }
@@ -245,14 +257,14 @@ __global__ __launch_bounds__(1024) void orthogonalise_flat(const OrthogonalisePa
       for (int k = 0; k < 4; ++k) {
         const int e = threadIdx.x + 1024 * k, i = along_n ? e >> 6 : e & 63, j = along_n ? e & 63 : e >> 6;
         const float v = i < M.m && j0 + j < M.n ? static_cast<float>(static_cast<float>(in[i * M.in_row + (j0 + j) * M.in_column]) * inverse) : 0.0f;
-        x[i * kPitch + j] = v;
+        x[small_at(i, j)] = v;
         mine[i * 64 + j] = v;
       }
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int e = threadIdx.x + 1024 * k, i = e >> 6, j = e & 63;
-        xt[j * kPitch + i] = mine[e];
+        xt[small_at(j, i)] = mine[e];
       }
       __syncthreads();
       if (flat) {
@@ -279,40 +291,51 @@ __global__ __launch_bounds__(1024) void orthogonalise_flat(const OrthogonalisePa
 }
 
 // ---- larger ------------------------------------------------------------------------------------------------------------------------
-// planes of one matrix, in halfs from its start: X hi, lo (mp x np); X^T hi, lo twice (np x mp); A hi, lo; Q hi, lo (mp x mp)
+// A matrix as a product reads it: cut into tiles of 16 rows x 32 along k, each tile 1 KB of hi followed by 1 KB of lo, the tiles of one k step
+// behind one another - what a workgroup needs for a step is contiguous, and one load of a wave is one tile, whole lines of it.
+struct Tiled {
+  _Float16* p;
+  int row_tiles;  // of the matrix
+  __device__ __forceinline__ int64_t at(int row, int k) const {
+    return (static_cast<int64_t>(k >> 5) * row_tiles + (row >> 4)) * 1024 + (row & 15) * 32 + (k & 31);
+  }
+};
+constexpr int kLo = 512;  // halfs from hi to lo
+
+// of one matrix: X (m x n), X^T twice, A, Q
 struct Planes {
-  _Float16 *x, *xt, *xt_next, *a, *q;  // (X^T of this step and of the next)
-  int64_t xs, as;  // from a hi plane to its lo plane
+  Tiled x, xt, xt_next, a, q;  // (X^T of this step and of the next)
 };
 __device__ __forceinline__ Planes planes_of(const OrthogonaliseParams& P, const MatrixGroup& M, int64_t which) {
-  Planes p;
-  p.xs = static_cast<int64_t>(M.mp) * M.np;
-  p.as = static_cast<int64_t>(M.mp) * M.mp;
-  p.x = P.planes + M.planes + which * M.stride;
-  p.xt = p.x + (P.odd ? 4 : 2) * p.xs;
-  p.xt_next = p.x + (P.odd ? 2 : 4) * p.xs;
-  p.a = p.x + 6 * p.xs;
-  p.q = p.a + 2 * p.as;
-  return p;
+  const int64_t xs = 2 * static_cast<int64_t>(M.mp) * M.np, as = 2 * static_cast<int64_t>(M.mp) * M.mp;
+  _Float16* p = P.planes + M.planes + which * M.stride;
+  const int m = M.mp / 16, n = M.np / 16;
+  return {{p, m}, {p + (P.odd ? 2 : 1) * xs, n}, {p + (P.odd ? 1 : 2) * xs, n}, {p + 3 * xs, m}, {p + 3 * xs + as, m}};
 }
 
-// sum of squares of one matrix, kNormBlocks workgroups each (M.first: in matrices; partials by matrix of the launch)
+// sum of squares of one matrix, kNormBlocks workgroups each (M.first: in matrices; partials by matrix of the launch); four loads of a thread at a time
 template <typename E>
-__global__ __launch_bounds__(256) void orthogonalise_norms(const OrthogonaliseParams P) {
-  __shared__ double lds[4];
+__global__ __launch_bounds__(1024) void orthogonalise_norms(const OrthogonaliseParams P) {
+  __shared__ double lds[16];
   int64_t which;
-  const int64_t matrix = blockIdx.x / kNormBlocks, part = blockIdx.x % kNormBlocks;
+  const int64_t matrix = blockIdx.x / kNormBlocks;
+  const uint32_t part = blockIdx.x % kNormBlocks;
   const MatrixGroup M = P.group[find_group(P, matrix, which)];
   const E* in = static_cast<const E*>(M.in) + which * M.in_batch;
   const bool along_n = M.in_column <= M.in_row;  // neighbours in memory to neighbouring threads
-  const int64_t fast = along_n ? M.n : M.m, slow = along_n ? M.m : M.n;
+  const uint32_t fast = along_n ? M.n : M.m, count = static_cast<uint32_t>(M.m) * static_cast<uint32_t>(M.n);  // (at most 2^30)
   const int64_t fast_stride = along_n ? M.in_column : M.in_row, slow_stride = along_n ? M.in_row : M.in_column;
   double sum = 0.0;
-  for (int64_t s = part; s < slow; s += kNormBlocks)
-    for (int64_t f = threadIdx.x; f < fast; f += 256) {
-      const float v = static_cast<float>(in[s * slow_stride + f * fast_stride]);
-      sum += static_cast<double>(v) * static_cast<double>(v);
+  for (uint32_t first = part * 4096; first < count; first += kNormBlocks * 4096) {
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t e = first + 1024 * k + threadIdx.x;
+      v[k] = e < count ? static_cast<float>(in[(e / fast) * slow_stride + (e % fast) * fast_stride]) : 0.0f;
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum += static_cast<double>(v[k]) * static_cast<double>(v[k]);
+  }
   sum = block_sum(sum, lds);
   if (threadIdx.x == 0) P.partials[blockIdx.x] = sum;
 }
@@ -345,24 +368,89 @@ __global__ __launch_bounds__(256) void orthogonalise_split(const OrthogonalisePa
   for (int k = 0; k < 16; ++k) {
     const int e = threadIdx.x + 256 * k, s = e >> 6, f = e & 63;
     const Halves h = split(tile[s][f]), g = split(tile[f][s]);
-    const int64_t ax = static_cast<int64_t>(i0 + s) * M.np + j0 + f, at_t = static_cast<int64_t>(j0 + s) * M.mp + i0 + f;
-    p.x[ax] = h.hi;
-    p.x[p.xs + ax] = h.lo;
-    p.xt[at_t] = g.hi;
-    p.xt[p.xs + at_t] = g.lo;
+    const int64_t ax = p.x.at(i0 + s, j0 + f), at_t = p.xt.at(j0 + s, i0 + f);
+    p.x.p[ax] = h.hi;
+    p.x.p[ax + kLo] = h.lo;
+    p.xt.p[at_t] = g.hi;
+    p.xt.p[at_t + kLo] = g.lo;
   }
 }
 
+// The order of a step's instructions: products with the reads, writes and loads strewn in between.  Left alone the requests come first, every wave's at
+// once, and no product starts before LDS has taken them all.
+template <int PRODUCTS, int READS, int TRANSFERS>
+__device__ __forceinline__ void interleave() {
+  constexpr int kRequests = READS + 2 * TRANSFERS, kEach = PRODUCTS / kRequests > 0 ? PRODUCTS / kRequests : 1;
+#pragma unroll
+  for (int i = 0; i < READS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);      // LDS read
+    __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);  // products
+  }
+#pragma unroll
+  for (int i = 0; i < TRANSFERS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);      // LDS write
+    __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+    __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);      // load from memory
+    __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+  }
+}
+
+// Where the 16-byte piece `piece` of a 64-byte row lies in LDS: the pieces of four rows are exchanged differently in each of the four quarters of a tile, so
+// that the sixteen lanes that a 16-byte read serves at a time - a run of rows, or half of them with the neighbouring piece of the other half - meet
+// sixteen different groups of banks.  (Rows 80 bytes apart are free of conflicts only for the first of these; counters showed half of LDS's time lost.)
+__device__ __forceinline__ int swizzle(int row, int piece) { return piece ^ (-(row >> 2) & 3); }
+
 enum : int { kGram = 0, kPolynomial = 1, kApply = 2 };
 
-// One T x T tile of a product, four waves of T/2 x T/2, k in steps of 32 through two LDS buffers: the next step's operands are on their way from
-// memory while this one's are multiplied.
-template <typename E, int T, int PRODUCT>
-__global__ __launch_bounds__(256) void orthogonalise_product(const OrthogonaliseParams P) {
-  constexpr int kRow = 32 + 8;                   // halfs of a row in LDS: 80 bytes apart, 16 rows in 64 different banks
-  constexpr int kBuffer = 4 * T * kRow;          // L hi, L lo, R hi, R lo
-  constexpr int F = T / 32;                      // 16 x 16 fragments of a wave along each side
-  constexpr int kLoads = T * 32 / 8 / 256 > 0 ? T * 32 / 8 / 256 : 1;  // 16-byte loads per thread and plane
+// The t-th tile: by bands of eight columns of tiles, row by row within a band, so that the run of tiles that one XCD works on is compact and its L2 is
+// asked for few rows of either operand.  Of a symmetric product, the upper triangle.
+template <bool SYMMETRIC>
+__device__ __forceinline__ void find_tile(int t, int rows, int columns, int& ti, int& tj) {
+  constexpr int kBand = 8;
+  for (int c0 = 0;; c0 += kBand) {
+    const int width = columns - c0 < kBand ? columns - c0 : kBand;
+    if (!SYMMETRIC) {
+      if (t < rows * width) {
+        ti = t / width;
+        tj = c0 + t % width;
+        return;
+      }
+      t -= rows * width;
+    } else {
+      if (t < c0 * width) {  // the rows above the band's own square have all of the band
+        ti = t / width;
+        tj = c0 + t % width;
+        return;
+      }
+      t -= c0 * width;
+      for (ti = c0; ti < c0 + width; ++ti) {
+        const int n = c0 + width - ti;
+        if (t < n) {
+          tj = ti + t;
+          return;
+        }
+        t -= n;
+      }
+    }
+  }
+}
+
+// One T x T tile of a product, WAVES waves of T/2 x 2 T/WAVES, k in steps of 32.  Three products of matrix instructions per step of one split
+// operand pair: 128 x 128 with eight waves has 768 cycles of them per SIMD and step, against 650 cycles of LDS (96 KB read, 32 KB written).
+// Measured at 2048 x 2048: 41 us for a symmetric product (136 workgroups on 256 compute units), 50 for the full one, where the matrix instructions
+// alone - the loop without its reads, writes and loads - take 32 and 36; 64 x 64 tiles take 46 and 70 there, but 11 and 13 us instead of 21 and 23
+// at 1024 x 1024, where 128 x 128 ones are too few.  What brought it there from 70 us: a barrier that does not wait for loads from memory (60), the
+// requests strewn between the products (53), LDS without bank conflicts (44).  What bounds it now: LDS writes and the barrier per step.
+template <typename E, int T, int WAVES, int PRODUCT>
+__global__ __launch_bounds__(64 * WAVES, 2) void orthogonalise_product(const OrthogonaliseParams P) {
+  constexpr int kRow = 32;                       // halfs of a row in LDS
+  constexpr int kPlane = T * kRow, kBuffer = 4 * kPlane;  // L hi, L lo, R hi, R lo
+  constexpr int FI = T / 32, FJ = 2 * T / WAVES / 16;  // 16 x 16 fragments of a wave along rows and columns
+  constexpr int kSweep = 16 * WAVES;             // rows that the workgroup loads at once: a tile per wave
+  constexpr int kTiles = T / kSweep, kTransfers = 4 * kTiles;  // of an operand that a wave loads; of both, in halves
+  // steps whose operands wait in registers or are on their way: even, since fragments alternate with it, and a divisor of every number of steps
+  constexpr int kAhead = T / 32;
+  static_assert(kTiles >= 1 && FJ >= 1 && kAhead % 2 == 0, "a tile has work for every wave");
   extern __shared__ _Float16 lds_product[];
   // neighbouring tiles to the same XCD (workgroups go round the eight of them), so that its L2 sees an operand's rows again
   const int64_t blocks = P.blocks, per = (blocks + 7) / 8;
@@ -370,86 +458,117 @@ __global__ __launch_bounds__(256) void orthogonalise_product(const Orthogonalise
   if (id >= blocks) return;
   int64_t at;
   const MatrixGroup M = P.group[find_group(P, id, at)];
-  const int rows = M.mp / T, columns = PRODUCT == kApply ? M.np / T : rows;
+  const int rows = M.mp / T, columns = (PRODUCT == kApply ? M.np : M.mp) / T;
   const int tiles = PRODUCT == kApply ? rows * columns : rows * (rows + 1) / 2;
   const int64_t which = at / tiles;
-  int t = static_cast<int>(at % tiles), ti, tj;
-  if (PRODUCT == kApply) {
-    ti = t % rows;
-    tj = t / rows;
-  } else {  // the upper triangle, row by row
-    ti = 0;
-    while (t >= rows - ti) t -= rows - ti, ++ti;
-    tj = ti + t;
-  }
+  int ti, tj;
+  find_tile<PRODUCT != kApply>(static_cast<int>(at % tiles), rows, columns, ti, tj);
   const Planes p = planes_of(P, M, which);
   const int kp = PRODUCT == kGram ? M.np : M.mp;  // both operands' row length
-  const _Float16* l = (PRODUCT == kGram ? p.x : PRODUCT == kPolynomial ? p.a : p.q) + static_cast<int64_t>(ti) * T * kp;
-  const _Float16* r = (PRODUCT == kGram ? p.x : PRODUCT == kPolynomial ? p.a : p.xt) + static_cast<int64_t>(tj) * T * kp;
-  const int64_t ls = PRODUCT == kGram ? p.xs : p.as, rs = PRODUCT == kPolynomial ? p.as : p.xs;
+  const Tiled left = PRODUCT == kGram ? p.x : PRODUCT == kPolynomial ? p.a : p.q;
+  const Tiled right = PRODUCT == kGram ? p.x : PRODUCT == kPolynomial ? p.a : p.xt;
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int row = T / 2 * (wave >> 1), column = T / 2 * (wave & 1);
-  float4v acc[F][F];
+  const int row = T / 2 * (wave & 1), column = 16 * FJ * (wave >> 1);
+  float4v acc[FI][FJ];
 #pragma unroll
-  for (int i = 0; i < F; ++i)
+  for (int i = 0; i < FI; ++i)
 #pragma unroll
-    for (int j = 0; j < F; ++j) acc[i][j] = float4v{0.f, 0.f, 0.f, 0.f};
-  half8 stage[4][kLoads];
-  const int load_row = threadIdx.x / 4, load_k = threadIdx.x % 4 * 8;  // 64 rows of 32 halfs per sweep
-  auto fetch = [&](int k) {
+    for (int j = 0; j < FJ; ++j) acc[i][j] = float4v{0.f, 0.f, 0.f, 0.f};
+  // kAhead steps' operands wait in registers or are on their way: a step takes a third of a memory latency
+  half8 stage[kAhead][kTransfers];
+  const int load_row = threadIdx.x / 4, load_k = 8 * swizzle(load_row, threadIdx.x % 4);  // a wave's lanes walk through one tile
+  const _Float16* l = left.p + static_cast<int64_t>(ti) * (T / 16) * 1024 + wave * 1024 + lane * 8;
+  const _Float16* r = right.p + static_cast<int64_t>(tj) * (T / 16) * 1024 + wave * 1024 + lane * 8;
+  const int64_t l_step = left.row_tiles * 1024, r_step = right.row_tiles * 1024;
+  const int steps = kp / 32;
+  // (steps behind the last fetch the last one again and nobody looks: without branches around loads the compiler knows which ones a wait is for)
+  auto fetch = [&](int ahead, half8 (&to)[kTransfers]) {
+    const int step = ahead < steps ? ahead : steps - 1;
+    const _Float16 *lp = l + step * l_step, *rp = r + step * r_step;
 #pragma unroll
-    for (int s = 0; s < kLoads; ++s) {
-      const int64_t off = static_cast<int64_t>(load_row + 64 * s) * kp + k + load_k;
-      stage[0][s] = *reinterpret_cast<const half8*>(l + off);
-      stage[1][s] = *reinterpret_cast<const half8*>(l + ls + off);
-      stage[2][s] = *reinterpret_cast<const half8*>(r + off);
-      stage[3][s] = *reinterpret_cast<const half8*>(r + rs + off);
+    for (int s = 0; s < kTiles; ++s) {
+      to[4 * s] = *reinterpret_cast<const half8*>(lp + s * WAVES * 1024);
+      to[4 * s + 1] = *reinterpret_cast<const half8*>(lp + s * WAVES * 1024 + kLo);
+      to[4 * s + 2] = *reinterpret_cast<const half8*>(rp + s * WAVES * 1024);
+      to[4 * s + 3] = *reinterpret_cast<const half8*>(rp + s * WAVES * 1024 + kLo);
     }
   };
-  auto put = [&](int buffer) {
+  auto put = [&](int buffer, const half8 (&from)[kTransfers]) {
+    _Float16* base = lds_product + buffer * kBuffer + load_row * kRow + load_k;
 #pragma unroll
-    for (int plane = 0; plane < 4; ++plane)
+    for (int s = 0; s < kTiles; ++s)
 #pragma unroll
-      for (int s = 0; s < kLoads; ++s)
-        *reinterpret_cast<half8*>(lds_product + buffer * kBuffer + plane * T * kRow + (load_row + 64 * s) * kRow + load_k) = stage[plane][s];
+      for (int plane = 0; plane < 4; ++plane) *reinterpret_cast<half8*>(base + plane * kPlane + s * kSweep * kRow) = from[4 * s + plane];
   };
-  fetch(0);
-  put(0);
-  __syncthreads();
-  int buffer = 0;
-  for (int k = 0; k < kp; k += 32, buffer ^= 1) {
-    const bool more = k + 32 < kp;
-    if (more) fetch(k + 32);
-    const _Float16* base = lds_product + buffer * kBuffer + (lane & 15) * kRow + 8 * (lane >> 4);
-    half8 lh[F], ll[F];
+  struct Fragments {
+    half8 lh[FI], ll[FI], rh[FJ], rl[FJ];
+  };
+  auto read = [&](int buffer, Fragments& f) {
+    const _Float16* base = lds_product + buffer * kBuffer + (lane & 15) * kRow + 8 * swizzle(lane & 15, lane >> 4);
 #pragma unroll
-    for (int i = 0; i < F; ++i) {
-      lh[i] = *reinterpret_cast<const half8*>(base + (row + 16 * i) * kRow);
-      ll[i] = *reinterpret_cast<const half8*>(base + T * kRow + (row + 16 * i) * kRow);
+    for (int j = 0; j < FJ; ++j) f.rl[j] = *reinterpret_cast<const half8*>(base + 3 * kPlane + (column + 16 * j) * kRow);
+#pragma unroll
+    for (int i = 0; i < FI; ++i) f.lh[i] = *reinterpret_cast<const half8*>(base + (row + 16 * i) * kRow);
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) f.rh[j] = *reinterpret_cast<const half8*>(base + 2 * kPlane + (column + 16 * j) * kRow);
+#pragma unroll
+    for (int i = 0; i < FI; ++i) f.ll[i] = *reinterpret_cast<const half8*>(base + kPlane + (row + 16 * i) * kRow);
+  };
+#pragma unroll
+  for (int d = 0; d < kAhead; ++d) {
+    fetch(d, stage[d]);
+    asm volatile("" ::: "memory");  // (in their order: a wait in the loop counts the loads behind the one it is for)
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  put(0, stage[0]);
+  fetch(kAhead, stage[0]);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  put(1, stage[1]);
+  fetch(kAhead + 1, stage[1]);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  lds_barrier();
+  // Step s multiplies the fragments it finds in registers, while those of step s + 1 come from one LDS buffer, step s + 2 is put into another - the
+  // third is the one that step s itself came from - and step s + 2 + kAhead is requested from memory.
+  Fragments fragments[2];
+  read(0, fragments[0]);
+  int next = 1, fill = 2;
+  for (int first = 0; first < steps; first += kAhead) {
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d) {
+      read(next, fragments[(d + 1) & 1]);
+      put(fill, stage[(d + 2) % kAhead]);
+      fetch(first + d + 2 + kAhead, stage[(d + 2) % kAhead]);
+      const Fragments& f = fragments[d & 1];
+#pragma unroll
+      for (int j = 0; j < FJ; ++j)
+#pragma unroll
+        for (int i = 0; i < FI; ++i) acc[i][j] = mfma(f.lh[i], f.rl[j], acc[i][j]);
+#pragma unroll
+      for (int j = 0; j < FJ; ++j)
+#pragma unroll
+        for (int i = 0; i < FI; ++i) acc[i][j] = mfma(f.lh[i], f.rh[j], acc[i][j]);
+#pragma unroll
+      for (int j = 0; j < FJ; ++j)
+#pragma unroll
+        for (int i = 0; i < FI; ++i) acc[i][j] = mfma(f.ll[i], f.rh[j], acc[i][j]);
+      interleave<3 * FI * FJ, 2 * (FI + FJ), kTransfers>();
+      __builtin_amdgcn_sched_barrier(0);  // (no product sinks below the barrier, in front of the next step's requests)
+      next = fill;
+      fill = fill == 2 ? 0 : fill + 1;
+      lds_barrier();
     }
-#pragma unroll
-    for (int j = 0; j < F; ++j) {
-      const half8 rh = *reinterpret_cast<const half8*>(base + 2 * T * kRow + (column + 16 * j) * kRow);
-      const half8 rl = *reinterpret_cast<const half8*>(base + 3 * T * kRow + (column + 16 * j) * kRow);
-#pragma unroll
-      for (int i = 0; i < F; ++i) acc[i][j] = mfma(lh[i], rl, acc[i][j]);
-#pragma unroll
-      for (int i = 0; i < F; ++i) acc[i][j] = mfma(ll[i], rh, acc[i][j]);
-#pragma unroll
-      for (int i = 0; i < F; ++i) acc[i][j] = mfma(lh[i], rh, acc[i][j]);
-    }
-    if (more) put(buffer ^ 1);
-    __syncthreads();
   }
 
   const int r0 = 4 * (lane >> 4), c0 = lane & 15;
   if (PRODUCT == kApply && P.last) {
     E* out = static_cast<E*>(M.out) + which * M.out_batch;
 #pragma unroll
-    for (int i = 0; i < F; ++i)
+    for (int i = 0; i < FI; ++i)
 #pragma unroll
-      for (int j = 0; j < F; ++j)
+      for (int j = 0; j < FJ; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int64_t y = ti * T + row + 16 * i + r0 + e, z = tj * T + column + 16 * j + c0;
@@ -458,15 +577,16 @@ __global__ __launch_bounds__(256) void orthogonalise_product(const Orthogonalise
     return;
   }
 #pragma unroll
-  for (int i = 0; i < F; ++i)
+  for (int i = 0; i < FI; ++i)
 #pragma unroll
-    for (int j = 0; j < F; ++j) {
+    for (int j = 0; j < FJ; ++j) {
       const int y = ti * T + row + 16 * i + r0, z = tj * T + column + 16 * j + c0;  // four rows y.., one column z
       half4 hi, lo;
       half4 ah, al;
       if (PRODUCT == kPolynomial) {  // A at (y + e, z) is A at (z, y + e)
-        ah = *reinterpret_cast<const half4*>(p.a + static_cast<int64_t>(z) * M.mp + y);
-        al = *reinterpret_cast<const half4*>(p.a + p.as + static_cast<int64_t>(z) * M.mp + y);
+        const _Float16* a = p.a.p + p.a.at(z, y);
+        ah = *reinterpret_cast<const half4*>(a);
+        al = *reinterpret_cast<const half4*>(a + kLo);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -483,18 +603,17 @@ __global__ __launch_bounds__(256) void orthogonalise_product(const Orthogonalise
         lo[e] = h.lo;
       }
       // turned, four neighbours at once; and as it stands, one by one (not for a tile on the diagonal, which is its own mirror image)
-      _Float16* turned = PRODUCT == kGram ? p.a : PRODUCT == kPolynomial ? p.q : p.xt_next;
-      _Float16* plain = PRODUCT == kGram ? p.a : PRODUCT == kPolynomial ? p.q : p.x;
-      const int64_t lo_plane = PRODUCT == kApply ? p.xs : p.as;
-      const int64_t to = static_cast<int64_t>(z) * M.mp + y;
-      *reinterpret_cast<half4*>(turned + to) = hi;
-      *reinterpret_cast<half4*>(turned + lo_plane + to) = lo;
+      const Tiled turned = PRODUCT == kGram ? p.a : PRODUCT == kPolynomial ? p.q : p.xt_next;
+      _Float16* to = turned.p + turned.at(z, y);
+      *reinterpret_cast<half4*>(to) = hi;
+      *reinterpret_cast<half4*>(to + kLo) = lo;
       if (PRODUCT == kApply || ti != tj) {
-        const int pitch = PRODUCT == kApply ? M.np : M.mp;
+        const Tiled plain = PRODUCT == kApply ? p.x : turned;
+        _Float16* as_is = plain.p + plain.at(y, z);  // (y is a multiple of four: y + e stays within its tile)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          plain[static_cast<int64_t>(y + e) * pitch + z] = hi[e];
-          plain[lo_plane + static_cast<int64_t>(y + e) * pitch + z] = lo[e];
+          as_is[32 * e] = hi[e];
+          as_is[32 * e + kLo] = lo[e];
         }
       }
     }
