@@ -126,10 +126,18 @@ __device__ __forceinline__ float4v tile_product(const float* l, const float* r, 
 struct SmallTile {
   int row, column;  // of this wave's tile
   int r0, c0;       // an accumulator's element r of this lane is at (row + r0 + r, column + c0)
-  __device__ __forceinline__ SmallTile() {
+  // SYMMETRIC: the ten tiles of the upper triangle to the first ten waves - at most three on a SIMD, which would have to work on four of a full product
+  __device__ __forceinline__ SmallTile(bool symmetric) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    row = 16 * (wave >> 2);
-    column = 16 * (wave & 3);
+    int i = wave >> 2, j = wave & 3;
+    if (symmetric) {
+      i = 0;
+      j = wave;
+      while (i < 4 && j >= 4 - i) j -= 4 - i, ++i;
+      j += i;
+    }
+    row = 16 * i;
+    column = 16 * j;
     r0 = 4 * (lane >> 4);
     c0 = lane & 15;
   }
@@ -139,9 +147,13 @@ struct SmallTile {
 #pragma unroll
     for (int r = 0; r < 4; ++r) plane[small_at(row + r0 + r, column + c0)] = v[r];
   }
+  __device__ __forceinline__ void put_symmetric(float* plane, float4v v) const {
+    put_turned(plane, v);
+    if (row != column) put(plane, v);
+  }
 };
 
-// Q from A, both in LDS; every wave calls it, mp a multiple of 16
+// Q from A, both in LDS; every wave calls it with its tile of a symmetric product, mp a multiple of 16
 __device__ __forceinline__ void small_polynomial(const OrthogonaliseParams& P, const SmallTile& T, const float* am, float* q, int mp) {
   if (T.row < mp && T.column < mp) {
     const float4v square = tile_product(am, am, T.row, T.column, mp);
@@ -152,7 +164,7 @@ __device__ __forceinline__ void small_polynomial(const OrthogonaliseParams& P, c
       v[r] = __builtin_fmaf(P.b, av[r], P.c * square[r]);
       if (T.row + T.r0 + r == T.column + T.c0) v[r] += P.a;
     }
-    T.put_turned(q, v);
+    T.put_symmetric(q, v);
   }
 }
 
@@ -183,13 +195,13 @@ __global__ __launch_bounds__(1024) void orthogonalise_small(const OrthogonaliseP
     xt[small_at(j, i)] = scaled;
   }
   __syncthreads();
-  const SmallTile T;
-  const bool square = T.row < M.mp && T.column < M.mp, flat = T.row < M.mp && T.column < M.np;
+  const SmallTile T(false), S(true);
+  const bool square = S.row < M.mp && S.column < M.mp, flat = T.row < M.mp && T.column < M.np;
   float4v acc = {0.f, 0.f, 0.f, 0.f};
   for (int step = 0; step < P.steps; ++step) {
-    if (square) T.put_turned(am, tile_product(x, x, T.row, T.column, M.np));  // (symmetric)
+    if (square) S.put_symmetric(am, tile_product(x, x, S.row, S.column, M.np));
     __syncthreads();
-    small_polynomial(P, T, am, q, M.mp);
+    small_polynomial(P, S, am, q, M.mp);
     __syncthreads();
     if (flat) acc = tile_product(q, xt, T.row, T.column, M.mp);
     if (step + 1 == P.steps) break;
@@ -226,9 +238,9 @@ __global__ __launch_bounds__(1024) void orthogonalise_flat(const OrthogonalisePa
   const float* before = all_shares + (launch & 1 ? 0 : 1) * static_cast<int64_t>(kMostShares) * 4096;
   float* after = all_shares + (launch & 1 ? 1 : 0) * static_cast<int64_t>(kMostShares) * 4096;
   float *x = lds_small, *xt = x + kSmallPlane, *am = xt + kSmallPlane, *q = am + kSmallPlane;
-  const SmallTile T;
+  const SmallTile T(false), S(true);
   const int mp = M.mp;
-  const bool square = T.row < mp && T.column < mp, flat = T.row < mp;
+  const bool square = S.row < mp && S.column < mp, flat = T.row < mp;
   double inverse = 0.0;
   if (launch == 0) {
     int64_t matrix = which;
@@ -242,7 +254,7 @@ __global__ __launch_bounds__(1024) void orthogonalise_flat(const OrthogonalisePa
     for (int w = 0; w < shares; ++w) a += *reinterpret_cast<const float4v*>(before + w * 4096 + i * 64 + j);
     *reinterpret_cast<float4v*>(am + small_at(i, j)) = a;
     __syncthreads();
-    small_polynomial(P, T, am, q, mp);
+    small_polynomial(P, S, am, q, mp);
   }
   const E* in = static_cast<const E*>(M.in) + which * M.in_batch;
   E* out = static_cast<E*>(M.out) + which * M.out_batch;
@@ -284,10 +296,18 @@ __global__ __launch_bounds__(1024) void orthogonalise_flat(const OrthogonalisePa
     }
     if (P.last) continue;
     __syncthreads();
-    if (square) gram += tile_product(x, x, T.row, T.column, 64);
+    if (square) gram += tile_product(x, x, S.row, S.column, 64);
   }
   if (P.last) return;
-  *reinterpret_cast<float4v*>(after + share * 4096 + (T.column + T.c0) * 64 + T.row + T.r0) = gram;  // (zeros where there is no tile)
+  // the whole 64 x 64: what this share has of A, its mirror image, and zeros where A has no tile
+  if (S.row < 64) {
+    float* share_of = after + share * 4096;
+    *reinterpret_cast<float4v*>(share_of + (S.column + S.c0) * 64 + S.row + S.r0) = gram;
+    if (S.row != S.column) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) share_of[(S.row + S.r0 + r) * 64 + S.column + S.c0] = gram[r];
+    }
+  }
 }
 
 // ---- larger ------------------------------------------------------------------------------------------------------------------------

@@ -34,10 +34,10 @@ def orthogonalise(updates: Union[torch.Tensor, Sequence[torch.Tensor]], *, steps
     steps = int(steps)
     if steps < 1:
         raise ValueError(f"steps = {steps}: at least one product is needed")
-    coefficients = [float(c) for c in coefficients]
+    coefficients, eps = [float(c) for c in coefficients], float(eps)
     if len(coefficients) != 3:
         raise ValueError(f"{len(coefficients)} coefficients: three (a, b, c) are needed")
-    outs, kept, described = [], [], []
+    outs, kept, described, needs_workspace = [], [], [], False
     tracked = torch.is_grad_enabled()
     for t in given:
         require(t, "updates", device, (dtype,))
@@ -48,24 +48,30 @@ def orthogonalise(updates: Union[torch.Tensor, Sequence[torch.Tensor]], *, steps
             raise ValueError("orthogonalise is not differentiable: detach the updates")
         out = torch.empty(shape, dtype=dtype, device=device)
         outs.append(out)
+        if not t.numel():
+            continue
+        rows, columns = shape[-2:]
         if len(shape) == 2:
-            rows, columns = shape
             batch, strides = 1, (0,) + t.stride()
         else:
-            rows, columns = shape[-2:]
-            t = t.reshape(-1, rows, columns) if t.numel() else t  # (a copy only where the batch axes do not fold)
-            batch, strides = t.shape[0], t.stride()[-3:]
-        if rows and columns and t.numel():
+            t = t.reshape(-1, rows, columns)  # (a copy only where the batch axes do not fold)
+            batch, strides = t.shape[0], t.stride()
             kept.append(t)
-            described.append((t.data_ptr(), out.data_ptr(), rows, columns, batch, strides, (rows * columns, columns, 1)))
+        needs_workspace = needs_workspace or rows > 64 or columns > 64
+        described.append((t.data_ptr(), out.data_ptr(), rows, columns, batch, strides, (rows * columns, columns, 1)))
     count = len(described)
     if count:
         matrices = (_native.MbtMatrix * count)(*described)
         lib = _native.load_library()
-        size = lib.mbt_orthogonalise_workspace(count, matrices)
-        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        _native.check(lib.mbt_orthogonalise(device.index, DTYPES[dtype], count, matrices, steps, (ctypes.c_double * 3)(*coefficients), float(eps),
-                                            workspace.data_ptr() if size else None, size, current_stream(device.index)))
+        size, address = 0, None
+        if needs_workspace:
+            size = lib.mbt_orthogonalise_workspace(count, matrices)
+            workspace = torch.empty(size, dtype=torch.uint8, device=device)
+            address = workspace.data_ptr()
+        code = lib.mbt_orthogonalise(device.index, DTYPES[dtype], count, matrices, steps, (ctypes.c_double * 3)(*coefficients), eps, address, size,
+                                     current_stream(device.index))
+        if code < 0:
+            _native.check(code)
     return outs[0] if single else outs
 
 
