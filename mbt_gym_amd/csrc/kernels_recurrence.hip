@@ -130,8 +130,8 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
 
   // Columns per thread: one float32 or two 16-bit elements, so that a wave's row is 256 bytes and the time axis can be cut finely; a recording with
   // columns enough for every wave of the chip to have 64 x 16 bytes of its own is walked forwards in such vectors, alone.
-  const int pair = inner_contiguous && size == 2 && P.inner >= 2 ? 2 : 1;
-  const bool wide = !backward && inner_contiguous && P.outer * (P.inner / vector) >= chip;
+  const int pair = inner_contiguous && size == 2 && P.inner % 2 == 0 ? 2 : 1;
+  const bool wide = !backward && inner_contiguous && P.inner % vector == 0 && P.outer * (P.inner / vector) >= chip;
   const int v = wide ? vector : pair;
   const int base = wide ? kColumnsWide : pair == 2 ? kColumnsPair : kColumnsScalar;
   P.vectors_per_outer = ceil_div(P.inner, v);
@@ -141,30 +141,40 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
   if (parallel > ceil_div(steps, chunk)) parallel = ceil_div(steps, chunk);
   if (wide || parallel <= 2) {
     plan.which = base + kAlone;
+    if (wide && batch * steps * static_cast<int64_t>(size) * count > (int64_t{256} << 20)) plan.which = base + kStreamed;  // (beyond the last cache)
     plan.threads = 256;
     plan.blocks = ceil_div(P.vectors, 256);
+    P.whole_blocks = 1;  // (a lane without a column has left)
     return MBT_OK;
   }
-  // a workgroup takes 64 column vectors (256 bytes of a row), fewer only when there are fewer
+  // A workgroup takes 64 column vectors (256 bytes of a row) and up to 1024 threads' worth of chunks of time, a tile.  Where that makes fewer workgroups
+  // than compute units, and
+  //   - the walk is at least four tiles long: the axis is cut into segments over workgroups as well (64 columns x 65536 steps, float32 logit
+  //     form: 25 us forward; with 16 columns a workgroup and fewer segments 32)
+  //   - it is shorter: a workgroup takes fewer columns, down to 16, or 8 if only that makes the walk one tile (1000 lanes x 200: 8.1 -> 5.6 us; 1024
+  //     columns x 500, bfloat16: 30 -> 11)
   int columns_log2 = 6;
   while (columns_log2 > 0 && (int64_t{1} << (columns_log2 - 1)) >= P.vectors) --columns_log2;
-  int chunks_log2 = log2_ceil(parallel);
-  if (chunks_log2 > 10 - columns_log2) chunks_log2 = 10 - columns_log2;
-  if (chunks_log2 + columns_log2 < 6) chunks_log2 = 6 - columns_log2;
-  const int64_t chunks = int64_t{1} << chunks_log2, columns = int64_t{1} << columns_log2;
-  P.lanes_log2 = columns_log2;
-  P.column_blocks = ceil_div(P.vectors, columns);
-  // segments: only where one workgroup per column group leaves most of the chip idle AND the walk is long
-  const int64_t tile = chunks * chunk;
-  if (P.column_blocks < 128 && steps >= 4 * tile) {
-    int64_t want = 256 / P.column_blocks;
-    const int64_t most = steps / tile;
+  const int chunks_wanted = log2_ceil(parallel);
+  auto chunks_with = [&](int columns) {
+    int chunks = chunks_wanted < 10 - columns ? chunks_wanted : 10 - columns;
+    return chunks + columns < 6 ? 6 - columns : chunks;
+  };
+  auto tile_with = [&](int columns) { return (int64_t{1} << chunks_with(columns)) * chunk; };
+  auto blocks_with = [&](int columns) { return ceil_div(P.vectors, int64_t{1} << columns); };
+  if (blocks_with(columns_log2) < 128 && steps >= 4 * tile_with(columns_log2)) {
+    const int64_t tile = tile_with(columns_log2), most = ceil_div(steps, tile);
+    int64_t want = 256 / blocks_with(columns_log2);
     want = want < most ? want : most;
-    if (want > 1) {
-      P.segment = ceil_div(ceil_div(steps, want), tile) * tile;
-      P.segments = static_cast<int32_t>(ceil_div(steps, P.segment));
-    }
+    P.segment = ceil_div(ceil_div(steps, want), tile) * tile;
+    P.segments = static_cast<int32_t>(ceil_div(steps, P.segment));
+  } else {
+    while (columns_log2 > 3 && blocks_with(columns_log2) < 256 && (columns_log2 > 4 || steps > tile_with(columns_log2))) --columns_log2;
   }
+  const int64_t chunks = int64_t{1} << chunks_with(columns_log2), columns = int64_t{1} << columns_log2;
+  P.lanes_log2 = columns_log2;
+  P.column_blocks = blocks_with(columns_log2);
+  P.whole_blocks = P.vectors % columns == 0;
   plan.which = base + kJoined;
   plan.threads = static_cast<unsigned>(chunks * columns);
   plan.blocks = P.column_blocks * P.segments;

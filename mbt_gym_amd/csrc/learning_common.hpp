@@ -65,6 +65,35 @@ __device__ __forceinline__ void store_pack(E* p, const Pack<E, V>& v) {
   __builtin_memcpy(p, &v, sizeof v);
 }
 
+template <int ALIGNED>
+struct Words;
+template <>
+struct Words<4> {
+  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4)));
+};
+template <>
+struct Words<2> {
+  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2)));
+};
+// The same past the caches, for arrays that are larger than they and read or written once: what they would drive out is worth more.
+template <typename E, int V>
+__device__ __forceinline__ Pack<E, V> stream_load_pack(const E* p) {
+  static_assert(sizeof(E) * V == 16, "one 16-byte access");
+  typedef typename Words<alignof(E)>::type words;
+  const words w = __builtin_nontemporal_load(reinterpret_cast<const words*>(p));
+  Pack<E, V> v;
+  __builtin_memcpy(&v, &w, 16);
+  return v;
+}
+template <typename E, int V>
+__device__ __forceinline__ void stream_store_pack(E* p, const Pack<E, V>& v) {
+  static_assert(sizeof(E) * V == 16, "one 16-byte access");
+  typedef typename Words<alignof(E)>::type words;
+  words w;
+  __builtin_memcpy(&w, &v, 16);
+  __builtin_nontemporal_store(w, reinterpret_cast<words*>(p));
+}
+
 inline size_t dtype_size(int dtype) { return dtype == MBT_FLOAT32 ? 4 : 2; }
 inline bool dtype_known(int dtype) { return dtype == MBT_FLOAT32 || dtype == MBT_BFLOAT16 || dtype == MBT_FLOAT16; }
 

@@ -45,6 +45,7 @@ struct RecurrenceParams {
   int64_t segment;                     // steps per segment
   int32_t segments;
   int32_t lanes_log2;     // columns: column vectors per workgroup; rows: lanes per row
+  int32_t whole_blocks;   // columns: no workgroup has lanes behind the last column
   int32_t batch_swapped;  // initial / final are (outer, inner) of the CALLER: 1 when the kernel's axes are exchanged
   int64_t column_blocks;
   // the constant gate as a float32 pair (0.99 is not a float32 number, and its error would be made at every step), and the powers of the
@@ -84,7 +85,6 @@ __device__ __forceinline__ void sigmoid_pair(float k, float& f, float& i) {
   const float q = e * r;
   f = k >= 0.0f ? r : q;
   i = k >= 0.0f ? q : r;
-  if (k != k) f = i = k;
 }
 
 // what multiplies the state (unless a reset drops it) and what multiplies the input; g is turned in place into the former
@@ -99,49 +99,39 @@ __device__ __forceinline__ void gate(const RecurrenceParams& P, float& g, float&
   }
 }
 
-// Steps of a chunk, held in registers: 16 elements of each array, so that a thread of a 1024-thread workgroup stays within its 128 registers - the
-// backward pass of the logit form holds four arrays over the join and takes half of that - and twice as many for a thread that walks alone
-// forwards with whole vectors.
+// Steps of a chunk, held in registers: 16 elements of each array, so that a thread stays within the 128 registers of four waves per SIMD - the
+// backward pass, where it holds four arrays at once, takes half of that.  (Rewards-to-go of 2^20 x 200 with 16, 32 and 64 elements: 332, 346, 380 us.)
 constexpr int chunk_steps(int form, bool backward, int v, bool alone) {
-  if (v > 2) return 32 / v;
-  return (backward && form == kGateLogit && !alone ? 8 : 16) / v;
+  return (backward && (form == kGateLogit || (alone && form == kGateValue)) ? 8 : 16) / v;
 }
 
 // ---- columns -----------------------------------------------------------------------------------------------------------------------
 // MODE: whole time axis in one thread (kAlone), cut over the threads of the workgroup (kJoined; after kComposites when there are segments).
 enum : int { kAlone = 0, kJoined = 1, kComposites = 2 };
+constexpr int kStreamed = 1;  // + kColumnsWide: past the caches
 
-template <typename E, int V>
+template <typename E, int V, bool STREAM>
 struct Column {
-  int64_t o, i;
-  int nv;  // valid columns of the V (0: a lane without work)
+  int64_t o, i;  // (the V columns of a thread are all there: the host takes V = 1 where V does not divide the axis)
 
   // address at step s; the next step's is t.st further (walked, not recomputed: an address per step and array would not fit the registers)
   __device__ __forceinline__ E* at(const Axis& t, int64_t s) const { return static_cast<E*>(t.p) + o * t.so + s * t.st + i * t.si; }
-  __device__ __forceinline__ void load(const E* p, float (&out)[V]) const {
-    if (nv == V) {
-      const Pack<E, V> v = load_pack<E, V>(p);
+  __device__ __forceinline__ static void load(const E* p, float (&out)[V]) {
+    Pack<E, V> v;
+    if constexpr (STREAM) v = stream_load_pack<E, V>(p);
+    else v = load_pack<E, V>(p);
 #pragma unroll
-      for (int j = 0; j < V; ++j) out[j] = static_cast<float>(v.e[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) out[j] = j < nv ? static_cast<float>(p[j]) : 0.0f;
-    }
+    for (int j = 0; j < V; ++j) out[j] = static_cast<float>(v.e[j]);
   }
-  __device__ __forceinline__ void store(E* p, const float (&in)[V]) const {
-    if (nv == V) {
-      Pack<E, V> v;
+  __device__ __forceinline__ static void store(E* p, const float (&in)[V]) {
+    Pack<E, V> v;
 #pragma unroll
-      for (int j = 0; j < V; ++j) v.e[j] = static_cast<E>(in[j]);
-      store_pack<E, V>(p, v);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (j < nv) p[j] = static_cast<E>(in[j]);
-    }
+    for (int j = 0; j < V; ++j) v.e[j] = static_cast<E>(in[j]);
+    if constexpr (STREAM) stream_store_pack<E, V>(p, v);
+    else store_pack<E, V>(p, v);
   }
   __device__ __forceinline__ bool flag(const Axis& t, int64_t s, int j) const {
-    return j < nv && static_cast<const uint8_t*>(t.p)[o * t.so + s * t.st + (i + j) * t.si] != 0;
+    return static_cast<const uint8_t*>(t.p)[o * t.so + s * t.st + (i + j) * t.si] != 0;
   }
   // (outer, inner) float32 of the caller
   __device__ __forceinline__ int64_t batch(const RecurrenceParams& P, int j) const {
@@ -149,7 +139,7 @@ struct Column {
   }
   __device__ __forceinline__ void load_batch(const RecurrenceParams& P, const float* p, float (&out)[V]) const {
 #pragma unroll
-    for (int j = 0; j < V; ++j) out[j] = p != nullptr && j < nv ? p[batch(P, j)] : 0.0f;
+    for (int j = 0; j < V; ++j) out[j] = p != nullptr ? p[batch(P, j)] : 0.0f;
   }
 };
 
@@ -175,9 +165,13 @@ __device__ __forceinline__ void join_chunks(Composite (&mine)[V], Composite (&ca
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     Composite front = carry[j];
-    for (int w = 0; w < wave; ++w) {
-      const float2 c = lds[((w + 1) * V + j) * columns + column];
-      front = then(front, {c.x, c.y});
+    for (int w = 0; w < wave; w += 4) {  // (four reads at a time: one after the other, each would wait for the one before it)
+      float2 c[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] = lds[((w + i < wave ? w + i + 1 : 1) * V + j) * columns + column];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (w + i < wave) front = then(front, {c[i].x, c[i].y});
     }
     mine[j] = then(front, mine[j]);
     if (more && wave == waves - 1 && lane >= 64 - columns) {
@@ -196,8 +190,158 @@ __device__ __forceinline__ void join_chunks(Composite (&mine)[V], Composite (&ca
   }
 }
 
-template <typename E, int FORM, int V, int K, bool BACKWARD, int MODE>
-__global__ __launch_bounds__(MODE == kAlone ? 256 : 1024) void recurrence_columns(const RecurrenceParams P) {
+// The K steps of one chunk in registers: loaded, joined with the other chunks of the workgroup, walked, stored.  FULL: all K steps are there - no
+// instruction of the chunk looks at n.
+template <typename E, int FORM, int V, int K, bool BACKWARD, int MODE, bool FULL, bool STREAM>
+__device__ __forceinline__ void walk_chunk(const RecurrenceParams& P, const Column<E, V, STREAM>& col, int64_t s0, int n, bool more, Composite (&carry)[V], float2* lds) {
+  constexpr bool kStates = !BACKWARD || (MODE != kComposites && FORM != kGateConstant);  // x and the states are looked at
+  float x[K][V], f[K][V], inject[K][V], up[BACKWARD ? K : 1][V], front[V], edge[V];
+  uint32_t cut[V];  // bit k: a reset at step k of the chunk
+  auto there = [&](int k) { return FULL || k < n; };
+  // every load of the chunk first, then the arithmetic: K independent rows in flight
+  {
+    const E *px = col.at(P.x, s0), *pg = col.at(P.g, s0), *pd = col.at(P.dh, s0);
+#pragma unroll
+    for (int k = 0; k < K; ++k, px += P.x.st, pg += P.g.st, pd += P.dh.st) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[k][j] = f[k][j] = 0.0f;
+      if (there(k)) {
+        if (kStates) col.load(px, x[k]);
+        if (FORM != kGateConstant) col.load(pg, f[k]);
+        if (BACKWARD) col.load(pd, up[k]);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) front[j] = 1.0f, edge[j] = 0.0f, cut[j] = 0;
+  if (BACKWARD && (FULL || n > 0)) {
+    // the gate that carries d into the chunk belongs to the step before it, the state in front of its last step to the step behind it
+    // (the backward pass walks from the end)
+    if (s0 > 0 && FORM != kGateConstant) col.load(col.at(P.g, s0 - 1), front);
+    if (kStates) {
+      if (s0 + n < P.steps) col.load(col.at(P.h, s0 + n), edge);
+      else col.load_batch(P, P.initial, edge);
+    }
+  }
+  if (P.reset.p != nullptr) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (there(k) && col.flag(P.reset, s0 + k, j)) cut[j] |= 1u << k;
+  }
+  if (BACKWARD && (FULL || n > 0) && s0 > 0) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float unused;
+      gate<FORM>(P, front[j], unused);
+      if (P.reset.p != nullptr && col.flag(P.reset, s0 - 1, j)) front[j] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) gate<FORM>(P, f[k][j], inject[k][j]);
+  auto keep = [&](int k, int j) { return cut[j] >> k & 1 ? 0.0f : f[k][j]; };
+  auto factor = [&](int k, int j) { return !BACKWARD ? keep(k, j) : k == 0 ? front[j] : keep(k - 1, j); };  // what multiplies the carried value at step k
+  if (!BACKWARD && FORM == kGateLogit) {  // (from here on only the product is wanted)
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[k][j] *= inject[k][j];
+  }
+  auto term = [&](int k, int j) { return BACKWARD ? up[k][j] : x[k][j]; };
+  float start[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) start[j] = carry[j].b;
+  if (MODE != kAlone) {
+    Composite mine[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float a = 1.0f, b = 0.0f;
+      bool dropped = false;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (there(k)) {
+          const float m = factor(k, j);
+          if (FORM != kGateConstant) a *= m;
+          b = advance<FORM>(P, m, b, term(k, j));
+          dropped = dropped || m == 0.0f;
+        }
+      }
+      if (FORM == kGateConstant) a = P.power[BACKWARD && s0 == 0 && n > 0 ? n - 1 : n];
+      mine[j] = {dropped ? 0.0f : a == 0.0f ? 1.4e-45f : a, b};  // (a product that underflowed does not drop anything)
+    }
+    join_chunks<V>(mine, carry, more, P.lanes_log2, lds);
+#pragma unroll
+    for (int j = 0; j < V; ++j) start[j] = mine[j].b;
+  }
+  if (MODE == kComposites) return;
+  if (!BACKWARD) {
+    E* ph = col.at(P.h, s0);
+#pragma unroll
+    for (int k = 0; k < K; ++k, ph += P.h.st) {
+      if (there(k)) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) start[j] = advance<FORM>(P, keep(k, j), start[j], x[k][j]);
+        col.store(ph, start);
+      }
+    }
+    if (P.final_state != nullptr && n > 0 && s0 + n == P.steps) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) P.final_state[col.batch(P, j)] = start[j];
+    }
+  } else {
+    if (kStates) {  // the states once more, in the order of the forward pass: x turns into what dg multiplies
+#pragma unroll
+      for (int k = K - 1; k >= 0; --k) {
+        if (there(k)) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float before = cut[j] >> k & 1 ? 0.0f : edge[j], value = x[k][j];
+            edge[j] = apply_step(keep(k, j), edge[j], inject[k][j] * value);
+            x[k][j] = FORM == kGateLogit ? f[k][j] * inject[k][j] * (before - value) : before;
+          }
+        }
+      }
+    }
+    E *pdx = col.at(P.dx, s0), *pdg = col.at(P.dg, s0);
+#pragma unroll
+    for (int k = 0; k < K; ++k, pdx += P.dx.st, pdg += P.dg.st) {
+      if (there(k)) {
+        float out[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          start[j] = advance<FORM>(P, factor(k, j), start[j], up[k][j]);
+          out[j] = inject[k][j] * start[j];
+        }
+        if (P.dx.p != nullptr) col.store(pdx, out);
+        if (kStates && P.dg.p != nullptr) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) out[j] = x[k][j] * start[j];
+          col.store(pdg, out);
+        }
+      }
+    }
+    if (P.dinitial != nullptr && n > 0 && s0 + n == P.steps) {  // (what multiplies d behind the last step is that step's own gate)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float last = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (k == n - 1) last = keep(k, j);
+        P.dinitial[col.batch(P, j)] = advance<FORM>(P, last, start[j], 0.0f);
+      }
+    }
+  }
+  if (MODE == kAlone) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) carry[j].b = start[j];
+  }
+}
+
+template <typename E, int FORM, int V, int K, bool BACKWARD, int MODE, bool STREAM = false>
+__global__ __launch_bounds__(MODE == kAlone ? 256 : 1024, 4) void recurrence_columns(const RecurrenceParams P) {
   static_assert(K <= kMostSteps, "the powers of a constant gate");
   extern __shared__ float2 lds[];
   const int columns = MODE == kAlone ? blockDim.x : 1 << P.lanes_log2;
@@ -206,13 +350,12 @@ __global__ __launch_bounds__(MODE == kAlone ? 256 : 1024) void recurrence_column
   const int64_t block = blockIdx.x;
   const int64_t segment = MODE == kAlone ? 0 : block / P.column_blocks;
   const int64_t vector = (MODE == kAlone ? block : block % P.column_blocks) * columns + (threadIdx.x & (columns - 1));
-  Column<E, V> col;
-  col.o = vector / P.vectors_per_outer;
-  col.i = (vector % P.vectors_per_outer) * V;
-  col.nv = vector >= P.vectors ? 0 : static_cast<int>(P.inner - col.i < V ? P.inner - col.i : V);
-  if (MODE == kAlone && col.nv == 0) return;
+  const bool active = vector < P.vectors;
+  if (MODE == kAlone && !active) return;
+  Column<E, V, STREAM> col;  // (a lane behind the last column has no steps to walk; it joins in with nothing)
+  col.o = active ? vector / P.vectors_per_outer : 0;
+  col.i = active ? (vector % P.vectors_per_outer) * V : 0;
   const int64_t begin = segment * P.segment, end = begin + P.segment < P.steps ? begin + P.segment : P.steps;
-  constexpr bool kStates = !BACKWARD || (MODE != kComposites && FORM != kGateConstant);  // x and the states are looked at
 
   Composite carry[V];  // a state (0, h), or - composites only - what the walk so far composes to
   {
@@ -226,13 +369,18 @@ __global__ __launch_bounds__(MODE == kAlone ? 256 : 1024) void recurrence_column
     const int64_t run = (segment + chunks - 1) / chunks, from = chunk * run, to = from + run < segment ? from + run : segment;
 #pragma unroll
     for (int j = 0; j < V; ++j) mine[j] = {1.0f, 0.0f};
-    for (int64_t q = from; q < to; ++q) {
+    if (active) {
+      for (int64_t q = from; q < to; q += 8) {  // (eight loads at a time)
+        float2 c[8][V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (j < col.nv) {
-          const float2 c = P.composites[(q * P.vectors + vector) * V + j];
-          mine[j] = then(mine[j], {c.x, c.y});
-        }
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j) c[i][j] = P.composites[((q + i < to ? q + i : q) * P.vectors + vector) * V + j];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (q + i < to) mine[j] = then(mine[j], {c[i][j].x, c[i][j].y});
       }
     }
     join_chunks<V>(mine, carry, true, P.lanes_log2, lds);
@@ -241,145 +389,18 @@ __global__ __launch_bounds__(MODE == kAlone ? 256 : 1024) void recurrence_column
   const int64_t tile = static_cast<int64_t>(chunks) * K;
   for (int64_t base = begin; base < end; base += tile) {
     const int64_t s0 = base + static_cast<int64_t>(chunk) * K;
-    const int n = col.nv == 0 || s0 >= end ? 0 : static_cast<int>(end - s0 < K ? end - s0 : K);
-    float x[K][V], f[K][V], inject[K][V], up[BACKWARD ? K : 1][V], front[V], edge[V];
-    uint32_t cut[V];  // bit k: a reset at step k of the chunk
-    // every load of the chunk first, then the arithmetic: K independent rows in flight
-    {
-      const E *px = col.at(P.x, s0), *pg = col.at(P.g, s0), *pd = col.at(P.dh, s0);
-#pragma unroll
-      for (int k = 0; k < K; ++k, px += P.x.st, pg += P.g.st, pd += P.dh.st) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) x[k][j] = f[k][j] = 0.0f;
-        if (k < n) {
-          if (kStates) col.load(px, x[k]);
-          if (FORM != kGateConstant) col.load(pg, f[k]);
-          if (BACKWARD) col.load(pd, up[k]);
-        }
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j) front[j] = 1.0f, edge[j] = 0.0f, cut[j] = 0;
-    if (BACKWARD && n > 0) {
-      // the gate that carries d into the chunk belongs to the step before it, the state in front of its last step to the step behind it
-      // (the backward pass walks from the end)
-      if (s0 > 0 && FORM != kGateConstant) col.load(col.at(P.g, s0 - 1), front);
-      if (kStates) {
-        if (s0 + n < P.steps) col.load(col.at(P.h, s0 + n), edge);
-        else col.load_batch(P, P.initial, edge);
-      }
-    }
-    if (P.reset.p != nullptr) {
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (k < n && col.flag(P.reset, s0 + k, j)) cut[j] |= 1u << k;
-    }
-    if (BACKWARD && n > 0 && s0 > 0) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float unused;
-        gate<FORM>(P, front[j], unused);
-        if (P.reset.p != nullptr && col.flag(P.reset, s0 - 1, j)) front[j] = 0.0f;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int j = 0; j < V; ++j) gate<FORM>(P, f[k][j], inject[k][j]);
-    auto keep = [&](int k, int j) { return cut[j] >> k & 1 ? 0.0f : f[k][j]; };
-    auto factor = [&](int k, int j) { return !BACKWARD ? keep(k, j) : k == 0 ? front[j] : keep(k - 1, j); };  // what multiplies the carried value at step k
-    auto term = [&](int k, int j) { return BACKWARD ? up[k][j] : FORM == kGateLogit ? inject[k][j] * x[k][j] : x[k][j]; };
-    float start[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) start[j] = carry[j].b;
-    if (MODE != kAlone) {
-      Composite mine[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        mine[j] = {1.0f, 0.0f};
-        if (FORM == kGateConstant) {
-          bool dropped = false;
-#pragma unroll
-          for (int k = 0; k < K; ++k) {
-            if (k < n) mine[j].b = advance<FORM>(P, factor(k, j), mine[j].b, term(k, j));
-            if (k < n && factor(k, j) == 0.0f) dropped = true;
-          }
-          mine[j].a = dropped ? 0.0f : P.power[BACKWARD && s0 == 0 && n > 0 ? n - 1 : n];
-        } else {
-#pragma unroll
-          for (int k = 0; k < K; ++k)
-            if (k < n) mine[j] = then(mine[j], {factor(k, j), term(k, j)});
-        }
-      }
-      join_chunks<V>(mine, carry, MODE == kComposites || base + tile < end, P.lanes_log2, lds);
-#pragma unroll
-      for (int j = 0; j < V; ++j) start[j] = mine[j].b;
-    }
-    if (MODE == kComposites) continue;
-    if (!BACKWARD) {
-      E* ph = col.at(P.h, s0);
-#pragma unroll
-      for (int k = 0; k < K; ++k, ph += P.h.st) {
-        if (k < n) {
-#pragma unroll
-          for (int j = 0; j < V; ++j) start[j] = advance<FORM>(P, keep(k, j), start[j], term(k, j));
-          col.store(ph, start);
-        }
-      }
-      if (P.final_state != nullptr && n > 0 && s0 + n == P.steps) {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (j < col.nv) P.final_state[col.batch(P, j)] = start[j];
-      }
+    const bool more = MODE == kComposites || base + tile < end;
+    // (decided for the whole workgroup, which meets at the join's barriers)
+    if (base + tile <= end && P.whole_blocks) {
+      walk_chunk<E, FORM, V, K, BACKWARD, MODE, true, STREAM>(P, col, s0, K, more, carry, lds);
     } else {
-      if (kStates) {  // the states once more, in the order of the forward pass: x turns into what dg multiplies
-#pragma unroll
-        for (int k = K - 1; k >= 0; --k) {
-          if (k < n) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-              const float before = cut[j] >> k & 1 ? 0.0f : edge[j], value = x[k][j];
-              edge[j] = apply_step(keep(k, j), edge[j], inject[k][j] * value);
-              x[k][j] = FORM == kGateLogit ? f[k][j] * inject[k][j] * (before - value) : before;
-            }
-          }
-        }
-      }
-      E *pdx = col.at(P.dx, s0), *pdg = col.at(P.dg, s0);
-#pragma unroll
-      for (int k = 0; k < K; ++k, pdx += P.dx.st, pdg += P.dg.st) {
-        if (k < n) {
-          float out[V];
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            start[j] = advance<FORM>(P, factor(k, j), start[j], up[k][j]);
-            out[j] = inject[k][j] * start[j];
-          }
-          if (P.dx.p != nullptr) col.store(pdx, out);
-          if (kStates && P.dg.p != nullptr) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) out[j] = x[k][j] * start[j];
-            col.store(pdg, out);
-          }
-          if (s0 + k + 1 == P.steps && P.dinitial != nullptr) {
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-              if (j < col.nv) P.dinitial[col.batch(P, j)] = advance<FORM>(P, keep(k, j), start[j], 0.0f);
-          }
-        }
-      }
-    }
-    if (MODE == kAlone) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) carry[j].b = start[j];
+      const int n = !active || s0 >= end ? 0 : static_cast<int>(end - s0 < K ? end - s0 : K);
+      walk_chunk<E, FORM, V, K, BACKWARD, MODE, false, STREAM>(P, col, s0, n, more, carry, lds);
     }
   }
-  if (MODE == kComposites && chunk == 0) {
+  if (MODE == kComposites && chunk == 0 && active) {
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (j < col.nv) P.composites[(segment * P.vectors + vector) * V + j] = make_float2(carry[j].a, carry[j].b);
+    for (int j = 0; j < V; ++j) P.composites[(segment * P.vectors + vector) * V + j] = make_float2(carry[j].a, carry[j].b);
   }
 }
 

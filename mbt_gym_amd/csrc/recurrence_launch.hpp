@@ -22,7 +22,9 @@ void (*pick_recurrence(int which))(RecurrenceParams) {
     return recurrence_rows<E, FORM, kVector<E>, BACKWARD, false>;
   }
   if constexpr (!BACKWARD) {
-    if (which == kColumnsWide + kAlone) return recurrence_columns<E, FORM, kVector<E>, chunk_steps(FORM, false, kVector<E>, true), false, kAlone>;
+    constexpr int V = kVector<E>, K = chunk_steps(FORM, false, V, true);
+    if (which == kColumnsWide) return recurrence_columns<E, FORM, V, K, false, kAlone>;
+    if (which == kColumnsWide + kStreamed) return recurrence_columns<E, FORM, V, K, false, kAlone, true>;
   }
   if constexpr (sizeof(E) == 2) {
     if (which >= kColumnsPair) return columns_kernel<E, FORM, 2, BACKWARD>(which - kColumnsPair);
