@@ -10,14 +10,25 @@ extern template int launch_policy_loss<float16>(const PolicyLossParams&, int, in
 
 namespace {
 
-// rows that a mask keeps, per workgroup: the gradients of the rows are divided by their number, so it has to be known first (one byte per row)
+// Rows that a mask keeps, per workgroup: the gradients of the rows are divided by their number, so it has to be known first (one byte per row).
+// FLAT: the bytes lie behind one another; sixteen at a time, the bytes that are not zero counted by their carry into the top bit.
+template <bool FLAT>
 __global__ __launch_bounds__(256) void count_rows(Rows mask, int64_t outer, int64_t inner, uint32_t* counts) {
   __shared__ uint32_t lds[4];
   uint32_t n = 0;
   const uint8_t* p = static_cast<const uint8_t*>(mask.p);
-  const int64_t total = outer * inner;
-  for (int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; at < total; at += static_cast<int64_t>(gridDim.x) * 256)
-    n += p[at / inner * mask.so + at % inner * mask.si] != 0;
+  const int64_t total = outer * inner, each = FLAT ? 16 : 1;
+  for (int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * each; at < total; at += static_cast<int64_t>(gridDim.x) * 256 * each) {
+    if (FLAT && at + 16 <= total) {
+      const Pack<uint8_t, 16> bytes = load_pack<uint8_t, 16>(p + at);
+      uint32_t words[4];
+      __builtin_memcpy(words, &bytes, 16);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) n += __popc(((((words[w] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | words[w]) & 0x80808080u));
+    } else {
+      for (int64_t b = at; b < at + each && b < total; ++b) n += p[FLAT ? b : b / inner * mask.so + b % inner * mask.si] != 0;
+    }
+  }
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) n += __shfl_xor(n, d);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = n;
@@ -25,36 +36,46 @@ __global__ __launch_bounds__(256) void count_rows(Rows mask, int64_t outer, int6
   if (threadIdx.x == 0) counts[blockIdx.x] = lds[0] + lds[1] + lds[2] + lds[3];
 }
 
-// the workgroups' partials, in their order: loss, rows, and the std gradient's sums
-__global__ __launch_bounds__(256) void finish_loss(const double* partials, int blocks, int actions, int columns, const uint32_t* counts, double rows, double* sums,
-                                                   float* loss, float* grad_std) {
-  __shared__ double lds[4];
-  if (counts != nullptr) {
-    double c = threadIdx.x < kCountBlocks ? static_cast<double>(counts[threadIdx.x]) : 0.0;
-    c = wave_sum(c);
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = c;
-    __syncthreads();
-    rows = lds[0] + lds[1] + lds[2] + lds[3];
-    __syncthreads();
+// The workgroups' partials, added in an order that does not depend on when they came: loss, rows, and the std gradient's sums.
+constexpr int kFinishThreads = 1024, kFinishWaves = kFinishThreads / 64;
+__global__ __launch_bounds__(kFinishThreads) void finish_loss(const double* partials, int blocks, int actions, int columns, const uint32_t* counts, double rows,
+                                                              double* sums, float* loss, float* grad_std) {
+  __shared__ double lds[kFinishWaves][2 + kMostActions];
+  static_assert(kCountBlocks <= kFinishThreads, "one partial count per thread");
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  double sum[2 + kMostActions];  // loss, components, rows
+#pragma unroll
+  for (int c = 0; c < 2 + kMostActions; ++c) sum[c] = 0.0;
+  for (int b = threadIdx.x; b < blocks; b += kFinishThreads) {
+#pragma unroll
+    for (int c = 0; c < 1 + kMostActions; ++c)
+      if (c < columns) sum[c] += partials[static_cast<int64_t>(b) * (1 + actions) + c];
   }
-  for (int column = 0; column < columns; ++column) {
-    double s = 0.0;
-    for (int b = threadIdx.x; b < blocks; b += 256) s += partials[static_cast<int64_t>(b) * (1 + actions) + column];
-    s = wave_sum(s);
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      s = lds[0] + lds[1] + lds[2] + lds[3];
-      if (column == 0) {
-        sums[0] = s;
-        sums[1] = rows;
-        *loss = rows > 0.0 ? static_cast<float>(-s / (rows * actions)) : 0.0f;
-      } else {
-        sums[1 + column] = s;
-        if (grad_std != nullptr) grad_std[column - 1] = rows > 0.0 ? static_cast<float>(-s / (rows * actions)) : 0.0f;
-      }
+  if (counts != nullptr && threadIdx.x < kCountBlocks) sum[1 + kMostActions] = static_cast<double>(counts[threadIdx.x]);
+#pragma unroll
+  for (int c = 0; c < 2 + kMostActions; ++c) {
+    if (c < columns || c == 1 + kMostActions) {
+      sum[c] = wave_sum(sum[c]);
+      if (lane == 0) lds[wave][c] = sum[c];
     }
-    __syncthreads();
+  }
+  __syncthreads();
+  if (threadIdx.x >= static_cast<unsigned>(columns)) return;
+  double kept = rows, s = 0.0;
+  if (counts != nullptr) {
+    kept = 0.0;
+    for (int w = 0; w < kFinishWaves; ++w) kept += lds[w][1 + kMostActions];
+  }
+  const int column = threadIdx.x;
+  for (int w = 0; w < kFinishWaves; ++w) s += lds[w][column];
+  const float mean = kept > 0.0 ? static_cast<float>(-s / (kept * actions)) : 0.0f;
+  if (column == 0) {
+    sums[0] = s;
+    sums[1] = kept;
+    *loss = mean;
+  } else {
+    sums[1 + column] = s;
+    if (grad_std != nullptr) grad_std[column - 1] = mean;
   }
 }
 
@@ -140,14 +161,16 @@ int mbt_policy_loss_forward(int device, const mbt_policy_loss* p, void* stream) 
   if (P.mask.p != nullptr) {
     uint32_t* counts = reinterpret_cast<uint32_t*>(P.partials + static_cast<int64_t>(plan.blocks) * (1 + p->actions));
     P.counts = counts;
-    count_rows<<<kCountBlocks, 256, 0, s>>>(P.mask, P.outer, P.inner, counts);
+    const bool flat = (P.inner == 1 || P.mask.si == 1) && (P.outer == 1 || P.mask.so == P.inner);
+    if (flat) count_rows<true><<<kCountBlocks, 256, 0, s>>>(P.mask, P.outer, P.inner, counts);
+    else count_rows<false><<<kCountBlocks, 256, 0, s>>>(P.mask, P.outer, P.inner, counts);
     rc = launch_status("policy loss (rows)");
     if (rc != MBT_OK) return rc;
   }
   rc = launch(p, plan, s);
   if (rc != MBT_OK) return rc;
   const bool components = p->std_kind == MBT_STD_COMPONENT;
-  finish_loss<<<1, 256, 0, s>>>(P.partials, static_cast<int>(plan.blocks), p->actions, components ? 1 + p->actions : 1, P.counts,
+  finish_loss<<<1, kFinishThreads, 0, s>>>(P.partials, static_cast<int>(plan.blocks), p->actions, components ? 1 + p->actions : 1, P.counts,
                                 static_cast<double>(P.outer) * static_cast<double>(P.inner), p->sums, p->loss,
                                 components ? static_cast<float*>(P.grad_std.p) : nullptr);
   return launch_status("policy loss (sum)");

@@ -65,33 +65,47 @@ __device__ __forceinline__ void store_pack(E* p, const Pack<E, V>& v) {
   __builtin_memcpy(p, &v, sizeof v);
 }
 
-template <int ALIGNED>
+// The same past the caches, for arrays that are larger than they and read or written once: what they would drive out is worth more.  Accesses of a
+// size that is no power of two are ordinary ones.
+template <int BYTES, int ALIGNED>
 struct Words;
-template <>
-struct Words<4> {
-  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4)));
+template <int ALIGNED>
+struct Words<4, ALIGNED> {
+  typedef uint32_t type;
 };
-template <>
-struct Words<2> {
-  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2)));
-};
-// The same past the caches, for arrays that are larger than they and read or written once: what they would drive out is worth more.
+#define LEARNING_WORDS(BYTES, ALIGNED)                                                          \
+  template <>                                                                                   \
+  struct Words<BYTES, ALIGNED> {                                                                \
+    typedef uint32_t type __attribute__((ext_vector_type(BYTES / 4), aligned(ALIGNED)));        \
+  };
+LEARNING_WORDS(8, 4)
+LEARNING_WORDS(8, 2)
+LEARNING_WORDS(16, 4)
+LEARNING_WORDS(16, 2)
 template <typename E, int V>
 __device__ __forceinline__ Pack<E, V> stream_load_pack(const E* p) {
-  static_assert(sizeof(E) * V == 16, "one 16-byte access");
-  typedef typename Words<alignof(E)>::type words;
-  const words w = __builtin_nontemporal_load(reinterpret_cast<const words*>(p));
+  constexpr int kBytes = sizeof(E) * V;
   Pack<E, V> v;
-  __builtin_memcpy(&v, &w, 16);
+  if constexpr ((kBytes == 4 && alignof(E) == 4) || kBytes == 8 || kBytes == 16) {
+    typedef typename Words<kBytes, alignof(E)>::type words;
+    const words w = __builtin_nontemporal_load(reinterpret_cast<const words*>(p));
+    __builtin_memcpy(&v, &w, kBytes);
+  } else {
+    v = load_pack<E, V>(p);
+  }
   return v;
 }
 template <typename E, int V>
 __device__ __forceinline__ void stream_store_pack(E* p, const Pack<E, V>& v) {
-  static_assert(sizeof(E) * V == 16, "one 16-byte access");
-  typedef typename Words<alignof(E)>::type words;
-  words w;
-  __builtin_memcpy(&w, &v, 16);
-  __builtin_nontemporal_store(w, reinterpret_cast<words*>(p));
+  constexpr int kBytes = sizeof(E) * V;
+  if constexpr ((kBytes == 4 && alignof(E) == 4) || kBytes == 8 || kBytes == 16) {
+    typedef typename Words<kBytes, alignof(E)>::type words;
+    words w;
+    __builtin_memcpy(&w, &v, kBytes);
+    __builtin_nontemporal_store(w, reinterpret_cast<words*>(p));
+  } else {
+    store_pack<E, V>(p, v);
+  }
 }
 
 inline size_t dtype_size(int dtype) { return dtype == MBT_FLOAT32 ? 4 : 2; }

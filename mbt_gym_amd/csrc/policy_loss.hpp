@@ -47,7 +47,18 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
-template <typename E, int A, int KIND>
+template <typename E, int A, bool STREAM>
+__device__ __forceinline__ Pack<E, A> read_row(const E* p) {
+  if constexpr (STREAM) return stream_load_pack<E, A>(p);
+  else return load_pack<E, A>(p);
+}
+template <typename E, int A, bool STREAM>
+__device__ __forceinline__ void write_row(E* p, const Pack<E, A>& v) {
+  if constexpr (STREAM) stream_store_pack<E, A>(p, v);
+  else store_pack<E, A>(p, v);
+}
+
+template <typename E, int A, int KIND, bool STREAM>
 __global__ __launch_bounds__(kLossThreads) void policy_loss_kernel(const PolicyLossParams P) {
   __shared__ double lds[kLossThreads / 64][1 + kMostActions];
   __shared__ double kept;
@@ -99,10 +110,10 @@ __global__ __launch_bounds__(kLossThreads) void policy_loss_kernel(const PolicyL
       keep[r] = in[r];
       w[r] = 0.0f;
       if (in[r]) {
-        mean[r] = load_pack<E, A>(static_cast<const E*>(P.mean.p) + o * P.mean.so + i * P.mean.si);
-        action[r] = load_pack<float, A>(static_cast<const float*>(P.action.p) + o * P.action.so + i * P.action.si);
+        mean[r] = read_row<E, A, STREAM>(static_cast<const E*>(P.mean.p) + o * P.mean.so + i * P.mean.si);
+        action[r] = read_row<float, A, STREAM>(static_cast<const float*>(P.action.p) + o * P.action.so + i * P.action.si);
         w[r] = static_cast<const float*>(P.weight.p)[o * P.weight.so + i * P.weight.si];
-        if (KIND == MBT_STD_FULL) std_row[r] = load_pack<E, A>(static_cast<const E*>(P.std_rows.p) + o * P.std_rows.so + i * P.std_rows.si);
+        if (KIND == MBT_STD_FULL) std_row[r] = read_row<E, A, STREAM>(static_cast<const E*>(P.std_rows.p) + o * P.std_rows.so + i * P.std_rows.si);
         if (P.mask.p != nullptr) keep[r] = static_cast<const uint8_t*>(P.mask.p)[o * P.mask.so + i * P.mask.si] != 0;
       }
     }
@@ -127,8 +138,8 @@ __global__ __launch_bounds__(kLossThreads) void policy_loss_kernel(const PolicyL
         gs.e[j] = static_cast<E>(keep[r] ? -scale * ds : 0.0f);
       }
       if (keep[r]) total += static_cast<double>(value);
-      if (P.grad_mean.p != nullptr) store_pack<E, A>(static_cast<E*>(P.grad_mean.p) + o * P.grad_mean.so + i * P.grad_mean.si, gm);
-      if (KIND == MBT_STD_FULL && P.grad_std.p != nullptr) store_pack<E, A>(static_cast<E*>(P.grad_std.p) + o * P.grad_std.so + i * P.grad_std.si, gs);
+      if (P.grad_mean.p != nullptr) write_row<E, A, STREAM>(static_cast<E*>(P.grad_mean.p) + o * P.grad_mean.so + i * P.grad_mean.si, gm);
+      if (KIND == MBT_STD_FULL && P.grad_std.p != nullptr) write_row<E, A, STREAM>(static_cast<E*>(P.grad_std.p) + o * P.grad_std.so + i * P.grad_std.si, gs);
     }
   }
   if (P.partials == nullptr) {
@@ -154,20 +165,24 @@ __global__ __launch_bounds__(kLossThreads) void policy_loss_kernel(const PolicyL
   }
 }
 
-template <typename E, int A>
+template <typename E, int A, bool STREAM>
 void (*pick_policy_loss(int kind))(PolicyLossParams) {
-  if (kind == MBT_STD_NUMBER) return policy_loss_kernel<E, A, MBT_STD_NUMBER>;
-  if (kind == MBT_STD_COMPONENT) return policy_loss_kernel<E, A, MBT_STD_COMPONENT>;
-  return policy_loss_kernel<E, A, MBT_STD_FULL>;
+  if (kind == MBT_STD_NUMBER) return policy_loss_kernel<E, A, MBT_STD_NUMBER, STREAM>;
+  if (kind == MBT_STD_COMPONENT) return policy_loss_kernel<E, A, MBT_STD_COMPONENT, STREAM>;
+  return policy_loss_kernel<E, A, MBT_STD_FULL, STREAM>;
 }
 
 // one translation unit per element type (kernels_policy_loss_*.hip)
 template <typename E>
 int launch_policy_loss(const PolicyLossParams& P, int actions, int kind, unsigned blocks, hipStream_t stream) {
-  void (*const by_actions[kMostActions])(PolicyLossParams) = {
-      pick_policy_loss<E, 1>(kind), pick_policy_loss<E, 2>(kind), pick_policy_loss<E, 3>(kind), pick_policy_loss<E, 4>(kind),
-      pick_policy_loss<E, 5>(kind), pick_policy_loss<E, 6>(kind), pick_policy_loss<E, 7>(kind), pick_policy_loss<E, 8>(kind)};
-  by_actions[actions - 1]<<<blocks, kLossThreads, 0, stream>>>(P);
+  // past the caches where the recording is larger than the last of them (2^18 x 200 rows of two float32 components: 268 us, through them 305)
+  const int64_t bytes = P.outer * P.inner * actions * static_cast<int64_t>(2 * sizeof(E) + 4);
+  const bool stream_it = bytes > (int64_t{256} << 20);
+  void (*kernel)(PolicyLossParams) = nullptr;
+#define LEARNING_PICK(A) if (actions == A) kernel = stream_it ? pick_policy_loss<E, A, true>(kind) : pick_policy_loss<E, A, false>(kind);
+  LEARNING_PICK(1) LEARNING_PICK(2) LEARNING_PICK(3) LEARNING_PICK(4) LEARNING_PICK(5) LEARNING_PICK(6) LEARNING_PICK(7) LEARNING_PICK(8)
+#undef LEARNING_PICK
+  kernel<<<blocks, kLossThreads, 0, stream>>>(P);
   return launch_status("policy loss");
 }
 
