@@ -81,7 +81,8 @@ class Muon(torch.optim.Optimizer):
         p <- (1 - lr weight_decay) p - lr sqrt(max(1, rows / columns)) orthogonalise(u)
 
     A parameter with more than two axes is the matrix (first axis, the rest); a vector - a bias - is a matrix of one column, whose orthogonal factor
-    is the vector at length one.  All parameters of a dtype are orthogonalised in one call."""
+    is the vector at length one.  Momentum and update are float32 whatever the parameters are; all parameters of a dtype and device are
+    orthogonalised in one call."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5,
                  coefficients: Sequence[float] = COEFFICIENTS, eps: float = 1e-7):
@@ -110,8 +111,8 @@ class Muon(torch.optim.Optimizer):
             if p.grad.is_sparse:
                 raise ValueError("Muon does not take sparse gradients")
             if "momentum" not in self.state[p]:
-                self.state[p]["momentum"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
-        grads, moving = [p.grad for p in params], [self.state[p]["momentum"] for p in params]
+                self.state[p]["momentum"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
+        grads, moving = [p.grad.float() for p in params], [self.state[p]["momentum"] for p in params]
         torch._foreach_mul_(moving, group["momentum"])
         torch._foreach_add_(moving, grads)
         updates = torch._foreach_add(grads, moving, alpha=group["momentum"]) if group["nesterov"] else moving
@@ -120,4 +121,4 @@ class Muon(torch.optim.Optimizer):
         if group["weight_decay"]:
             torch._foreach_mul_(params, 1.0 - group["lr"] * group["weight_decay"])
         torch._foreach_mul_(turned, [-group["lr"] * math.sqrt(max(1.0, t.shape[0] / t.shape[1])) for t in turned])
-        torch._foreach_add_(params, [t.reshape(p.shape) for t, p in zip(turned, params)])
+        torch._foreach_add_(params, [t.reshape(p.shape).to(p.dtype) for t, p in zip(turned, params)])

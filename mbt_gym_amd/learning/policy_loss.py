@@ -179,4 +179,6 @@ def policy_gradient_loss(mean: torch.Tensor, actions: torch.Tensor, weights: tor
     if mean.numel() == 0:
         zero = mean.sum(dtype=torch.float32) if std is None else mean.sum(dtype=torch.float32) + 0.0 * std.sum(dtype=torch.float32)
         return zero  # (no rows: a loss of zero that is still connected to its leaves)
+    if not torch.is_grad_enabled():  # (nothing will ask for the gradients)
+        mean, std = mean.detach(), None if std is None else std.detach()
     return _PolicyLoss.apply(mean, std, actions, weights, mask, number, entropy_weight)

@@ -131,6 +131,7 @@ class _LinearRecurrence(torch.autograd.Function):
         if reset is not None:
             r.reset.data = reset.data_ptr()
         if initial is not None:
+            initial = initial.contiguous()  # (as it was saved, unless a hook brought it back otherwise)
             r.initial = initial.data_ptr()
         wanted = ctx.needs_input_grad
         grad_inputs = grad_gate = grad_initial = None

@@ -84,6 +84,32 @@ def test_a_large_recording():
     check(*make((100, 1 << 17), 2, "float32", "component", seed=5, padded=True), 0.01, "float32")
 
 
+def test_without_gradients_none_are_computed():
+    mean, actions, weights, std, _ = make((20, 30), 2, "float32", "component", seed=14)
+    expected = loss_of(mean, actions, weights, std)
+    with torch.no_grad():
+        before = torch.cuda.memory_allocated()
+        loss = loss_of(mean, actions, weights, std)
+        assert torch.cuda.memory_allocated() - before < mean.numel() * 4  # (no room for a gradient of mean was taken and kept)
+    assert not loss.requires_grad and torch.equal(loss, expected.detach())
+
+
+def test_rows_beyond_32_bits_of_offset():
+    """2^30 + 777 rows of two bfloat16 components and float32 actions (8.6 GB): the last rows count, and their gradients are where they belong"""
+    rows = (1 << 30) + 777
+    mean = torch.zeros(rows, 2, dtype=torch.bfloat16, device="cuda")
+    actions = torch.zeros(rows, 2, device="cuda")
+    weights = torch.zeros(rows, device="cuda")
+    mean[-3:], actions[-3:], weights[-3:] = 0.25, torch.tensor([0.5, 0.125], device="cuda"), torch.tensor([1e9, -2e9, 3e9], device="cuda")
+    mean.requires_grad_(True)
+    loss = loss_of(mean, actions, weights, 0.5)
+    grad, = torch.autograd.grad(loss, mean)
+    ref = PolicyLoss(to64(mean[-3:]), to64(actions[-3:]), to64(weights[-3:]) * 3 / rows, 0.5, dtype="bfloat16")
+    assert_within(to64(loss), ref.loss, ref.loss_bound, "loss")
+    assert_within(to64(grad[-3:]), ref.grad_mean, ref.grad_mean_bound, "grad")
+    assert int((grad != 0).sum()) == 6
+
+
 def test_masked_rows_count_for_nothing_whatever_they_hold():
     mean, actions, weights, std, _ = make((40, 100), 2, "float32", "full", seed=6)
     keep = torch.rand(40, 100, device="cuda") < 0.5

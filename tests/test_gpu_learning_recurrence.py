@@ -357,3 +357,55 @@ def test_refusals_on_the_device():
         step(torch.randn(3, 5, device="cuda").t(), x, x)
     with pytest.raises(ValueError, match="not differentiable"):
         step(x, x, x.clone().requires_grad_(True))
+
+
+@pytest.mark.parametrize("layout", ["time_first", "time_last"])
+def test_offsets_beyond_32_bits(layout):
+    """more than 2^31 elements (4.7 GB in bfloat16): the last columns and the last rows are where they belong"""
+    steps, lanes = (2200, 1 << 20) if layout == "time_first" else (1 << 15, 70000)
+    shape = (steps, lanes) if layout == "time_first" else (lanes, steps)
+    axis = 0 if layout == "time_first" else 1
+    x = torch.zeros(shape, dtype=torch.bfloat16, device="cuda")
+    pick = torch.tensor([0, 1, lanes // 2, lanes - 2, lanes - 1], device="cuda")
+    part = torch.randn(steps, 5, device="cuda").bfloat16()
+    x.index_copy_(1 - axis, pick, part if axis == 0 else part.t())
+    with torch.no_grad():
+        states, final = learning().linear_recurrence(x, 0.75, dim=axis, reverse=True, return_final=True)
+    ref = Recurrence(to64(part), 0.75, "constant", reverse=True, dtype="bfloat16")
+    got = states.index_select(1 - axis, pick)
+    assert_within(to64(got if axis == 0 else got.t()), *ref.states(), layout)
+    assert_within(to64(final[pick]), ref.final, ref.final_bound, layout)
+    assert int((states != 0).sum()) == int((got != 0).sum())  # and nothing landed anywhere else
+    del states, got
+    gate = torch.full((1, 1), 0.5, dtype=torch.bfloat16, device="cuda").expand(shape)
+    with torch.no_grad():
+        states = learning().linear_recurrence(x, gate, dim=axis)
+    ref = Recurrence(to64(part), np.full((steps, 5), 0.5), "value", dtype="bfloat16")
+    got = states.index_select(1 - axis, pick)
+    assert_within(to64(got if axis == 0 else got.t()), *ref.states(), layout)
+
+
+def test_saved_tensors_that_come_back_from_elsewhere():
+    """a hook that keeps what autograd saves on the host, and one that brings it back in another layout"""
+    x, gate, h0, cut = make((30, 12, 5), "logit", "float32", 21, reset=True)
+    leaves = [t.requires_grad_(True) for t in (x, gate, h0)]
+    up = torch.randn(30, 12, 5, device="cuda")
+    plain = torch.autograd.grad(learning().linear_recurrence(x, gate, h0, reset=cut, gate_is_logit=True), leaves, up)
+    for pack, unpack in ((lambda t: t.cpu(), lambda t: t.cuda()),
+                         (lambda t: t.clone(), lambda t: t.transpose(0, -1).contiguous().transpose(0, -1))):
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            states = learning().linear_recurrence(x, gate, h0, reset=cut, gate_is_logit=True)
+        ref = Recurrence(to64(x), to64(gate), "logit", to64(h0), cut.cpu().numpy())
+        for name, got, same in zip(("inputs", "gate", "initial"), torch.autograd.grad(states, leaves, up), plain):
+            assert_within(to64(got), *ref.gradients(to64(up))[name], name)
+            assert got.shape == same.shape
+
+
+def test_a_leaf_that_changed_is_noticed():
+    x, gate, h0, _ = make((9, 4), "value", "float32", 22)
+    x, gate = x.requires_grad_(True), gate.requires_grad_(True)
+    states = learning().linear_recurrence(x, gate, h0)
+    with torch.no_grad():
+        gate.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        states.sum().backward()
