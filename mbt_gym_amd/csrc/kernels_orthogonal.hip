@@ -53,7 +53,7 @@ MatrixGroup group_of(const mbt_matrix& m, int tile) {
 
 int check_matrices(uint32_t count, const mbt_matrix* matrices) {
   if (count < 1 || matrices == nullptr) return mbt_set_error(MBT_ERR_INVALID, "no matrices");
-  uint64_t total = 0;
+  uint64_t total = 0, blocks = 0;
   for (uint32_t k = 0; k < count; ++k) {
     const mbt_matrix& m = matrices[k];
     if (m.in == nullptr || m.out == nullptr) return mbt_set_error(MBT_ERR_INVALID, "matrix %u: null argument", k);
@@ -63,6 +63,10 @@ int check_matrices(uint32_t count, const mbt_matrix* matrices) {
     const MatrixGroup g = group_of(m, 128);
     total += m.batch * (static_cast<uint64_t>(g.mp) * g.np / 4096 + 1);
     if (total > (uint64_t{1} << 28)) return mbt_set_error(MBT_ERR_INVALID, "more elements than one call takes (2^40)");
+    // a launch counts its threads in 32 bits: in workgroups of 1024, the norms' for a matrix beyond 64 x 64, or the products' 64 x 64 tiles at 256 each
+    const uint64_t tiles = static_cast<uint64_t>(g.mp) * g.np / 4096 / 4;
+    blocks += m.batch * (kind_of(m) == kSmallMatrix ? 1 : tiles > kNormBlocks ? tiles : kNormBlocks);
+    if (blocks >= (uint64_t{1} << 22)) return mbt_set_error(MBT_ERR_INVALID, "more matrices than one launch takes");
   }
   return MBT_OK;
 }
@@ -142,7 +146,6 @@ int run_small(uint32_t count, const mbt_matrix* matrices, OrthogonaliseParams& P
       blocks += g.batch;
     }
     if (P.groups == kMostGroups || (k == count && P.groups > 0)) {
-      if (blocks > 0x7fffff00) return mbt_set_error(MBT_ERR_INVALID, "more matrices than one launch takes");
       orthogonalise_small<E><<<static_cast<unsigned>(blocks), 1024, kSmallLds, stream>>>(P);
       const int rc = launch_status("orthogonalise");
       if (rc != MBT_OK) return rc;
@@ -183,7 +186,6 @@ int run_kind(Kind kind, uint32_t count, const mbt_matrix* matrices, int tile, Or
       shares += g.batch * g.shares;
     }
     if (P.groups == 0) break;
-    if (split_tiles > 0x7fffff00 || shares > 0x7fffff00 || matrices_in > 0x7fffff00 / kNormBlocks) return mbt_set_error(MBT_ERR_INVALID, "more matrices than one launch takes");
     P.partials = reinterpret_cast<double*>(next);
     next += matrices_in * kNormBlocks * sizeof(double);
     P.planes = reinterpret_cast<_Float16*>(next);

@@ -107,12 +107,14 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
   const int64_t batch = P.outer * P.inner;
   const int64_t chip = 256 * 1024;  // threads that fill it at 16 waves per compute unit
 
-  if (time_contiguous && steps > 1 && !(inner_contiguous && P.inner >= 64)) {
-    // rows: as many lanes as the steps of a row need; a long row is cut into segments, one wave each, while the chip has room for them
+  if (time_contiguous && steps > 1) {
+    // rows: as many lanes as the steps of a row need; a long row is cut into segments, one wave each, while the chip has room for them (8 rows of
+    // 65536 steps, float32: 16.4 us, 328 in one piece; 64 x 4096 16.2 us, 24.6 in one piece).  From twelve tiles on: with eight the launch
+    // that the segments' composites take costs more than it gains (256 x 2048 float32: 16.4 us, 14.4 in one piece; 64 x 4096 bfloat16 18.5 and 16.9)
     const int lanes = log2_ceil(ceil_div(steps, vector));
     P.lanes_log2 = lanes < 6 ? lanes : 6;
     const int64_t tile = (int64_t{1} << P.lanes_log2) * vector;
-    if (P.lanes_log2 == 6 && steps >= 8 * tile) {
+    if (P.lanes_log2 == 6 && steps >= 12 * tile) {
       int64_t want = chip / 64 / 2 / batch;                  // (8 waves per compute unit)
       const int64_t most = steps / (4 * tile);              // a segment shorter than four tiles costs more in composites than it gains
       want = want < most ? want : most;
@@ -129,9 +131,11 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
   }
 
   // Columns per thread: one float32 or two 16-bit elements, so that a wave's row is 256 bytes and the time axis can be cut finely; a recording with
-  // columns enough for every wave of the chip to have 64 x 16 bytes of its own is walked forwards in such vectors, alone.
+  // columns enough for every wave of the chip to have 64 x 16 bytes of its own is walked forwards in such vectors, alone (value gates, 50 steps x 2^20
+  // float32 120 us, 135 by single columns; x 2^21 bfloat16 115 us, 133 by pairs; rewards-to-go 84 and 91, 80 and 91).  Not gated float32 rows of
+  // 8 MB and more: 100 x 2^21 535 us, 501 by single columns; 50 x 2^22 600 and 501.
   const int pair = inner_contiguous && size == 2 && P.inner % 2 == 0 ? 2 : 1;
-  const bool wide = !backward && inner_contiguous && P.inner % vector == 0 && P.outer * (P.inner / vector) >= chip;
+  const bool wide = !backward && !(gated && size == 4 && P.inner >= (1 << 21)) && inner_contiguous && P.inner % vector == 0 && P.outer * (P.inner / vector) >= chip;
   const int v = wide ? vector : pair;
   const int base = wide ? kColumnsWide : pair == 2 ? kColumnsPair : kColumnsScalar;
   P.vectors_per_outer = ceil_div(P.inner, v);
@@ -139,7 +143,9 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
   const int chunk = chunk_steps(r->form, backward, v, false);
   int64_t parallel = ceil_div(chip, P.vectors);
   if (parallel > ceil_div(steps, chunk)) parallel = ceil_div(steps, chunk);
-  if (wide || parallel <= 2) {
+  // With two thirds of the chip's threads or more a thread walks its columns alone, without joins (200 x 3 * 2^16 bfloat16: 40 us forward and 98
+  // backward, 51 and 116 joined; 50 x 3 * 2^16 15 and 18, 21 and 35); with a half it would not (200 x 2^16 float32: 29.4 and 56, joined 28.3 and 51).
+  if (wide || parallel <= 3) {
     plan.which = base + kAlone;
     if (wide && batch * steps * static_cast<int64_t>(size) * count > (int64_t{256} << 20)) plan.which = base + kStreamed;  // (beyond the last cache)
     plan.threads = 256;
@@ -187,7 +193,8 @@ int run(int device, const mbt_recurrence* r, bool backward, void* stream) {
   Plan plan;
   int rc = make_plan(r, backward, plan);
   if (rc != MBT_OK) return rc;
-  if (plan.blocks > 0x7fffffff) return mbt_set_error(MBT_ERR_INVALID, "%llu x %llu sequences are more than one launch can walk", (unsigned long long)r->outer, (unsigned long long)r->inner);
+  if (plan.blocks > 0xffffffffll / plan.threads) return  // (a launch counts its threads in 32 bits)
+      mbt_set_error(MBT_ERR_INVALID, "%llu x %llu sequences are more than one launch can walk", (unsigned long long)r->outer, (unsigned long long)r->inner);
   if (plan.workspace > 0 && (r->workspace == nullptr || r->workspace_bytes < plan.workspace))
     return mbt_set_error(MBT_ERR_INVALID, "the workspace has %llu bytes; %llu are needed (mbt_recurrence_workspace)",
                          (unsigned long long)(r->workspace == nullptr ? 0 : r->workspace_bytes), (unsigned long long)plan.workspace);
@@ -230,7 +237,7 @@ int mbt_recurrence_step(int device, int dtype, int form, uint64_t rows, uint64_t
   if (!dtype_known(dtype)) return mbt_set_error(MBT_ERR_INVALID, "dtype %d: float32, bfloat16 and float16 are known", dtype);
   if (form != kGateValue && form != kGateLogit) return mbt_set_error(MBT_ERR_INVALID, "a single step takes MBT_GATE_VALUE or MBT_GATE_LOGIT");
   if (state == nullptr || inputs == nullptr || gate == nullptr || out == nullptr || new_state == nullptr) return mbt_set_error(MBT_ERR_INVALID, "null argument");
-  if (rows < 1 || columns < 1 || rows > (uint64_t{1} << 38) / columns) return mbt_set_error(MBT_ERR_INVALID, "rows x columns has to be within 1 .. 2^38");
+  if (rows < 1 || columns < 1 || rows > (uint64_t{1} << 33) / columns) return mbt_set_error(MBT_ERR_INVALID, "rows x columns has to be within 1 .. 2^33");
   DeviceScope scope;
   int rc = scope.enter(device);
   if (rc != MBT_OK) return rc;

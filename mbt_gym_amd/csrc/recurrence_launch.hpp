@@ -45,8 +45,9 @@ int launch_recurrence(const RecurrenceParams& P, int form, bool backward, int wh
 template <typename E>
 int launch_recurrence_step(const float* state, const void* x, const void* g, const uint8_t* reset, int64_t reset_columns, int64_t rs, int64_t rc, void* out,
                            float* new_state, int64_t n, int form, hipStream_t stream) {
-  // two steps' worth of elements per thread only where the chip is full anyway: below that, more and smaller waves finish sooner
-  const bool wide = n >= (1 << 20);
+  // 16 bytes per thread only where the chip is full anyway (2^22 bfloat16: 9.3 us, 11.6 with one element each); below that more and smaller waves
+  // finish sooner (2^16: 2.3 us, 2.8 wide; 2^21: 5.4 and 5.8)
+  const bool wide = n >= (1 << 22);
   const int v = wide ? kVector<E> : 1;
   const unsigned blocks = static_cast<unsigned>((n + 256 * static_cast<int64_t>(v) - 1) / (256 * static_cast<int64_t>(v)));
   const E *xe = static_cast<const E*>(x), *ge = static_cast<const E*>(g);

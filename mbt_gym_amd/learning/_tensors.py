@@ -14,6 +14,8 @@ def require(tensor, name, device=None, dtypes=None, shape=None):
         raise ValueError(f"{name} lives on {tensor.device}: the operators run on the GPU and have no CPU path")
     if tensor.layout is not torch.strided:
         raise TypeError(f"{name} has the layout {tensor.layout}: strided tensors only")
+    if tensor.is_neg():
+        raise ValueError(f"{name} is a view that negates what lies in memory: resolve_neg() first")
     if device is not None and tensor.device != device:
         raise ValueError(f"{name} lives on {tensor.device}, the other tensors on {device}")
     if dtypes is not None and tensor.dtype not in dtypes:

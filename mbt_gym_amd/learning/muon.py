@@ -106,6 +106,13 @@ class Muon(torch.optim.Optimizer):
                 self._step(params, group)
         return loss
 
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)  # (which rounds a state to the type of its parameter)
+        keys = [key for group in state_dict["param_groups"] for key in group["params"]]
+        for key, p in zip(keys, (p for group in self.param_groups for p in group["params"])):
+            if "momentum" in state_dict["state"].get(key, ()):
+                self.state[p]["momentum"] = state_dict["state"][key]["momentum"].to(device=p.device, dtype=torch.float32, copy=True)
+
     def _step(self, params, group):
         for p in params:
             if p.grad.is_sparse:

@@ -215,7 +215,8 @@ def linear_recurrence_step(state: torch.Tensor, inputs: torch.Tensor, gate: torc
     require(gate, "gate", inputs.device, (inputs.dtype,), inputs.shape)
     if torch.is_grad_enabled() and (state.requires_grad or inputs.requires_grad or gate.requires_grad):
         raise ValueError("linear_recurrence_step is not differentiable: use torch.no_grad(), or linear_recurrence on the sequence")
-    if new_state is None:
+    given = new_state is not None
+    if not given:
         new_state = torch.empty(inputs.shape, dtype=torch.float32, device=inputs.device)
     elif new_state is not state:
         require(new_state, "new_state", inputs.device, (torch.float32,), inputs.shape)
@@ -232,6 +233,15 @@ def linear_recurrence_step(state: torch.Tensor, inputs: torch.Tensor, gate: torc
         folded = reset.reshape(rows, columns)
         flags, row_stride, column_stride = folded.data_ptr(), folded.stride(0), folded.stride(1)
     inputs, gate = inputs.contiguous(), gate.contiguous()
+    if given:
+        start, size = new_state.data_ptr(), 4 * inputs.numel()
+        for name, t in (("state", state), ("inputs", inputs), ("gate", gate)):
+            # (each element is read before its own place is written, by the thread that writes it: the very same place is all right, another is not)
+            at = t.data_ptr()
+            if at < start + size and start < at + t.element_size() * t.numel() and not (at == start and t.dtype == torch.float32):
+                raise ValueError(f"new_state lies over {name}, but not in its place")
+        if not new_state.is_inference():
+            torch.autograd.graph.increment_version(new_state)  # (so that a backward pass that saved it notices)
     index = inputs.device.index
     _native.check(_native.load_library().mbt_recurrence_step(
         index, DTYPES[inputs.dtype], _native.GATE_LOGIT if gate_is_logit else _native.GATE_VALUE, rows, columns, state.data_ptr(), inputs.data_ptr(),

@@ -208,6 +208,26 @@ def test_muon_keeps_its_momentum_in_float32(dtype):
         assert np.linalg.norm(moved) <= 0.05 * (bound + 485 * 8 * U) + HALF_STEP[dtype] * (0.05 * np.linalg.norm(value) + np.linalg.norm(to64(p)) * 1.01)
 
 
+def test_muon_restores_its_momentum():
+    import copy
+
+    from mbt_gym_amd.learning import Muon
+
+    p = torch.nn.Parameter(torch.randn(12, 7, device="cuda").bfloat16())
+    optimizer = Muon([p])
+    p.grad = torch.randn(12, 7, device="cuda").bfloat16()
+    for _ in range(2):
+        optimizer.step()
+    saved, twin = copy.deepcopy(optimizer.state_dict()), torch.nn.Parameter(p.detach().clone())
+    again = Muon([twin])
+    again.load_state_dict(saved)
+    assert again.state[twin]["momentum"].dtype == torch.float32
+    twin.grad = p.grad.clone()
+    optimizer.step(), again.step()
+    assert torch.equal(p, twin) and torch.equal(optimizer.state[p]["momentum"], again.state[twin]["momentum"])
+    assert not torch.equal(saved["state"][0]["momentum"], again.state[twin]["momentum"])  # (the saved one is not what the optimiser goes on with)
+
+
 def test_muon_skips_what_has_no_gradient_and_keeps_its_state():
     from mbt_gym_amd.learning import Muon
 

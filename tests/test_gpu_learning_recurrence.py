@@ -409,3 +409,37 @@ def test_a_leaf_that_changed_is_noticed():
         gate.mul_(2.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         states.sum().backward()
+
+
+def test_a_step_in_place_is_noticed_and_one_over_its_operands_refused():
+    step = learning().linear_recurrence_step
+    x, gate = torch.randn(4, 6, device="cuda"), torch.rand(4, 6, device="cuda")
+    room = torch.zeros(60, device="cuda")
+    state = room[:24].view(4, 6)
+    leaf = torch.rand(9, 4, 6, device="cuda", requires_grad=True)
+    states = learning().linear_recurrence(leaf, leaf, state)
+    step(state, x, gate, new_state=state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        states.sum().backward()
+    for over in (room[8:32].view(4, 6), room[1:25].view(4, 6)):
+        with pytest.raises(ValueError, match="lies over state"):
+            step(state, x, gate, new_state=over)
+    with pytest.raises(ValueError, match="lies over gate"):
+        step(torch.zeros(4, 6, device="cuda"), x, room[20:44].view(4, 6), new_state=state)
+    half = room[:12].view(torch.bfloat16).view(4, 6)
+    with pytest.raises(ValueError, match="lies over inputs"):
+        step(torch.zeros(4, 6, device="cuda"), half, gate.bfloat16(), new_state=state)
+    expected = (room[24:48].view(4, 6) * gate + x).clone()  # next to each other is no overlap, and the inputs' own place is none either
+    out, same = step(room[24:48].view(4, 6), x, gate, new_state=state)
+    assert torch.allclose(out, expected) and same is state
+    _, same = step(room[24:48].view(4, 6), x, gate, new_state=x)
+    assert torch.allclose(x, expected) and same is x
+    with torch.inference_mode():
+        step(state, x, gate, new_state=torch.zeros(4, 6, device="cuda"))
+
+
+def test_negated_views_are_refused():
+    x = torch.randn(5, 6, dtype=torch.complex64, device="cuda").conj().imag
+    assert x.is_neg()
+    with pytest.raises(ValueError, match="resolve_neg"):
+        learning().linear_recurrence(x, 0.5)

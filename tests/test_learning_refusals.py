@@ -93,6 +93,13 @@ def test_a_long_walk_needs_its_workspace(lib):
     assert lib.mbt_recurrence_workspace(C.byref(recurrence_struct()), 0) == 0
 
 
+def test_more_sequences_than_a_launch_has_threads_are_refused(lib):
+    for sizes in (dict(outer=1 << 40, inner=1), dict(outer=1, inner=1 << 34), dict(outer=1 << 20, inner=(1 << 12) + 1)):
+        r = recurrence_struct(steps=1, **sizes)
+        refused(lib, lib.mbt_recurrence_forward(0, C.byref(r), None), "more than one launch can walk")
+        refused(lib, lib.mbt_recurrence_backward(0, C.byref(r), None), "more than one launch can walk")
+
+
 def test_the_library_refuses_a_malformed_step(lib):
     args = dict(device=0, dtype=0, form=_native.GATE_VALUE, rows=3, columns=4, state=4096, inputs=4096, gate=4096, reset=None, rs=0, cs=0, out=4096, new=4096)
 
@@ -103,8 +110,8 @@ def test_the_library_refuses_a_malformed_step(lib):
     refused(lib, step(form=_native.GATE_CONSTANT), "MBT_GATE_VALUE or MBT_GATE_LOGIT")
     for name in ("state", "inputs", "gate", "out", "new"):
         refused(lib, step(**{name: None}), "null argument")
-    for sizes in ((0, 1), (1, 0), (1 << 20, 1 << 20)):
-        refused(lib, step(rows=sizes[0], columns=sizes[1]), "2^38")
+    for sizes in ((0, 1), (1, 0), (1 << 20, 1 << 20), ((1 << 33) + 1, 1), (1, (1 << 33) + 1)):
+        refused(lib, step(rows=sizes[0], columns=sizes[1]), "2^33")
 
 
 def test_tensors_that_are_not_on_the_device_are_refused():
@@ -213,6 +220,8 @@ def test_the_library_refuses_malformed_matrices(lib):
         refused(lib, call(bad), "1 .. 32768")
     refused(lib, call(matrix(batch=0)), "batch of 0")
     refused(lib, call(matrix(rows=32768, columns=32768, batch=1 << 20)), "more elements")
+    for many in (matrix(rows=3, columns=2, batch=1 << 22), matrix(rows=80, columns=66, batch=1 << 14), matrix(rows=66, columns=5, batch=1 << 14)):
+        refused(lib, call(many), "more matrices than one launch takes")
     for steps in (0, -1, 65):
         refused(lib, call(matrix(), steps=steps), f"{steps} steps")
     for c in ((4.5, 0.0, 0.0), (1.0, 2.0, 0.0), (float("inf"), 0.0, 0.0), (0.0, float("nan"), 0.0)):
