@@ -1959,7 +1959,7 @@ __device__ __forceinline__ void rollout_body(const StepBuffers& B, const StepPar
       // (Advancing the pair TOGETHER on 2-vectors - v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32 for everything after the Bernoulli
       // decisions - was built and measured in round 3: 15 fewer arithmetic instructions per pair and step, 23 more v_mov to put
       // lane values into adjacent registers and SGPR spills from the longer live ranges: 3.48e11 instead of 3.62e11 env-steps/s at
-      // 2^20 lanes.  profiles/r03_experiments.txt.  The compiler already packs the two SIDES of a lane where that is free.)
+      // 2^20 lanes.  profiles/r03_experiments.txt.  The build now leaves packed float32 instructions out altogether.)
       const LaneResult r = V::PRECISE ? lane_step_exact<V>(core[l], lam[l], lo[l], act[l], make_draw<V>(nz[l], P), qi[l], terminal, P, nz[l].z, t_now, t, zu[l])
                                       : lane_step<V>(core[l], lam[l], act[l], make_draw<V>(nz[l], P), qi[l], static_cast<float>(t), terminal, P, nz[l].z, t_now, zu[l], HostStep{}, t, lo[l]);
       core[l] = r.core;

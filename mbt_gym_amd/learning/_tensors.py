@@ -20,7 +20,7 @@ def require(tensor, name, device=None, dtypes=None, shape=None):
         raise ValueError(f"{name} lives on {tensor.device}, the other tensors on {device}")
     if dtypes is not None and tensor.dtype not in dtypes:
         raise TypeError(f"{name} is {tensor.dtype}: one of {', '.join(str(d) for d in dtypes)} is needed")
-    if shape is not None and tuple(tensor.shape) != tuple(shape):
+    if shape is not None and tensor.shape != shape:
         raise ValueError(f"{name} has the shape {tuple(tensor.shape)}, {tuple(shape)} is needed")
     return tensor
 

@@ -177,7 +177,7 @@ def linear_recurrence(inputs: torch.Tensor, gate: Union[float, torch.Tensor], in
     if not -inputs.dim() <= dim < inputs.dim():
         raise IndexError(f"dim {dim} of a tensor with {inputs.dim()} dimensions")
     axis = dim % inputs.dim()
-    batch = [n for d, n in enumerate(inputs.shape) if d != axis]
+    batch = tuple(n for d, n in enumerate(inputs.shape) if d != axis)
     constant = 0.0
     if isinstance(gate, torch.Tensor):
         require(gate, "gate", inputs.device, (inputs.dtype,), inputs.shape)
@@ -211,42 +211,51 @@ def linear_recurrence_step(state: torch.Tensor, inputs: torch.Tensor, gate: torc
     new_state  where the float32 state goes: None = a new tensor; `state` itself updates it in place
     Not differentiable: an actor is trained on whole sequences."""
     require(inputs, "inputs", dtypes=DTYPES)
-    require(state, "state", inputs.device, (torch.float32,), inputs.shape)
-    require(gate, "gate", inputs.device, (inputs.dtype,), inputs.shape)
+    shape, dtype, device = inputs.shape, inputs.dtype, inputs.device
+    require(state, "state", device, (torch.float32,), shape)
+    require(gate, "gate", device, (dtype,), shape)
     if torch.is_grad_enabled() and (state.requires_grad or inputs.requires_grad or gate.requires_grad):
         raise ValueError("linear_recurrence_step is not differentiable: use torch.no_grad(), or linear_recurrence on the sequence")
     given = new_state is not None
     if not given:
-        new_state = torch.empty(inputs.shape, dtype=torch.float32, device=inputs.device)
+        new_state = torch.empty(shape, dtype=torch.float32, device=device)
     elif new_state is not state:
-        require(new_state, "new_state", inputs.device, (torch.float32,), inputs.shape)
+        require(new_state, "new_state", device, (torch.float32,), shape)
     if not (state.is_contiguous() and new_state.is_contiguous()):
         raise ValueError("state and new_state have to be contiguous")
-    out = torch.empty(inputs.shape, dtype=inputs.dtype, device=inputs.device)
-    if inputs.numel() == 0:
+    out, count = torch.empty(shape, dtype=dtype, device=device), inputs.numel()
+    if not count:
         return out, new_state
-    columns = inputs.shape[-1] if inputs.dim() else 1
-    rows = inputs.numel() // columns
-    flags = row_stride = column_stride = 0
+    columns = shape[-1] if shape else 1
+    rows = count // columns
+    flags, row_stride, column_stride = None, 0, 0
     if reset is not None:
-        require(reset, "reset", inputs.device, (torch.bool, torch.uint8), inputs.shape)
+        require(reset, "reset", device, (torch.bool, torch.uint8), shape)
         folded = reset.reshape(rows, columns)
-        flags, row_stride, column_stride = folded.data_ptr(), folded.stride(0), folded.stride(1)
+        flags, (row_stride, column_stride) = folded.data_ptr(), folded.stride()
     inputs, gate = inputs.contiguous(), gate.contiguous()
+    state_at, inputs_at, gate_at, new_at = state.data_ptr(), inputs.data_ptr(), gate.data_ptr(), new_state.data_ptr()
     if given:
-        start, size = new_state.data_ptr(), 4 * inputs.numel()
-        for name, t in (("state", state), ("inputs", inputs), ("gate", gate)):
-            # (each element is read before its own place is written, by the thread that writes it: the very same place is all right, another is not)
-            at = t.data_ptr()
-            if at < start + size and start < at + t.element_size() * t.numel() and not (at == start and t.dtype == torch.float32):
-                raise ValueError(f"new_state lies over {name}, but not in its place")
+        size = 4 * count
+        width = size if dtype is torch.float32 else size // 2
+        if (new_at != state_at and -size < new_at - state_at < size) or -width < new_at - inputs_at < width or -width < new_at - gate_at < width:
+            _refuse_overlap(new_at, size, (("state", state_at, size), ("inputs", inputs_at, width), ("gate", gate_at, width)))
         if not new_state.is_inference():
             torch.autograd.graph.increment_version(new_state)  # (so that a backward pass that saved it notices)
-    index = inputs.device.index
-    _native.check(_native.load_library().mbt_recurrence_step(
-        index, DTYPES[inputs.dtype], _native.GATE_LOGIT if gate_is_logit else _native.GATE_VALUE, rows, columns, state.data_ptr(), inputs.data_ptr(),
-        gate.data_ptr(), flags or None, row_stride, column_stride, out.data_ptr(), new_state.data_ptr(), current_stream(index)))
+    index = device.index
+    code = _native.load_library().mbt_recurrence_step(
+        index, DTYPES[dtype], _native.GATE_LOGIT if gate_is_logit else _native.GATE_VALUE, rows, columns, state_at, inputs_at, gate_at, flags, row_stride,
+        column_stride, out.data_ptr(), new_at, current_stream(index))
+    if code < 0:
+        _native.check(code)
     return out, new_state
+
+
+def _refuse_overlap(new_at, size, operands):
+    """Each element is read before its own place is written, by the thread that writes it: the very same place is all right, another is not."""
+    for name, at, width in operands:
+        if at < new_at + size and new_at < at + width and not (at == new_at and width == size):
+            raise ValueError(f"new_state lies over {name}, but not in its place")
 
 
 def rewards_to_go(rewards: torch.Tensor, discount: float = 1.0, *, dim: int = -1, done: Optional[torch.Tensor] = None) -> torch.Tensor:
