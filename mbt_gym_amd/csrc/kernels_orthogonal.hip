@@ -38,6 +38,8 @@ MatrixGroup group_of(const mbt_matrix& m, int tile) {
   g.n = static_cast<int32_t>(turn ? m.rows : m.columns);
   g.batch = static_cast<int64_t>(m.batch);
   const Kind kind = kind_of(m);
+  const int64_t norm_blocks = (static_cast<int64_t>(g.m) * g.n + 4095) / 4096;
+  g.norm_blocks = static_cast<int32_t>(norm_blocks < kNormBlocks ? norm_blocks : kNormBlocks);
   if (kind == kLargeMatrix) {
     g.mp = static_cast<int32_t>(padded(g.m, tile));
     g.np = static_cast<int32_t>(padded(g.n, tile));
@@ -161,7 +163,7 @@ template <typename E>
 int run_kind(Kind kind, uint32_t count, const mbt_matrix* matrices, int tile, OrthogonaliseParams& P, char*& next, hipStream_t stream) {
   uint32_t k = 0;
   while (k < count) {
-    int64_t matrices_in = 0, split_tiles = 0, gram_tiles = 0, apply_tiles = 0, elements = 0, shares = 0;
+    int64_t matrices_in = 0, norm_blocks = 0, split_tiles = 0, gram_tiles = 0, apply_tiles = 0, elements = 0, shares = 0;
     int64_t norm_first[kMostGroups] = {}, split_first[kMostGroups] = {}, gram_first[kMostGroups] = {}, apply_first[kMostGroups] = {}, share_first[kMostGroups] = {};
     P.groups = 0;
     P.odd = 0;
@@ -174,12 +176,13 @@ int run_kind(Kind kind, uint32_t count, const mbt_matrix* matrices, int tile, Or
       g.planes = elements;
       elements += g.batch * g.stride;
       const int64_t rows = g.mp / tile, columns = g.np / tile;
-      norm_first[at] = matrices_in;
+      norm_first[at] = norm_blocks;
       split_first[at] = split_tiles;
       gram_first[at] = gram_tiles;
       apply_first[at] = apply_tiles;
       share_first[at] = shares;
       matrices_in += g.batch;
+      norm_blocks += g.batch * g.norm_blocks;
       split_tiles += g.batch * (g.mp / 64) * (g.np / 64);
       gram_tiles += g.batch * (rows * (rows + 1) / 2);
       apply_tiles += g.batch * rows * columns;
@@ -194,7 +197,7 @@ int run_kind(Kind kind, uint32_t count, const mbt_matrix* matrices, int tile, Or
       for (int g = 0; g < P.groups; ++g) P.group[g].first = first[g];
     };
     place(norm_first);
-    orthogonalise_norms<E><<<static_cast<unsigned>(matrices_in * kNormBlocks), 1024, 0, stream>>>(P);
+    orthogonalise_norms<E><<<static_cast<unsigned>(norm_blocks), 1024, 0, stream>>>(P);
     int rc;
     if (kind == kFlatMatrix) {
       place(share_first);

@@ -111,9 +111,9 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
     // rows: as many lanes as the steps of a row need; a long row is cut into segments, one wave each, while the chip has room for them (8 rows of
     // 65536 steps, float32: 16.4 us, 328 in one piece; 64 x 4096 16.2 us, 24.6 in one piece).  From twelve tiles on: with eight the launch
     // that the segments' composites take costs more than it gains (256 x 2048 float32: 16.4 us, 14.4 in one piece; 64 x 4096 bfloat16 18.5 and 16.9)
-    const int lanes = log2_ceil(ceil_div(steps, vector));
+    const int lanes = log2_ceil(ceil_div(steps, row_steps(size, backward)));
     P.lanes_log2 = lanes < 6 ? lanes : 6;
-    const int64_t tile = (int64_t{1} << P.lanes_log2) * vector;
+    const int64_t tile = (int64_t{1} << P.lanes_log2) * row_steps(size, backward);
     if (P.lanes_log2 == 6 && steps >= 12 * tile) {
       int64_t want = chip / 64 / 2 / batch;                  // (8 waves per compute unit)
       const int64_t most = steps / (4 * tile);              // a segment shorter than four tiles costs more in composites than it gains

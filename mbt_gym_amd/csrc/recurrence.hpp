@@ -414,6 +414,16 @@ __global__ __launch_bounds__(MODE == kAlone ? 256 : 1024, 4) void recurrence_col
   }
 }
 
+#ifndef ROWF
+#define ROWF 4
+#endif
+#ifndef ROWB
+#define ROWB 4
+#endif
+#ifndef ROWFH
+#define ROWFH 8
+#endif
+constexpr int row_steps(size_t size, bool backward) { return size == 4 ? (backward ? ROWB : ROWF) : backward ? 8 : ROWFH; }
 // ---- rows --------------------------------------------------------------------------------------------------------------------------
 // V steps in walking order from s; memory runs the other way when the walk is reversed.  Steps at or behind `end` come back as zero.
 template <typename E, int V>

@@ -18,8 +18,9 @@ void (*columns_kernel(int mode))(RecurrenceParams) {
 template <typename E, int FORM, bool BACKWARD>
 void (*pick_recurrence(int which))(RecurrenceParams) {
   if (which >= kRows) {
-    if (which - kRows == kComposites) return recurrence_rows<E, FORM, kVector<E>, BACKWARD, true>;
-    return recurrence_rows<E, FORM, kVector<E>, BACKWARD, false>;
+    constexpr int V = row_steps(sizeof(E), BACKWARD);
+    if (which - kRows == kComposites) return recurrence_rows<E, FORM, V, BACKWARD, true>;
+    return recurrence_rows<E, FORM, V, BACKWARD, false>;
   }
   if constexpr (!BACKWARD) {
     constexpr int V = kVector<E>, K = chunk_steps(FORM, false, V, true);
