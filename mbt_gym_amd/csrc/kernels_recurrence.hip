@@ -108,20 +108,19 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
   const int64_t chip = 256 * 1024;  // threads that fill it at 16 waves per compute unit
 
   if (time_contiguous && steps > 1) {
-    // rows: as many lanes as the steps of a row need; a long row is cut into segments, one wave each, while the chip has room for them (8 rows of
-    // 65536 steps, float32: 16.4 us, 328 in one piece; 64 x 4096 16.2 us, 24.6 in one piece).  From twelve tiles on: with eight the launch
-    // that the segments' composites take costs more than it gains (256 x 2048 float32: 16.4 us, 14.4 in one piece; 64 x 4096 bfloat16 18.5 and 16.9)
-    const int lanes = log2_ceil(ceil_div(steps, row_steps(size, backward)));
+    // rows: as many lanes as the steps of a row need; a row longer than 64 lanes' is cut into segments of a tile or more, one wave each, while the chip has
+    // room for them (64 rows x 4096 steps, float32 logit form: forward 10.0 us, backward 11.0; in one piece 17.4 and 30.4).  From four segments on -
+    // backwards three: the launch that their composites take costs 3 us more than it gains with fewer (64 x 1100: forward 10.9 us, 9.4 in one piece;
+    // backward 12.1 and 14.1; 1024 x 4096 in two segments: forward 22.7, 19.9 in one piece)
+    const int lanes = log2_ceil(ceil_div(steps, kRowSteps));
     P.lanes_log2 = lanes < 6 ? lanes : 6;
-    const int64_t tile = (int64_t{1} << P.lanes_log2) * row_steps(size, backward);
-    if (P.lanes_log2 == 6 && steps >= 12 * tile) {
-      int64_t want = chip / 64 / 2 / batch;                  // (8 waves per compute unit)
-      const int64_t most = steps / (4 * tile);              // a segment shorter than four tiles costs more in composites than it gains
-      want = want < most ? want : most;
-      if (want > 1) {
-        P.segment = ceil_div(ceil_div(steps, want), tile) * tile;
-        P.segments = static_cast<int32_t>(ceil_div(steps, P.segment));
-      }
+    const int64_t tile = (int64_t{1} << P.lanes_log2) * kRowSteps;
+    int64_t want = chip / 64 / 2 / batch;  // (8 waves per compute unit)
+    const int64_t most = ceil_div(steps, tile);
+    want = want < most ? want : most;
+    if (want >= (backward ? 3 : 4)) {  // (more than one tile: a group is a wave)
+      P.segment = ceil_div(ceil_div(steps, want), tile) * tile;
+      P.segments = static_cast<int32_t>(ceil_div(steps, P.segment));
     }
     plan.which = kRows + kJoined;
     plan.threads = 256;
@@ -155,10 +154,11 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
   }
   // A workgroup takes 64 column vectors (256 bytes of a row) and up to 1024 threads' worth of chunks of time, a tile.  Where that makes fewer workgroups
   // than compute units, and
-  //   - the walk is at least four tiles long: the axis is cut into segments over workgroups as well (64 columns x 65536 steps, float32 logit
-  //     form: 25 us forward; with 16 columns a workgroup and fewer segments 32)
-  //   - it is shorter: a workgroup takes fewer columns, down to 16, or 8 if only that makes the walk one tile (1000 lanes x 200: 8.1 -> 5.6 us; 1024
-  //     columns x 500, bfloat16: 30 -> 11)
+  //   - the walk is at least four tiles long, and eight columns a workgroup would not make it one tile or leave much to walk (2^21 steps in all): the
+  //     axis is cut into segments over workgroups as well (64 columns x 65536 steps, float32 logit form: 25 us forward; with 16 columns a
+  //     workgroup and fewer segments 32.  2000 columns x 2000 float32: backward 31 us, 40 in narrow workgroups)
+  //   - otherwise: a workgroup takes fewer columns, down to 16, or 8 if only that makes the walk one tile (1000 lanes x 200: 8.1 -> 5.6 us; 512
+  //     columns x 1000 bfloat16: forward 11 us, backward 17; in segments 21 and 26.  4000 columns 20 and 27, 26 and 35)
   int columns_log2 = 6;
   while (columns_log2 > 0 && (int64_t{1} << (columns_log2 - 1)) >= P.vectors) --columns_log2;
   const int chunks_wanted = log2_ceil(parallel);
@@ -168,7 +168,8 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
   };
   auto tile_with = [&](int columns) { return (int64_t{1} << chunks_with(columns)) * chunk; };
   auto blocks_with = [&](int columns) { return ceil_div(P.vectors, int64_t{1} << columns); };
-  if (blocks_with(columns_log2) < 128 && steps >= 4 * tile_with(columns_log2)) {
+  const bool narrow = steps <= tile_with(3) && steps * P.vectors <= (int64_t{1} << 21);
+  if (blocks_with(columns_log2) < 128 && steps >= 4 * tile_with(columns_log2) && !narrow) {
     const int64_t tile = tile_with(columns_log2), most = ceil_div(steps, tile);
     int64_t want = 256 / blocks_with(columns_log2);
     want = want < most ? want : most;

@@ -19,7 +19,7 @@
 //            columns each.  A thread walks K steps at a time, all their loads in flight; it is alone with its columns, or the time axis is cut into
 //            chunks over the threads of a workgroup (LDS joins them) and, where even that leaves the chip empty, into segments over workgroups
 //            (a first launch writes their composites).  Very many columns are walked forwards four or eight (16 bytes) to a thread.
-//   rows     time is contiguous: lanes lie along time, 16 bytes of steps each, and a group of 2^n lanes scans by wave shuffles; segments as above
+//   rows     time is contiguous: lanes lie along time, eight steps each, and a group of 2^n lanes scans by wave shuffles; segments as above
 //
 // Measured, against 5.15 TB/s of a copy of 839 MB and 8.6 of one that stays in the last cache (128 MB):
 //   columns, 200 steps x 65536, logit form      float32   forward 29.5 us (5.3 TB/s)   backward 57 us (4.6 TB/s)
@@ -27,8 +27,10 @@
 //   columns, 200 x 2^20, constant gate          float32   333 us (5.0 TB/s): a copy's rate
 //   columns, 65536 x 64, logit form             float32   forward 25 us, backward 37 us, two launches each: 2.0 and 2.3 TB/s, bound by latency - the
 //                                               segments' composites are a second walk over x and g that has to end first
-//   rows, 65536 x 200 steps, logit form         float32   forward 45 us (3.5 TB/s), backward 102 us (2.6 TB/s): bound by the shuffles of the scans and the
-//                                               registers, 4 waves per SIMD.  (The scan by DPP moves instead of shuffles: 66 us forward, it spills.)
+//   rows, 65536 x 200 steps, logit form         float32   forward 36.6 us (4.3 TB/s), backward 84 us (3.1 TB/s): bound by the instructions of the scans and
+//                                               the registers of the backward pass.  (The scan by DPP moves instead of shuffles: slower, it spills.)
+//                value gates                    float32   forward 31.7 us (5.0 TB/s), backward 65 us (4.1 TB/s)
+//   rows, 1665 x 1001, value gates              float32   forward 8.3 us, backward 13.4 us (2.4 and 2.5 TB/s)
 #pragma once
 #include "learning_common.hpp"
 
@@ -414,20 +416,16 @@ __global__ __launch_bounds__(MODE == kAlone ? 256 : 1024, 4) void recurrence_col
   }
 }
 
-#ifndef ROWF
-#define ROWF 4
-#endif
-#ifndef ROWB
-#define ROWB 4
-#endif
-#ifndef ROWFH
-#define ROWFH 8
-#endif
-constexpr int row_steps(size_t size, bool backward) { return size == 4 ? (backward ? ROWB : ROWF) : backward ? 8 : ROWFH; }
 // ---- rows --------------------------------------------------------------------------------------------------------------------------
-// V steps in walking order from s; memory runs the other way when the walk is reversed.  Steps at or behind `end` come back as zero.
+// Steps of a lane: more of them mean fewer levels and lanes of the scans that bound this layout (65536 x 200 float32, value gates, 4 / 8 / 16: forward
+// 40 / 32 / 48 us, backward 81 / 65 / -).
+constexpr int kRowSteps = 8;
+
+// V steps in walking order from s; memory runs the other way when the walk is reversed.  Steps at or behind `end` come back as zero.  A row's last
+// lane may have some of its 16-byte pieces.
 template <typename E, int V>
 __device__ __forceinline__ void load_steps(const E* row, int64_t st, int64_t s, int64_t end, float (&out)[V]) {
+  constexpr int W = 16 / sizeof(E);
   if (s + V <= end) {
     if (st > 0) {
       const Pack<E, V> v = load_pack<E, V>(row + s);
@@ -438,6 +436,14 @@ __device__ __forceinline__ void load_steps(const E* row, int64_t st, int64_t s, 
 #pragma unroll
       for (int j = 0; j < V; ++j) out[j] = static_cast<float>(v.e[V - 1 - j]);
     }
+  } else if constexpr (V > W) {
+    float part[V / W][W];
+#pragma unroll
+    for (int k = 0; k < V / W; ++k) {
+      load_steps<E, W>(row, st, s + k * W, end, part[k]);
+#pragma unroll
+      for (int j = 0; j < W; ++j) out[k * W + j] = part[k][j];
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j) out[j] = s + j < end ? static_cast<float>(row[(s + j) * st]) : 0.0f;
@@ -445,6 +451,7 @@ __device__ __forceinline__ void load_steps(const E* row, int64_t st, int64_t s, 
 }
 template <typename E, int V>
 __device__ __forceinline__ void store_steps(E* row, int64_t st, int64_t s, int64_t end, const float (&in)[V]) {
+  constexpr int W = 16 / sizeof(E);
   if (s + V <= end) {
     Pack<E, V> v;
     if (st > 0) {
@@ -456,11 +463,34 @@ __device__ __forceinline__ void store_steps(E* row, int64_t st, int64_t s, int64
       for (int j = 0; j < V; ++j) v.e[V - 1 - j] = static_cast<E>(in[j]);
       store_pack<E, V>(row - s - (V - 1), v);
     }
+  } else if constexpr (V > W) {
+#pragma unroll
+    for (int k = 0; k < V / W; ++k) {
+      float part[W];
+#pragma unroll
+      for (int j = 0; j < W; ++j) part[j] = in[k * W + j];
+      store_steps<E, W>(row, st, s + k * W, end, part);
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
       if (s + j < end) row[(s + j) * st] = static_cast<E>(in[j]);
   }
+}
+
+// what V steps of one lane compose to, in walking order (DOWN: from the last).  Products that underflow do not drop anything.
+template <int V, bool DOWN>
+__device__ __forceinline__ Composite compose(const float (&keep)[V], const float (&term)[V]) {
+  float a = 1.0f, b = 0.0f;
+  bool dropped = false;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int j = DOWN ? V - 1 - i : i;
+    a *= keep[j];
+    b = apply_step(keep[j], b, term[j]);
+    dropped = dropped || keep[j] == 0.0f;
+  }
+  return {dropped ? 0.0f : a == 0.0f ? 1.4e-45f : a, b};
 }
 
 // n steps of a constant gate without a reset, the power from the table
@@ -473,16 +503,17 @@ __device__ __forceinline__ Composite constant_run(const RecurrenceParams& P, int
   return {P.power[n], b};
 }
 
-// inclusive prefix of the composites over a group of 2^log2 lanes (UP: towards higher lanes), then the exclusive one; `total`: the whole group's
+// inclusive prefix of the composites over a group of 2^log2 lanes (UP: towards higher lanes), then the exclusive one; `total`, where it is wanted: the
+// whole group's
 template <bool UP>
-__device__ __forceinline__ void group_scan(Composite mine, int log2, Composite& exclusive, Composite& total) {
+__device__ __forceinline__ void group_scan(Composite mine, int log2, Composite& exclusive, Composite& total, bool want_total) {
   const int width = 1 << log2, at = (threadIdx.x & 63) & (width - 1);
   for (int d = 1; d < width; d <<= 1) {
     const Composite other = UP ? Composite{__shfl_up(mine.a, d, width), __shfl_up(mine.b, d, width)}
                                : Composite{__shfl_down(mine.a, d, width), __shfl_down(mine.b, d, width)};
     if (UP ? at >= d : at + d < width) mine = then(other, mine);
   }
-  total = {__shfl(mine.a, UP ? width - 1 : 0, width), __shfl(mine.b, UP ? width - 1 : 0, width)};
+  if (want_total) total = {__shfl(mine.a, UP ? width - 1 : 0, width), __shfl(mine.b, UP ? width - 1 : 0, width)};
   if (width > 1) {
     const Composite other = UP ? Composite{__shfl_up(mine.a, 1, width), __shfl_up(mine.b, 1, width)}
                                : Composite{__shfl_down(mine.a, 1, width), __shfl_down(mine.b, 1, width)};
@@ -521,7 +552,7 @@ __global__ __launch_bounds__(256) void recurrence_rows(const RecurrenceParams P)
         const float2 c = P.composites[row * P.segments + q + lane];
         mine = {c.x, c.y};
       }
-      group_scan<true>(mine, log2, exclusive, total);
+      group_scan<true>(mine, log2, exclusive, total, true);
       before = then(before, total);
     }
     carry = then(carry, before);
@@ -563,6 +594,7 @@ __global__ __launch_bounds__(256) void recurrence_rows(const RecurrenceParams P)
   Tile t, next;
   fetch(begin, t);
   for (int64_t base = begin; base < last; base += tile, t = next) {
+    const bool more = COMPOSITES || base + tile < last;
     if (base + tile < last) fetch(base + tile, next);
     const int64_t s = base + static_cast<int64_t>(lane) * V;
     float keep[V], inject[V], term[V];
@@ -574,11 +606,9 @@ __global__ __launch_bounds__(256) void recurrence_rows(const RecurrenceParams P)
       term[j] = FORM == kGateLogit ? inject[j] * t.x[j] : s + j < end ? t.x[j] : 0.0f;
     }
     if (!BACKWARD) {
-      Composite mine = {1.0f, 0.0f}, exclusive, total;
-#pragma unroll
-      for (int j = 0; j < V; ++j) mine = then(mine, {keep[j], term[j]});
+      Composite mine = compose<V, false>(keep, term), exclusive, total;
       if (FORM == kGateConstant && t.cut == 0 && s < end) mine = constant_run(P, s + V <= end ? V : static_cast<int>(end - s), term);
-      group_scan<true>(mine, log2, exclusive, total);
+      group_scan<true>(mine, log2, exclusive, total, more);
       if (!COMPOSITES) {
         float h = then(carry, exclusive).b, out[V];
 #pragma unroll
@@ -589,25 +619,24 @@ __global__ __launch_bounds__(256) void recurrence_rows(const RecurrenceParams P)
         store_steps<E, V>(at(P.h), P.h.st, s, end, out);
         if (P.final_state != nullptr && s < P.steps && s + V >= P.steps && end == P.steps) P.final_state[batch] = h;
       }
-      carry = then(carry, total);
+      if (more) carry = then(carry, total);
     } else {
       // d: the gate in front of each step is its left neighbour's
       const float left = __shfl_up(keep[V - 1], 1, width);
       const float front = lane == 0 ? keep_before : left;
-      Composite mine = {1.0f, 0.0f}, exclusive, total;
+      float factor[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) mine = then(mine, s + j < end ? Composite{j == 0 ? front : keep[j - 1], t.up[j]} : Composite{1.0f, 0.0f});
-      group_scan<true>(mine, log2, exclusive, total);
+      for (int j = 0; j < V; ++j) factor[j] = s + j >= end ? 1.0f : j == 0 ? front : keep[j - 1];
+      Composite mine = compose<V, false>(factor, t.up), exclusive, total;  // (nothing comes in behind the end: up is zero there)
+      group_scan<true>(mine, log2, exclusive, total, more);
       keep_before = __shfl(keep[V - 1], width - 1, width);  // (read only when another tile follows, and then this one was full)
       if (!COMPOSITES) {
         float scale[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) scale[j] = 0.0f;
         if (FORM != kGateConstant) {  // the states once more: forward order runs towards lower lanes
-          Composite states = {1.0f, 0.0f}, behind, unused;
-#pragma unroll
-          for (int j = V - 1; j >= 0; --j) states = then(states, {keep[j], term[j]});
-          group_scan<false>(states, log2, behind, unused);
+          Composite behind, unused;
+          group_scan<false>(compose<V, true>(keep, term), log2, behind, unused, false);
           float h = apply_step(behind.a, t.edge, behind.b);
 #pragma unroll
           for (int j = V - 1; j >= 0; --j) {
@@ -631,7 +660,7 @@ __global__ __launch_bounds__(256) void recurrence_rows(const RecurrenceParams P)
         if (P.dx.p != nullptr) store_steps<E, V>(at(P.dx), P.dx.st, s, end, out);
         if (FORM != kGateConstant && P.dg.p != nullptr) store_steps<E, V>(at(P.dg), P.dg.st, s, end, gate_out);
       }
-      carry = then(carry, total);
+      if (more) carry = then(carry, total);
     }
   }
   if (COMPOSITES && lane == 0 && active) P.composites[row * P.segments + segment] = make_float2(carry.a, carry.b);

@@ -5,7 +5,7 @@
 namespace mbt_learning {
 
 template <typename E>
-constexpr int kVector = 16 / static_cast<int>(sizeof(E));  // columns (or steps) of one 16-byte access
+constexpr int kVector = 16 / static_cast<int>(sizeof(E));  // columns of one 16-byte access
 
 template <typename E, int FORM, int V, bool BACKWARD>
 void (*columns_kernel(int mode))(RecurrenceParams) {
@@ -18,9 +18,8 @@ void (*columns_kernel(int mode))(RecurrenceParams) {
 template <typename E, int FORM, bool BACKWARD>
 void (*pick_recurrence(int which))(RecurrenceParams) {
   if (which >= kRows) {
-    constexpr int V = row_steps(sizeof(E), BACKWARD);
-    if (which - kRows == kComposites) return recurrence_rows<E, FORM, V, BACKWARD, true>;
-    return recurrence_rows<E, FORM, V, BACKWARD, false>;
+    if (which - kRows == kComposites) return recurrence_rows<E, FORM, kRowSteps, BACKWARD, true>;
+    return recurrence_rows<E, FORM, kRowSteps, BACKWARD, false>;
   }
   if constexpr (!BACKWARD) {
     constexpr int V = kVector<E>, K = chunk_steps(FORM, false, V, true);
