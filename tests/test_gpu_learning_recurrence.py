@@ -443,3 +443,13 @@ def test_negated_views_are_refused():
     assert x.is_neg()
     with pytest.raises(ValueError, match="resolve_neg"):
         learning().linear_recurrence(x, 0.5)
+
+
+@pytest.mark.parametrize("shape", [(1024, 3), (1025, 70), (1537, 9), (2048, 5), (2051, 33), (2100, 300), (1000, 1000), (13, 40), (14, 9), (21, 300)], ids=str)
+@pytest.mark.parametrize("layout", ["time_first", "time_last"])
+def test_where_the_splits_of_the_axis_change(shape, layout):
+    """one tile, a few, one segment more or less; rows that end in every piece of a lane's steps"""
+    for form, dtype in (("constant", "float32"), ("logit", "float32"), ("value", "bfloat16"), ("logit", "float16")):
+        print(shape, layout, form, dtype, flush=True)
+        run_case(shape, form, dtype, reverse=False, reset=True, initial=True, layout=layout, seed=31)
+        run_case(shape, form, dtype, reverse=True, reset=False, initial=True, layout=layout, seed=32)
