@@ -706,12 +706,12 @@ typedef struct mbt_recurrence {
   int32_t dtype;                 /* of inputs, gate, states and their gradients */
   int32_t form;                  /* MBT_GATE_* */
   int32_t reverse;
-  int32_t reserved;
+  int32_t edge_steps;            /* how far the states in `edges` lie apart, a power of two; 0 = no `edges` (the two fields at the end are not read) */
   double constant;               /* MBT_GATE_CONSTANT */
   mbt_array3 inputs;             /* forward, and backward unless the gate is a constant */
   mbt_array3 gate;               /* unless the gate is a constant */
   mbt_array3 reset;              /* bytes, or absent */
-  mbt_array3 states;             /* forward: output; backward: that output, unless the gate is a constant */
+  mbt_array3 states;             /* forward: output; backward: that output, where grad_gate is wanted and no `edges` are given */
   const float* initial;          /* (outer, inner) contiguous, or NULL = zeros */
   float* final_state;            /* forward output, (outer, inner) contiguous: the last state in walking order, unrounded; or NULL */
   mbt_array3 grad_states;        /* backward input */
@@ -721,7 +721,14 @@ typedef struct mbt_recurrence {
   float* grad_initial;           /* backward output, (outer, inner), or NULL */
   void* workspace;
   uint64_t workspace_bytes;      /* at least what mbt_recurrence_workspace says */
+  float* edges;                  /* 16-bit states, with grad_gate: forward output (or absent), backward input */
+  uint64_t edges_bytes;          /* at least (ceil(steps / edge_steps) - 1) * outer * inner * 4 */
 } mbt_recurrence;
+/* The gradient of a gate is made of the states, which the backward call works out once more from the inputs, piece by piece.  A piece starts from a state
+ * that the forward call left: of 16-bit `states` that is a rounded one, and its rounding goes into grad_gate, amplified where a state is close to its input.
+ * With `edges` the pieces start from states in float32: the forward call writes them edge_steps apart, for the backward call of the same walk.  This
+ * function says how far apart the backward call of a struct needs them (any power of two that divides it will do); 0 = it needs none. */
+int32_t mbt_recurrence_edge_steps(const mbt_recurrence* r);
 /* Bytes of workspace for these sizes, strides and direction (0 is common); the same struct is then passed to the call. */
 uint64_t mbt_recurrence_workspace(const mbt_recurrence* r, int backward);
 int mbt_recurrence_forward(int device, const mbt_recurrence* r, void* stream);

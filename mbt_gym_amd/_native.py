@@ -205,11 +205,11 @@ class MbtRecurrence(C.Structure):
     """struct mbt_recurrence (include/mbt_env.h)."""
 
     _fields_ = [("outer", C.c_uint64), ("steps", C.c_uint64), ("inner", C.c_uint64), ("dtype", C.c_int32), ("form", C.c_int32),
-                ("reverse", C.c_int32), ("reserved", C.c_int32), ("constant", C.c_double),
+                ("reverse", C.c_int32), ("edge_steps", C.c_int32), ("constant", C.c_double),
                 ("inputs", MbtArray3), ("gate", MbtArray3), ("reset", MbtArray3), ("states", MbtArray3),
                 ("initial", C.c_void_p), ("final_state", C.c_void_p), ("grad_states", MbtArray3), ("grad_final", C.c_void_p),
                 ("grad_inputs", MbtArray3), ("grad_gate", MbtArray3), ("grad_initial", C.c_void_p),
-                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64), ("edges", C.c_void_p), ("edges_bytes", C.c_uint64)]
 
 
 STD_NUMBER, STD_COMPONENT, STD_FULL = 0, 1, 2
@@ -335,6 +335,7 @@ SIGNATURES = {
     "mbt_rng_fill_user_host": (C.c_int, [C.c_int, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint64, _F]),
     "mbt_philox4x32_10_host": (C.c_int, [C.c_int, C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), C.POINTER(C.c_uint32)]),
     "mbt_recurrence_workspace": (C.c_uint64, [C.POINTER(MbtRecurrence), C.c_int]),
+    "mbt_recurrence_edge_steps": (C.c_int32, [C.POINTER(MbtRecurrence)]),
     "mbt_recurrence_forward": (C.c_int, [C.c_int, C.POINTER(MbtRecurrence), C.c_void_p]),
     "mbt_recurrence_backward": (C.c_int, [C.c_int, C.POINTER(MbtRecurrence), C.c_void_p]),
     "mbt_recurrence_step": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_uint64, C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,

@@ -15,6 +15,7 @@ struct Plan {
   int64_t blocks;
   size_t lds;
   uint64_t workspace;
+  int64_t piece;        // steps that the backward pass recomputes from one state
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -46,7 +47,8 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
     return mbt_set_error(MBT_ERR_INVALID, "sizes beyond 2^40");
   const bool gated = r->form != kGateConstant;
   if (gated && r->gate.data == nullptr) return mbt_set_error(MBT_ERR_INVALID, "this form needs a gate array");
-  if ((!backward || gated) && (r->inputs.data == nullptr || r->states.data == nullptr)) return mbt_set_error(MBT_ERR_INVALID, "inputs and states are needed");
+  if ((!backward || gated) && (r->inputs.data == nullptr || (!backward && r->states.data == nullptr)))
+    return mbt_set_error(MBT_ERR_INVALID, "inputs and states are needed");
   if (backward && r->grad_states.data == nullptr) return mbt_set_error(MBT_ERR_INVALID, "the backward pass needs grad_states");
   if (!gated && r->grad_gate.data != nullptr) return mbt_set_error(MBT_ERR_INVALID, "a constant gate has no gradient array");
   if (!gated && !(r->constant - r->constant == 0.0)) return mbt_set_error(MBT_ERR_INVALID, "the constant gate is not finite");
@@ -89,6 +91,18 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
   P.final_state = backward ? nullptr : r->final_state;
   P.dfinal = r->grad_final;
   P.dinitial = r->grad_initial;
+  if (r->edge_steps != 0) {
+    const int64_t apart = r->edge_steps;
+    if (apart < 0 || (apart & (apart - 1)) != 0) return mbt_set_error(MBT_ERR_INVALID, "edge_steps %d is no power of two", r->edge_steps);
+    if (!gated || size != 2) return mbt_set_error(MBT_ERR_INVALID, "edges belong to 16-bit states with gates");
+    const uint64_t needed = (static_cast<uint64_t>(ceil_div(steps, apart)) - 1) * r->outer * r->inner * sizeof(float);
+    if (needed > 0 && (r->edges == nullptr || r->edges_bytes < needed))
+      return mbt_set_error(MBT_ERR_INVALID, "edges has %llu bytes; %llu are needed", (unsigned long long)(r->edges == nullptr ? 0 : r->edges_bytes),
+                           (unsigned long long)needed);
+    if (reinterpret_cast<uintptr_t>(r->edges) % sizeof(float) != 0) return mbt_set_error(MBT_ERR_INVALID, "edges is not aligned to 4 bytes");
+    P.edges = r->edges;
+    P.edge_log2 = log2_ceil(apart);
+  }
   P.steps = steps;
   P.outer = static_cast<int64_t>(swap ? r->inner : r->outer);
   P.inner = static_cast<int64_t>(swap ? r->outer : r->inner);
@@ -123,6 +137,7 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
       P.segments = static_cast<int32_t>(ceil_div(steps, P.segment));
     }
     plan.which = kRows + kJoined;
+    plan.piece = tile;
     plan.threads = 256;
     plan.blocks = ceil_div(batch * P.segments, 256 >> P.lanes_log2);
     if (P.segments > 1) plan.workspace = static_cast<uint64_t>(batch) * P.segments * sizeof(float2);
@@ -140,12 +155,14 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
   P.vectors_per_outer = ceil_div(P.inner, v);
   P.vectors = P.outer * P.vectors_per_outer;
   const int chunk = chunk_steps(r->form, backward, v, false);
+  plan.piece = chunk;
   int64_t parallel = ceil_div(chip, P.vectors);
   if (parallel > ceil_div(steps, chunk)) parallel = ceil_div(steps, chunk);
   // With two thirds of the chip's threads or more a thread walks its columns alone, without joins (200 x 3 * 2^16 bfloat16: 40 us forward and 98
   // backward, 51 and 116 joined; 50 x 3 * 2^16 15 and 18, 21 and 35); with a half it would not (200 x 2^16 float32: 29.4 and 56, joined 28.3 and 51).
   if (wide || parallel <= 3) {
     plan.which = base + kAlone;
+    plan.piece = chunk_steps(r->form, backward, v, true);
     if (wide && batch * steps * static_cast<int64_t>(size) * count > (int64_t{256} << 20)) plan.which = base + kStreamed;  // (beyond the last cache)
     plan.threads = 256;
     plan.blocks = ceil_div(P.vectors, 256);
@@ -200,6 +217,10 @@ int run(int device, const mbt_recurrence* r, bool backward, void* stream) {
     return mbt_set_error(MBT_ERR_INVALID, "the workspace has %llu bytes; %llu are needed (mbt_recurrence_workspace)",
                          (unsigned long long)(r->workspace == nullptr ? 0 : r->workspace_bytes), (unsigned long long)plan.workspace);
   if (reinterpret_cast<uintptr_t>(r->workspace) % sizeof(float2) != 0) return mbt_set_error(MBT_ERR_INVALID, "the workspace is not aligned to 8 bytes");
+  if (backward && r->form != kGateConstant && r->grad_gate.data != nullptr && r->edge_steps == 0 && r->states.data == nullptr && plan.params.steps > plan.piece)
+    return mbt_set_error(MBT_ERR_INVALID, "grad_gate needs states or edges");
+  if (backward && r->edge_steps != 0 && plan.piece % r->edge_steps != 0)
+    return mbt_set_error(MBT_ERR_INVALID, "edges %d steps apart: every %lld steps one is needed (mbt_recurrence_edge_steps)", r->edge_steps, (long long)plan.piece);
   DeviceScope scope;
   rc = scope.enter(device);
   if (rc != MBT_OK) return rc;
@@ -226,6 +247,13 @@ extern "C" {
 uint64_t mbt_recurrence_workspace(const mbt_recurrence* r, int backward) {
   mbt_learning::Plan plan;
   return mbt_learning::make_plan(r, backward != 0, plan) == MBT_OK ? plan.workspace : 0;
+}
+
+int32_t mbt_recurrence_edge_steps(const mbt_recurrence* r) {
+  using namespace mbt_learning;
+  Plan plan;
+  if (make_plan(r, true, plan) != MBT_OK || dtype_size(r->dtype) != 2 || r->form == kGateConstant) return 0;
+  return plan.params.steps > plan.piece ? static_cast<int32_t>(plan.piece) : 0;
 }
 
 int mbt_recurrence_forward(int device, const mbt_recurrence* r, void* stream) { return mbt_learning::run(device, r, false, stream); }

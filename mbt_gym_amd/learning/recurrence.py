@@ -42,6 +42,8 @@ class _Plan:
         for name in ("inputs", "states", "grad_states", "grad_inputs") + (() if gate is None else ("gate", "grad_gate")):
             getattr(r, name).data = 16
         self.workspace = lib.mbt_recurrence_workspace(r, 0), lib.mbt_recurrence_workspace(r, 1)
+        self.edge_steps = lib.mbt_recurrence_edge_steps(r)
+        self.edges = -(-shape[axis] // self.edge_steps) - 1 if self.edge_steps else 0
 
     def struct(self):
         return _native.MbtRecurrence.from_buffer_copy(self.template)
@@ -70,8 +72,8 @@ def _plan_of(inputs, gate, reset, settings):
     return plan
 
 
-def _forward(inputs, gate, initial, reset, settings):
-    """(states, final state, plan, and the operands it belongs to)"""
+def _forward(inputs, gate, initial, reset, settings, for_gate=False):
+    """(states, final state, edges - for the gate's gradient, if it is wanted and they are needed, else None - plan, and the operands it belongs to)"""
     plan = _plan_of(inputs, gate, reset, settings)
     if not plan.folds:  # (batch axes that do not fold into two: copies that do)
         inputs, gate, reset = (None if t is None else t.contiguous() for t in (inputs, gate, reset))
@@ -87,18 +89,23 @@ def _forward(inputs, gate, initial, reset, settings):
         r.reset.data = reset.data_ptr()
     if initial is not None:
         r.initial = initial.data_ptr()
+    edges = None
+    if for_gate and plan.edges:
+        edges = torch.empty([plan.edges] + plan.batch, dtype=torch.float32, device=device)
+        r.edge_steps, r.edges, r.edges_bytes = plan.edge_steps, edges.data_ptr(), 4 * edges.numel()
     plan.launch(_native.load_library().mbt_recurrence_forward, r, 0, device)
-    return states, final, plan, inputs, gate, reset
+    return states, final, edges, plan, inputs, gate, reset
 
 
 class _LinearRecurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, inputs, gate, initial, reset, settings):
-        states, final, plan, inputs, gate, reset = _forward(inputs, gate, initial, reset, settings)
+        states, final, edges, plan, inputs, gate, reset = _forward(inputs, gate, initial, reset, settings, ctx.needs_input_grad[1])
         if gate is None:
-            ctx.save_for_backward(None, None, initial, reset, None)
-        else:
-            ctx.save_for_backward(inputs, gate, initial, reset, states)
+            ctx.save_for_backward(None, None, initial, reset, None, None)
+        else:  # (the backward pass looks at states only for the gate's gradient: float32 ones as they were stored, or the edges)
+            ctx.save_for_backward(inputs, gate, initial, reset, states if ctx.needs_input_grad[1] and states.dtype is torch.float32 else None, edges)
+        ctx.edge_steps = plan.edge_steps
         ctx.plan, ctx.settings, ctx.shape, ctx.dtype, ctx.device = plan, settings, states.shape, states.dtype, states.device
         ctx.reset_strides = None if reset is None else reset.stride()
         ctx.set_materialize_grads(False)
@@ -107,17 +114,21 @@ class _LinearRecurrence(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_states, grad_final):
-        inputs, gate, initial, reset, states = ctx.saved_tensors
+        inputs, gate, initial, reset, states, edges = ctx.saved_tensors
         if grad_states is None and grad_final is None:
             return (None,) * 5
         plan, device = ctx.plan, ctx.device
+        if initial is not None:
+            initial = initial.contiguous()  # (as it was saved, unless a hook brought it back otherwise)
         if gate is not None:
             plan = _plan_of(inputs, gate, reset, ctx.settings)  # (the same one, unless a hook on saved tensors brought them back in another layout)
             if not plan.folds:
                 inputs, gate, reset = (None if t is None else t.contiguous() for t in (inputs, gate, reset))
                 plan = _plan_of(inputs, gate, reset, ctx.settings)
-            if states.stride() != plan.strides:
+            if states is not None and states.stride() != plan.strides:
                 states = _laid_out(states, plan.strides)
+            if ctx.needs_input_grad[1] and plan.edges and plan.edge_steps != ctx.edge_steps:  # (that layout is walked in other pieces)
+                edges = _forward(inputs, gate, initial, reset, ctx.settings, True)[2]
         elif reset is not None and reset.stride() != ctx.reset_strides:
             reset = _laid_out(reset, ctx.reset_strides)
         if grad_states is None:
@@ -127,11 +138,15 @@ class _LinearRecurrence(torch.autograd.Function):
         r = plan.struct()
         r.grad_states.data = grad_states.data_ptr()
         if gate is not None:
-            r.inputs.data, r.gate.data, r.states.data = inputs.data_ptr(), gate.data_ptr(), states.data_ptr()
+            r.inputs.data, r.gate.data = inputs.data_ptr(), gate.data_ptr()
+            if states is not None:
+                r.states.data = states.data_ptr()
+            if ctx.needs_input_grad[1] and plan.edges:
+                edges = edges.contiguous()
+                r.edge_steps, r.edges, r.edges_bytes = plan.edge_steps, edges.data_ptr(), 4 * edges.numel()
         if reset is not None:
             r.reset.data = reset.data_ptr()
         if initial is not None:
-            initial = initial.contiguous()  # (as it was saved, unless a hook brought it back otherwise)
             r.initial = initial.data_ptr()
         wanted = ctx.needs_input_grad
         grad_inputs = grad_gate = grad_initial = None
@@ -169,8 +184,8 @@ def linear_recurrence(inputs: torch.Tensor, gate: Union[float, torch.Tensor], in
     return_final  also return the last state of the walk in float32, for a recording that comes in pieces
 
     A gate of exactly zero, like a reset, drops the state it meets whatever that holds: infinities and NaN do not pass it.  A sequence without
-    steps has no states, and its final state is the initial one.  Gradients are exact for the stored inputs and gates: the states that they
-    need are recomputed from them.  Second derivatives are refused."""
+    steps has no states, and its final state is the initial one.  Gradients are those of the stored inputs and gates: the
+    states that they need are recomputed from them, in float32 whatever the states are stored in.  Second derivatives are refused."""
     require(inputs, "inputs", dtypes=DTYPES)
     if inputs.dim() == 0:
         raise ValueError("inputs is a scalar: it has no time axis")

@@ -1,0 +1,109 @@
+"""mbt_gym_amd.learning: gradients of the recurrence where they can lose accuracy that float32 states and a double constant have."""
+import numpy as np
+import pytest
+
+from tests.learning_oracle import U, Recurrence, assert_within
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
+
+
+def learning():
+    from mbt_gym_amd import learning as module
+
+    return module
+
+
+def to64(t):
+    return t.detach().double().cpu().numpy()
+
+
+class Float32States(Recurrence):
+    """The definition with the bounds of states that the gradients use in float32: no rounding to the element type in front of a gradient."""
+
+    def __init__(self, *args, **options):
+        super().__init__(*args, **options)
+        first = 64 * U * np.abs(self.h0)
+        self.before_bound = np.where(self.cut, 0.0, np.concatenate([first[None], self.bound[:-1]]))
+
+
+def levels(shape, kind, seed):
+    """Inputs with a level, as prices and biased layers have them: noise of a twentieth around one, or a slow wave around one."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    if kind == "noise":
+        return 1.0 + 0.05 * torch.randn(shape, generator=gen, device="cuda")
+    t = torch.arange(shape[0], device="cuda", dtype=torch.float32).reshape((-1,) + (1,) * (len(shape) - 1))
+    return 1.0 + 0.3 * torch.sin(t / 40.0 + 6.0 * torch.rand(shape[1:], generator=gen, device="cuda"))
+
+
+def place(t, layout):
+    return t.movedim(0, -1).contiguous().movedim(-1, 0) if layout == "time_last" else t.contiguous()
+
+
+def check(x, gate, h0, cut, form, dtype, reverse, what, hooks=None):
+    leaves = [t.detach().requires_grad_(True) for t in (x, gate, h0)]
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    up, up_final = torch.randn(x.shape, generator=gen, device="cuda").to(x.dtype), torch.randn(h0.shape, generator=gen, device="cuda")
+    with hooks or torch.enable_grad():
+        states, final = learning().linear_recurrence(*leaves, reset=cut, reverse=reverse, gate_is_logit=form == "logit", return_final=True)
+    grads = torch.autograd.grad([states, final], leaves, [up, up_final])
+    ref = Float32States(to64(x), to64(gate), form, to64(h0), None if cut is None else cut.cpu().numpy(), reverse, dtype)
+    for name, grad in zip(("inputs", "gate", "initial"), grads):
+        value, bound = ref.gradients(to64(up), to64(up_final))[name]
+        assert_within(to64(grad), value, bound, (name,) + what)
+
+
+# in pieces of every kind: alone with its column, chunks of a workgroup, segments, pairs and single columns, rows of one tile and of several, in segments
+@pytest.mark.parametrize("shape, layout", [((5, 7), "time_first"), ((200, 2048), "time_first"), ((20, 1 << 18), "time_first"), ((21, (1 << 18) + 1), "time_first"),
+                                           ((2100, 33), "time_first"), ((9000, 66), "time_first"), ((70, 6, 3), "time_last"), ((600, 500), "time_last"),
+                                           ((2100, 40), "time_last"), ((9001, 5), "time_last")], ids=str)
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_gate_gradients_of_16_bit_states_do_not_carry_their_rounding(shape, layout, dtype):
+    for kind, form, reverse, reset in (("noise", "logit", False, False), ("wave", "logit", True, True), ("noise", "value", True, False)):
+        print(shape, layout, dtype, kind, form, flush=True)
+        gen = torch.Generator(device="cuda").manual_seed(3)
+        gate = torch.randn(shape, generator=gen, device="cuda") + 2.0
+        gate = gate if form == "logit" else torch.sigmoid(gate)
+        x, gate = (place(t.to(DTYPES[dtype]), layout) for t in (levels(shape, kind, 1), gate))
+        cut = place(torch.rand(shape, generator=gen, device="cuda") < 0.02, layout) if reset else None
+        check(x, gate, torch.ones(shape[1:], device="cuda"), cut, form, dtype, reverse, (shape, layout, dtype, kind, form))
+
+
+@pytest.mark.parametrize("shape, layout", [((70, 10), "time_first"), ((300, 7), "time_first"), ((1100, 6), "time_last")], ids=str)
+def test_states_beyond_float16_leave_the_gradients_finite(shape, layout):
+    """gates of 0.9 carry inputs of 30000 to a state of 300000, which float16 stores as an infinity"""
+    x = place(torch.full(shape, 30000.0, device="cuda").half(), layout)
+    gate = place(torch.full(shape, 0.9, device="cuda").half(), layout).requires_grad_(True)
+    up = torch.full(shape, 1e-3, device="cuda").half()
+    states = learning().linear_recurrence(x, gate)
+    assert torch.isinf(states).any()
+    grad, = torch.autograd.grad(states, gate, up)
+    ref = Float32States(to64(x), to64(gate), "value", dtype="float16")
+    assert_within(to64(grad), *ref.gradients(to64(up))["gate"], shape)
+
+
+def test_saved_16_bit_operands_that_come_back_in_another_layout():
+    """... are walked in other pieces than the ones that the forward pass left states for"""
+    other = (lambda t: t.clone(), lambda t: t.movedim(0, -1).contiguous().movedim(-1, 0) if t.dim() > 1 else t)
+    host = (lambda t: t.cpu(), lambda t: t.cuda())
+    for shape, layout in (((900, 12, 4), "time_first"), ((900, 12, 4), "time_last")):
+        gen = torch.Generator(device="cuda").manual_seed(3)
+        gate = place((torch.randn(shape, generator=gen, device="cuda") + 2.0).bfloat16(), layout)
+        x = place(levels(shape, "noise", 1).bfloat16(), layout)
+        back = other if layout == "time_first" else (lambda t: t.clone(), lambda t: t.contiguous())
+        for hooks in (back, host):
+            check(x, gate, torch.ones(shape[1:], device="cuda"), None, "logit", "bfloat16", False, (shape, layout), torch.autograd.graph.saved_tensors_hooks(*hooks))
+
+
+def test_gradients_of_some_operands_alone():
+    shape = (300, 64)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for dtype in ("float32", "bfloat16"):
+        x, gate = (t.to(DTYPES[dtype]) for t in (levels(shape, "noise", 1), torch.randn(shape, generator=gen, device="cuda") + 2.0))
+        h0, up = torch.ones(64, device="cuda"), torch.randn(shape, generator=gen, device="cuda").to(DTYPES[dtype])
+        expected = Float32States(to64(x), to64(gate), "logit", to64(h0), dtype=dtype).gradients(to64(up))
+        for which, name in enumerate(("inputs", "gate", "initial")):
+            operands = [t.detach().requires_grad_(k == which) for k, t in enumerate((x, gate, h0))]
+            grad, = torch.autograd.grad(learning().linear_recurrence(*operands, gate_is_logit=True), operands[which], up)
+            assert_within(to64(grad), *expected[name], (dtype, name))
