@@ -15,7 +15,7 @@
 // piece.  That is the stored one where states are float32; of 16-bit states the forward pass leaves the ones that the backward pass starts from in
 // float32 as well (`edges`: a float every 4 to 16 steps of a column, every 512 of a row), so that their rounding stays out of dg = d f (1 - f) (h - x),
 // which is a small difference wherever a state follows its input (inputs 1 + 0.05 noise, bfloat16, 200 steps: dg off by 0.0017, one rounding; started
-// from rounded states by 0.0095).
+// from rounded states by 0.0096).
 //
 // Two layouts, each with one element of time per register so that no shared-memory transpose is needed:
 //   columns  a batch axis is contiguous (time-major recordings, (B, T, C) activations): lanes lie across the batch, one float32 or two 16-bit
@@ -81,11 +81,11 @@ __device__ __forceinline__ Composite then(Composite first, Composite second) {
   if (a == 0.0f && first.a != 0.0f && second.a != 0.0f) a = 1.4e-45f;
   return {a, apply_step(second.a, first.b, second.b)};
 }
-// one step of the walk
+// one step of the walk.  ENTERING: the backward pass's first, where d = grad_final comes in with a factor of one, not with the constant and its rest
 template <int FORM>
-__device__ __forceinline__ float advance(const RecurrenceParams& P, float keep, float h, float b) {
+__device__ __forceinline__ float advance(const RecurrenceParams& P, float keep, float h, float b, bool entering = false) {
   if (FORM != kGateConstant) return apply_step(keep, h, b);
-  return keep == 0.0f ? b : __builtin_fmaf(keep, h, __builtin_fmaf(P.constant_rest, h, b));
+  return keep == 0.0f ? b : __builtin_fmaf(keep, h, __builtin_fmaf(entering ? 0.0f : P.constant_rest, h, b));
 }
 
 // f = sigmoid(k) and 1 - f, each to about an ulp: e = exp(-|k|) with the rounding of the exponent's product carried along, r = 1 / (1 + e) by one
@@ -351,7 +351,7 @@ __device__ __forceinline__ void walk_chunk(const RecurrenceParams& P, const Colu
         float out[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          start[j] = advance<FORM>(P, factor(k, j), start[j], up[k][j]);
+          start[j] = advance<FORM>(P, factor(k, j), start[j], up[k][j], k == 0 && s0 == 0);
           out[j] = inject[k][j] * start[j];
         }
         if (P.dx.p != nullptr) col.store(pdx, out);
@@ -686,7 +686,7 @@ __global__ __launch_bounds__(256) void recurrence_rows(const RecurrenceParams P)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           if (s + j < end) {
-            d = advance<FORM>(P, j == 0 ? front : keep[j - 1], d, t.up[j]);
+            d = advance<FORM>(P, j == 0 ? front : keep[j - 1], d, t.up[j], j == 0 && s == 0);
             if (s + j + 1 == P.steps && P.dinitial != nullptr) P.dinitial[batch] = advance<FORM>(P, keep[j], d, 0.0f);
           }
           out[j] = inject[j] * d;

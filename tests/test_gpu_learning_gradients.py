@@ -107,3 +107,25 @@ def test_gradients_of_some_operands_alone():
             operands = [t.detach().requires_grad_(k == which) for k, t in enumerate((x, gate, h0))]
             grad, = torch.autograd.grad(learning().linear_recurrence(*operands, gate_is_logit=True), operands[which], up)
             assert_within(to64(grad), *expected[name], (dtype, name))
+
+
+class Constant(Float32States):
+    """A constant gate as the double that it is: the definition with a gate array."""
+
+    def __init__(self, x, constant, **options):
+        super().__init__(x, np.full(np.shape(x), constant), "value", **options)
+
+
+@pytest.mark.parametrize("constant", [1000.1, -1000000.03, 0.1, 1.0])
+@pytest.mark.parametrize("steps", [1, 2, 3])
+@pytest.mark.parametrize("layout", ["time_first", "time_last"])
+def test_the_gradient_of_the_final_state_enters_a_constant_walk_with_a_factor_of_one(constant, steps, layout):
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    x, h0, up_final = (torch.randn(s, generator=gen, device="cuda") for s in ((steps, 6), (6,), (6,)))
+    leaves = [place(x, layout).requires_grad_(True), h0.requires_grad_(True)]
+    for up in (torch.zeros_like(x), torch.randn(x.shape, generator=gen, device="cuda")):
+        states, final = learning().linear_recurrence(leaves[0], constant, leaves[1], return_final=True)
+        grads = torch.autograd.grad([states, final], leaves, [up, up_final])
+        expected = Constant(to64(x), constant, initial=to64(h0)).gradients(to64(up), to64(up_final))
+        for name, grad in zip(("inputs", "initial"), grads):
+            assert_within(to64(grad), *expected[name], (name, constant, steps, layout))
