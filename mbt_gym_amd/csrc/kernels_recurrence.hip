@@ -1,4 +1,6 @@
 // The C entry points of the gated linear recurrence: argument checks, the choice of layout and split, launches (kernels: recurrence.hpp).
+#include <cmath>
+
 #include "recurrence.hpp"
 
 namespace mbt_learning {
@@ -107,11 +109,15 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
   P.outer = static_cast<int64_t>(swap ? r->inner : r->outer);
   P.inner = static_cast<int64_t>(swap ? r->outer : r->inner);
   P.batch_swapped = swap ? 1 : 0;
-  P.constant = static_cast<float>(r->constant);
+  auto not_dropped = [&](double v) {  // (only a constant of zero drops what it meets: one that float32 cannot hold is its smallest number)
+    const float f = static_cast<float>(v);
+    return f == 0.0f && r->constant != 0.0 ? std::copysign(1.4e-45f, f) : f;
+  };
+  P.constant = not_dropped(r->constant);
   P.constant_rest = static_cast<float>(r->constant - static_cast<double>(P.constant));
   double power = 1.0;
   for (int k = 0; k <= kMostSteps; ++k) {
-    P.power[k] = static_cast<float>(power);
+    P.power[k] = not_dropped(power);
     power *= r->constant;
   }
   P.segments = 1;

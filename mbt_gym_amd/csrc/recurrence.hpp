@@ -66,7 +66,7 @@ struct RecurrenceParams {
   int32_t batch_swapped;  // initial / final are (outer, inner) of the CALLER: 1 when the kernel's axes are exchanged
   int64_t column_blocks;
   // the constant gate as a float32 pair (0.99 is not a float32 number, and its error would be made at every step), and the powers of the
-  // double that a chunk of n steps composes to
+  // double that a chunk of n steps composes to; neither is zero unless the double is
   float constant, constant_rest;
   float power[kMostSteps + 1];
 };
@@ -75,10 +75,13 @@ struct Composite {
   float a, b;
 };
 __device__ __forceinline__ float apply_step(float keep, float h, float b) { return keep == 0.0f ? b : __builtin_fmaf(keep, h, b); }
-// first, then second.  The product of two non-zero gates must not underflow to the zero that means "dropped".  A state is the composite (0, h).
+// The product of gates that are not zero must not underflow to the zero that means "dropped": it stays the smallest number, of its own sign (an
+// infinity that it meets changes sign with it).
+__device__ __forceinline__ float not_dropped(float a) { return a == 0.0f ? __builtin_copysignf(1.4e-45f, a) : a; }
+// first, then second.  A state is the composite (0, h).
 __device__ __forceinline__ Composite then(Composite first, Composite second) {
   float a = first.a * second.a;
-  if (a == 0.0f && first.a != 0.0f && second.a != 0.0f) a = 1.4e-45f;
+  if (first.a != 0.0f && second.a != 0.0f) a = not_dropped(a);
   return {a, apply_step(second.a, first.b, second.b)};
 }
 // one step of the walk.  ENTERING: the backward pass's first, where d = grad_final comes in with a factor of one, not with the constant and its rest
@@ -305,7 +308,7 @@ __device__ __forceinline__ void walk_chunk(const RecurrenceParams& P, const Colu
         }
       }
       if (FORM == kGateConstant) a = P.power[BACKWARD && s0 == 0 && n > 0 ? n - 1 : n];
-      mine[j] = {dropped ? 0.0f : a == 0.0f ? 1.4e-45f : a, b};  // (a product that underflowed does not drop anything)
+      mine[j] = {dropped ? 0.0f : not_dropped(a), b};
     }
     join_chunks<V>(mine, carry, more, P.lanes_log2, lds);
 #pragma unroll
@@ -505,7 +508,7 @@ __device__ __forceinline__ void store_steps(E* row, int64_t st, int64_t s, int64
   }
 }
 
-// what V steps of one lane compose to, in walking order (DOWN: from the last).  Products that underflow do not drop anything.
+// what V steps of one lane compose to, in walking order (DOWN: from the last)
 template <int V, bool DOWN>
 __device__ __forceinline__ Composite compose(const float (&keep)[V], const float (&term)[V]) {
   float a = 1.0f, b = 0.0f;
@@ -517,7 +520,7 @@ __device__ __forceinline__ Composite compose(const float (&keep)[V], const float
     b = apply_step(keep[j], b, term[j]);
     dropped = dropped || keep[j] == 0.0f;
   }
-  return {dropped ? 0.0f : a == 0.0f ? 1.4e-45f : a, b};
+  return {dropped ? 0.0f : not_dropped(a), b};
 }
 
 // n steps of a constant gate without a reset, the power from the table

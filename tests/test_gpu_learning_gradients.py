@@ -129,3 +129,34 @@ def test_the_gradient_of_the_final_state_enters_a_constant_walk_with_a_factor_of
         expected = Constant(to64(x), constant, initial=to64(h0)).gradients(to64(up), to64(up_final))
         for name, grad in zip(("inputs", "initial"), grads):
             assert_within(to64(grad), *expected[name], (name, constant, steps, layout))
+
+
+@pytest.mark.parametrize("constant", [1e-7, -1e-30, 1e-50, 0.2])
+@pytest.mark.parametrize("steps", [3, 16, 100, 3000])
+@pytest.mark.parametrize("layout", ["time_first", "time_last"])
+def test_a_constant_gate_that_is_not_zero_drops_nothing(constant, steps, layout):
+    """a NaN goes on to the end of the walk, forwards and backwards, however small the constant's powers get"""
+    x, h0 = torch.zeros(steps, 6, device="cuda"), torch.zeros(6, device="cuda")
+    h0[0], x[steps // 2, 1] = float("nan"), float("nan")
+    leaves = [place(x, layout).requires_grad_(True), h0.requires_grad_(True)]
+    states, final = learning().linear_recurrence(leaves[0], constant, leaves[1], return_final=True)
+    nan = torch.isnan(states)
+    assert nan[:, 0].all() and nan[steps // 2:, 1].all() and not nan[:steps // 2, 1].any() and not nan[:, 2:].any()
+    assert torch.isnan(final).tolist() == [True, True] + [False] * 4
+    up_final = torch.zeros(6, device="cuda")
+    up_final[3] = float("nan")
+    grads = torch.autograd.grad(final, leaves, up_final)
+    assert torch.isnan(grads[0])[:, 3].all() and torch.isnan(grads[1]).tolist() == [False] * 3 + [True] + [False] * 2
+    dropped = learning().linear_recurrence(leaves[0], 0.0, leaves[1])  # (a constant of zero does)
+    assert int(torch.isnan(dropped).sum()) == 1
+
+
+@pytest.mark.parametrize("steps", [20, 300, 3000])
+@pytest.mark.parametrize("layout", ["time_first", "time_last"])
+def test_an_infinity_keeps_the_sign_of_the_product_of_its_gates(steps, layout):
+    """... of gates whose product has long underflown"""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    signs = torch.sign(torch.rand(steps, 40, generator=gen, device="cuda") - 0.4)
+    x, gate = torch.zeros(steps, 40, device="cuda"), 1e-6 * signs
+    states = learning().linear_recurrence(place(x, layout), place(gate, layout), torch.full((40,), float("inf"), device="cuda"))
+    assert np.array_equal(to64(states), np.cumprod(to64(signs), axis=0) * np.inf)
