@@ -88,7 +88,9 @@ __device__ __forceinline__ Composite then(Composite first, Composite second) {
 template <int FORM>
 __device__ __forceinline__ float advance(const RecurrenceParams& P, float keep, float h, float b, bool entering = false) {
   if (FORM != kGateConstant) return apply_step(keep, h, b);
-  return keep == 0.0f ? b : __builtin_fmaf(keep, h, __builtin_fmaf(entering ? 0.0f : P.constant_rest, h, b));
+  // (an infinite state is one times the constant; times its rest, which may be zero or of the other sign, it would turn into a NaN)
+  const float finite = __builtin_amdgcn_fmed3f(h, -3.40282347e38f, 3.40282347e38f);
+  return keep == 0.0f ? b : __builtin_fmaf(keep, h, __builtin_fmaf(entering ? 0.0f : P.constant_rest, finite, b));
 }
 
 // f = sigmoid(k) and 1 - f, each to about an ulp: e = exp(-|k|) with the rounding of the exponent's product carried along, r = 1 / (1 + e) by one

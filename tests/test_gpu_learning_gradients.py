@@ -160,3 +160,27 @@ def test_an_infinity_keeps_the_sign_of_the_product_of_its_gates(steps, layout):
     x, gate = torch.zeros(steps, 40, device="cuda"), 1e-6 * signs
     states = learning().linear_recurrence(place(x, layout), place(gate, layout), torch.full((40,), float("inf"), device="cuda"))
     assert np.array_equal(to64(states), np.cumprod(to64(signs), axis=0) * np.inf)
+
+
+@pytest.mark.parametrize("constant", [1.0, 0.5, 0.99, 0.1, -0.3])
+@pytest.mark.parametrize("steps", [1, 5, 40, 3000])
+@pytest.mark.parametrize("layout", ["time_first", "time_last"])
+def test_an_infinite_state_under_a_constant_gate_stays_one(constant, steps, layout):
+    """forwards and backwards, from the first step and from the middle; signs change with a negative gate"""
+    x, h0 = torch.zeros(steps, 70, device="cuda"), torch.zeros(70, device="cuda")
+    h0[0], h0[1], x[steps // 2, 2] = float("inf"), float("-inf"), float("inf")
+    leaves = [place(x, layout).requires_grad_(True), h0.requires_grad_(True)]
+    states, final = learning().linear_recurrence(leaves[0], constant, leaves[1], return_final=True)
+    for column, start, first in ((0, 1.0, 0), (1, -1.0, 0), (2, 1.0, steps // 2)):
+        powers = np.sign(constant) ** np.arange(1 if column < 2 else 0, steps - first + (1 if column < 2 else 0))
+        assert np.array_equal(to64(states)[first:, column], start * powers * np.inf), column
+    assert not torch.isnan(states).any() and np.array_equal(to64(final), to64(states[-1]))
+    up = torch.zeros(steps, 70, device="cuda")
+    up[steps // 2, 3] = float("inf")
+    up_final = torch.zeros(70, device="cuda")
+    up_final[4] = float("-inf")
+    grads = torch.autograd.grad([states, final], leaves, [up, up_final])
+    signs = np.sign(constant) ** np.arange(steps)
+    assert np.array_equal(to64(grads[0])[:steps // 2 + 1, 3], signs[:steps // 2 + 1][::-1] * np.inf)
+    assert np.array_equal(to64(grads[0])[:, 4], -signs[::-1] * np.inf)
+    assert not torch.isnan(grads[0]).any() and not torch.isnan(grads[1]).any()
