@@ -525,14 +525,20 @@ __device__ __forceinline__ Composite compose(const float (&keep)[V], const float
   return {dropped ? 0.0f : not_dropped(a), b};
 }
 
-// n steps of a constant gate without a reset, the power from the table
+// what the first n steps of one lane compose to under a constant gate: the constant with its rest, its power from the table (a drop leaves none).
+// ENTERING: the first factor is one, not the constant.
 template <int V>
-__device__ __forceinline__ Composite constant_run(const RecurrenceParams& P, int n, const float (&term)[V]) {
+__device__ __forceinline__ Composite constant_run(const RecurrenceParams& P, int n, bool entering, const float (&factor)[V], const float (&term)[V]) {
   float b = 0.0f;
+  bool dropped = false;
 #pragma unroll
-  for (int j = 0; j < V; ++j)
-    if (j < n) b = advance<kGateConstant>(P, P.constant, b, term[j]);
-  return {P.power[n], b};
+  for (int j = 0; j < V; ++j) {
+    if (j < n) {
+      b = advance<kGateConstant>(P, factor[j], b, term[j], j == 0 && entering);
+      dropped = dropped || factor[j] == 0.0f;
+    }
+  }
+  return {dropped ? 0.0f : P.power[entering && n > 0 ? n - 1 : n], b};
 }
 
 // inclusive prefix of the composites over a group of 2^log2 lanes (UP: towards higher lanes), then the exclusive one; `total`, where it is wanted: the
@@ -631,6 +637,7 @@ __global__ __launch_bounds__(256) void recurrence_rows(const RecurrenceParams P)
     const bool more = COMPOSITES || base + tile < last;
     if (base + tile < last) fetch(base + tile, next);
     const int64_t s = base + static_cast<int64_t>(lane) * V;
+    const int n = s >= end ? 0 : end - s < V ? static_cast<int>(end - s) : V;
     float keep[V], inject[V], term[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -640,8 +647,8 @@ __global__ __launch_bounds__(256) void recurrence_rows(const RecurrenceParams P)
       term[j] = FORM == kGateLogit ? inject[j] * t.x[j] : s + j < end ? t.x[j] : 0.0f;
     }
     if (!BACKWARD) {
-      Composite mine = compose<V, false>(keep, term), exclusive, total;
-      if (FORM == kGateConstant && t.cut == 0 && s < end) mine = constant_run(P, s + V <= end ? V : static_cast<int>(end - s), term);
+      const Composite mine = FORM == kGateConstant ? constant_run(P, n, false, keep, term) : compose<V, false>(keep, term);
+      Composite exclusive, total;
       group_scan<true>(mine, log2, exclusive, total, more);
       if (!COMPOSITES) {
         float h = then(carry, exclusive).b, out[V];
@@ -667,7 +674,9 @@ __global__ __launch_bounds__(256) void recurrence_rows(const RecurrenceParams P)
       float factor[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) factor[j] = s + j >= end ? 1.0f : j == 0 ? front : keep[j - 1];
-      Composite mine = compose<V, false>(factor, t.up), exclusive, total;  // (nothing comes in behind the end: up is zero there)
+      // (nothing comes in behind the end: up is zero there)
+      const Composite mine = FORM == kGateConstant ? constant_run(P, n, s == 0, factor, t.up) : compose<V, false>(factor, t.up);
+      Composite exclusive, total;
       group_scan<true>(mine, log2, exclusive, total, more);
       keep_before = __shfl(keep[V - 1], width - 1, width);  // (read only when another tile follows, and then this one was full)
       if (!COMPOSITES) {

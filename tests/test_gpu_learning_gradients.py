@@ -184,3 +184,36 @@ def test_an_infinite_state_under_a_constant_gate_stays_one(constant, steps, layo
     assert np.array_equal(to64(grads[0])[:steps // 2 + 1, 3], signs[:steps // 2 + 1][::-1] * np.inf)
     assert np.array_equal(to64(grads[0])[:, 4], -signs[::-1] * np.inf)
     assert not torch.isnan(grads[0]).any() and not torch.isnan(grads[1]).any()
+
+
+@pytest.mark.parametrize("steps, lanes", [(200, 3000), (3000, 40), (65536, 4)], ids=str)
+@pytest.mark.parametrize("flags", [False, True])
+@pytest.mark.parametrize("layout", ["time_first", "time_last"])
+def test_a_long_walk_decays_with_the_double_constant(steps, lanes, flags, layout):
+    """The response to one input, forwards, and to one gradient, backwards, is c^D at distance D, relative to which every rounding counts the same.  A step of
+    the walk is one rounding (of the product with the constant; that with its rest is 2^-24 of it).  Chunks of n >= 8 steps compose to a rounded power,
+    and each composite is multiplied into the next with one rounding more: 2 U a chunk, and 16 steps walked at either end.  The constant is nearly
+    half a float32 step off the next float32 number, so a walk with that one leaves the bound."""
+    nearest = float(np.float32(0.9999))
+    constant = nearest + 0.49 * 2.0 ** -24
+    assert float(np.float32(constant)) == nearest
+    distance = np.arange(steps)
+    expected = constant ** distance.astype(np.float64)
+    bound = expected * (2 * U * np.ceil(distance / 8) + 40 * U)
+    if steps > 10000:
+        assert np.any(np.abs(nearest ** distance.astype(np.float64) - expected) > bound)
+    cut = place(torch.zeros(steps, lanes, dtype=torch.bool, device="cuda"), layout) if flags else None
+    x = torch.zeros(steps, lanes, device="cuda")
+    x[0] = 1.0
+    leaf = place(x, layout).requires_grad_(True)
+    for reverse in (False, True):
+        states, final = learning().linear_recurrence(leaf if not reverse else leaf.flip(0), constant, reverse=reverse, reset=cut, return_final=True)
+        got = to64(states) if not reverse else to64(states)[::-1]
+        assert_within(got, np.broadcast_to(expected[:, None], got.shape), np.broadcast_to(bound[:, None], got.shape), ("forwards", layout, reverse))
+        for seed in (torch.zeros_like(states), None):
+            if seed is None:
+                grad, = torch.autograd.grad(final, leaf, torch.ones_like(final))
+            else:
+                seed[0 if reverse else -1] = 1.0
+                grad, = torch.autograd.grad(states, leaf, seed, retain_graph=True)
+            assert_within(to64(grad)[::-1], np.broadcast_to(expected[:, None], got.shape), np.broadcast_to(bound[:, None], got.shape), ("backwards", layout, reverse))
