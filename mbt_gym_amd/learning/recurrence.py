@@ -185,7 +185,8 @@ def linear_recurrence(inputs: torch.Tensor, gate: Union[float, torch.Tensor], in
 
     A gate of exactly zero, like a reset, drops the state it meets whatever that holds: infinities and NaN do not pass it.  A sequence without
     steps has no states, and its final state is the initial one.  Gradients are those of the stored inputs and gates: the
-    states that they need are recomputed from them, in float32 whatever the states are stored in.  Second derivatives are refused."""
+    states that they need are recomputed from them, in float32 whatever the states are stored in.  Second and
+    forward-mode derivatives are refused."""
     require(inputs, "inputs", dtypes=DTYPES)
     if inputs.dim() == 0:
         raise ValueError("inputs is a scalar: it has no time axis")
