@@ -9,7 +9,7 @@ from typing import Sequence, Union
 import torch
 
 from mbt_gym_amd import _native
-from mbt_gym_amd.learning._tensors import DTYPES, current_stream, require
+from mbt_gym_amd.learning._tensors import DTYPES, current_stream, refuse_recording, require
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # of the published method: steep at zero, and [0.7, 1.2] is mapped near itself
 
@@ -25,6 +25,7 @@ def orthogonalise(updates: Union[torch.Tensor, Sequence[torch.Tensor]], *, steps
 
     A matrix of zeros stays zero; a NaN or an infinity anywhere in a matrix makes that matrix NaN.  Not differentiable.  A list costs one launch for all its
     matrices up to 64 x 64, seven for those with one side longer and seventeen for the rest, however many there are (per sixteen shapes)."""
+    refuse_recording("orthogonalise")
     single = isinstance(updates, torch.Tensor)
     given = [updates] if single else list(updates)
     if not given:

@@ -7,7 +7,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from mbt_gym_amd import _native
-from mbt_gym_amd.learning._tensors import DTYPES, batch_groups, current_stream, require
+from mbt_gym_amd.learning._tensors import DTYPES, batch_groups, current_stream, refuse_recording, require
 
 
 class _Plan:
@@ -148,6 +148,7 @@ def policy_gradient_loss(mean: torch.Tensor, actions: torch.Tensor, weights: tor
     entropy_weight  of the entropy bonus H(std) = log std + log(2 pi e) / 2, per component
 
     The gradients are computed with the loss, in one pass over the recording; backward() only has more to do when the loss was scaled on the way."""
+    refuse_recording("policy_gradient_loss", by_autograd=True)
     require(mean, "mean", dtypes=DTYPES)
     if mean.dim() == 0 or not 1 <= mean.shape[-1] <= 8:
         raise ValueError(f"mean has the shape {tuple(mean.shape)}: the last axis holds 1 to 8 action components")

@@ -9,7 +9,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from mbt_gym_amd import _native
-from mbt_gym_amd.learning._tensors import DTYPES, batch_groups, current_stream, dense_strides, require
+from mbt_gym_amd.learning._tensors import DTYPES, batch_groups, current_stream, dense_strides, refuse_recording, require
 
 
 class _Plan:
@@ -187,6 +187,7 @@ def linear_recurrence(inputs: torch.Tensor, gate: Union[float, torch.Tensor], in
     steps has no states, and its final state is the initial one.  Gradients are those of the stored inputs and gates: the
     states that they need are recomputed from them, in float32 whatever the states are stored in.  Second and
     forward-mode derivatives are refused."""
+    refuse_recording("linear_recurrence", by_autograd=True)
     require(inputs, "inputs", dtypes=DTYPES)
     if inputs.dim() == 0:
         raise ValueError("inputs is a scalar: it has no time axis")
@@ -215,7 +216,10 @@ def linear_recurrence(inputs: torch.Tensor, gate: Union[float, torch.Tensor], in
         return (states, final) if return_final else states
     tracked = torch.is_grad_enabled() and (inputs.requires_grad or (gate is not None and gate.requires_grad) or (initial is not None and initial.requires_grad))
     settings = (axis, form, constant, 1 if reverse else 0)
-    states, final = _LinearRecurrence.apply(inputs, gate, initial, reset, settings) if tracked else _forward(inputs, gate, initial, reset, settings)[:2]
+    if tracked or torch._C._get_tracing_state() is not None:
+        states, final = _LinearRecurrence.apply(inputs, gate, initial, reset, settings)
+    else:
+        states, final = _forward(inputs, gate, initial, reset, settings)[:2]
     return (states, final) if return_final else states
 
 
@@ -226,6 +230,7 @@ def linear_recurrence_step(state: torch.Tensor, inputs: torch.Tensor, gate: torc
     state      float32, the inputs' shape; contiguous
     new_state  where the float32 state goes: None = a new tensor; `state` itself updates it in place
     Not differentiable: an actor is trained on whole sequences."""
+    refuse_recording("linear_recurrence_step")
     require(inputs, "inputs", dtypes=DTYPES)
     shape, dtype, device = inputs.shape, inputs.dtype, inputs.device
     require(state, "state", device, (torch.float32,), shape)

@@ -1,4 +1,4 @@
-"""Forward-mode derivatives: refused, since a tangent would be passed by in silence."""
+"""Forward-mode derivatives and tracers, which see the tensors of a kernel call and not the call: refused where they would be passed by in silence."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -30,6 +30,53 @@ def test_tangents_are_refused():
     tangents_are_refused("cpu")
 
 
+def recorders_are_refused(device):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = torch.rand(5, 3, device=device)
+    for name in calls(x):
+        with pytest.raises(RuntimeError, match="cannot record"):
+            make_fx(lambda a: calls(a)[name]())(x)
+    for name in ("step", "state", "orthogonalise"):
+        for grad in (False, True):
+            with pytest.raises(RuntimeError, match="cannot record"), torch.set_grad_enabled(grad):
+                torch.jit.trace(lambda a: calls(a)[name](), (x,), check_trace=False)
+
+
+def test_tracers_that_would_record_nothing_are_refused():
+    recorders_are_refused("cpu")
+
+
 @pytest.mark.gpu
 def test_tangents_are_refused_on_the_device():
     tangents_are_refused("cuda")
+
+
+@pytest.mark.gpu
+def test_tracers_are_refused_on_the_device():
+    recorders_are_refused("cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_traced_sequence_answers_for_its_own_inputs(grad):
+    """torch.jit.trace records the recurrence and the loss as one operation each, with gradients enabled or not"""
+    from mbt_gym_amd import learning
+
+    def actor(obs, gate, reset, actions, weights):
+        h, final = learning.linear_recurrence(obs, gate, obs[0], reset=reset, gate_is_logit=True, return_final=True)
+        to_go = learning.rewards_to_go(weights, 0.9, dim=0)
+        return h, final, to_go, learning.policy_gradient_loss(h, actions, to_go, 0.3)
+
+    def inputs():
+        return (*(torch.randn(30, 20, 4, device="cuda") for _ in range(2)), torch.rand(30, 20, 4, device="cuda") < 0.1, torch.randn(30, 20, 4, device="cuda"),
+                torch.randn(30, 20, device="cuda"))
+
+    with torch.set_grad_enabled(grad):
+        traced = torch.jit.trace(actor, inputs(), check_trace=False)
+        for _ in range(3):
+            given = inputs()
+            used = [torch.full((30, 20, 4), 7.0, device="cuda") for _ in range(20)]  # (memory that a result which nobody wrote could lie in)
+            del used
+            for got, expected in zip(traced(*given), actor(*given)):
+                assert torch.equal(got, expected)
