@@ -771,8 +771,12 @@ typedef struct mbt_policy_loss {
 #define MBT_POLICY_LOSS_SUMS 10
 uint64_t mbt_policy_loss_workspace(const mbt_policy_loss* p);
 int mbt_policy_loss_forward(int device, const mbt_policy_loss* p, void* stream);
-/* Writes the gradients for *grad_loss.  With gradients_ready and *grad_loss == 1 - decided on the device - it touches nothing. */
+/* Writes the gradients for *grad_loss.  With gradients_ready and *grad_loss == 1 - decided on the device - it touches nothing: where the call is captured
+ * into a HIP graph, gradients_ready belongs to the graph that holds the forward call too, and only to it (mbt_stream_capture_id). */
 int mbt_policy_loss_backward(int device, const mbt_policy_loss* p, void* stream);
+
+/* Which capture into a HIP graph `stream` is part of: a number of its own for each, 0 = none. */
+uint64_t mbt_stream_capture_id(void* stream);
 
 /* Orthogonalised updates, for a learner that steps along them instead of along the gradient (the Muon optimiser): with X = G / (|G| + eps), |G| the
  * Frobenius norm, `steps` Newton-Schulz products X <- a X + (b X X^T + c (X X^T)^2) X (a matrix with more rows than columns is turned).

@@ -343,6 +343,7 @@ SIGNATURES = {
     "mbt_policy_loss_workspace": (C.c_uint64, [C.POINTER(MbtPolicyLoss)]),
     "mbt_policy_loss_forward": (C.c_int, [C.c_int, C.POINTER(MbtPolicyLoss), C.c_void_p]),
     "mbt_policy_loss_backward": (C.c_int, [C.c_int, C.POINTER(MbtPolicyLoss), C.c_void_p]),
+    "mbt_stream_capture_id": (C.c_uint64, [C.c_void_p]),
     "mbt_orthogonalise_workspace": (C.c_uint64, [C.c_uint32, C.POINTER(MbtMatrix)]),
     "mbt_orthogonalise": (C.c_int, [C.c_int, C.c_int, C.c_uint32, C.POINTER(MbtMatrix), C.c_int, C.POINTER(C.c_double), C.c_double, C.c_void_p,
                                     C.c_uint64, C.c_void_p]),

@@ -176,6 +176,17 @@ int mbt_policy_loss_forward(int device, const mbt_policy_loss* p, void* stream) 
   return launch_status("policy loss (sum)");
 }
 
+uint64_t mbt_stream_capture_id(void* stream) {
+  if (stream == nullptr) return 0;  // (the default stream cannot be captured)
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &id) != hipSuccess) {
+    (void)hipGetLastError();
+    return 0;
+  }
+  return status == hipStreamCaptureStatusActive ? id : 0;
+}
+
 int mbt_policy_loss_backward(int device, const mbt_policy_loss* p, void* stream) {
   using namespace mbt_learning;
   LossPlan plan;

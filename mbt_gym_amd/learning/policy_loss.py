@@ -101,10 +101,12 @@ class _PolicyLoss(torch.autograd.Function):
         p.entropy_weight, p.loss, p.sums = entropy_weight, loss.data_ptr(), sums.data_ptr()
         p.workspace, p.workspace_bytes = workspace.data_ptr(), plan.workspace
         ctx.gradients = _gradients(ctx, p, *operands[:2])
-        index = device.index
-        code = _native.load_library().mbt_policy_loss_forward(index, p, current_stream(index))
+        lib, index = _native.load_library(), device.index
+        stream = current_stream(index)
+        code = lib.mbt_policy_loss_forward(index, p, stream)
         if code < 0:
             _native.check(code)
+        ctx.capture = lib.mbt_stream_capture_id(stream)
         ctx.save_for_backward(*operands, sums)
         ctx.settings = number, entropy_weight
         return loss
@@ -115,9 +117,13 @@ class _PolicyLoss(torch.autograd.Function):
         *operands, sums = ctx.saved_tensors
         number, entropy_weight = ctx.settings
         _, p, operands = _operands(*operands, number)
-        # the arrays that the forward call filled are handed out once; a graph that is walked again gets new ones
+        lib, index = _native.load_library(), sums.device.index
+        stream = current_stream(index)
+        capture = lib.mbt_stream_capture_id(stream)
+        # The arrays that the forward call filled are handed out once; a graph that is walked again gets new ones.  So does a pass that is captured without the
+        # forward call: its replays come again and again, with other loss gradients and after what the program did to the arrays.
         gradients, ctx.gradients = ctx.gradients, None
-        if gradients is not None:
+        if gradients is not None and capture in (0, ctx.capture):
             grad_mean, grad_std = gradients
             p.gradients_ready = 1
             if grad_mean is not None:
@@ -128,8 +134,7 @@ class _PolicyLoss(torch.autograd.Function):
             gradients = _gradients(ctx, p, *operands[:2])
         grad_loss = grad_loss.contiguous()
         p.entropy_weight, p.sums, p.grad_loss = entropy_weight, sums.data_ptr(), grad_loss.data_ptr()
-        index = sums.device.index
-        code = _native.load_library().mbt_policy_loss_backward(index, p, current_stream(index))
+        code = lib.mbt_policy_loss_backward(index, p, stream)
         if code < 0:
             _native.check(code)
         return gradients + (None,) * 5
