@@ -142,6 +142,15 @@ class PolicyGradientAgent(Agent):
         std = None if deterministic else [self._std()] * self.action_size
         return _native.mlp_policy(layers, activation, action_std=std, clip=False)
 
+    @property
+    def _epoch_is_its_own(self) -> bool:
+        """The sampling, the rewards-to-go and the distribution are the ones of this class.  Where a subclass, or a program, has put its own in
+        their place, `train` asks those for them and takes the loss of what they answer."""
+        import torch
+
+        return (getattr(self._sample_on_device, "__func__", None) is _OWN_SAMPLE and self._calculate_future_rewards is _OWN_FUTURE_REWARDS
+                and self.noise_dist is torch.distributions.Normal)
+
     # ---- one epoch of data ----------------------------------------------------------------------------------------------------
     def _record_on_device(self):
         """One fused rollout launch: (observations (T, N, D), actions (T, N, A), rewards (T, N)), views of the padded recording on the device."""
@@ -162,17 +171,29 @@ class PolicyGradientAgent(Agent):
         """(rewards (N, 1, T) tensor, log-probabilities (N, A, T) tensor with gradients), from one fused rollout launch."""
         where = self._module_device()
         o, a, r = (t.to(where) for t in self._record_on_device())
-        log_prob = self.noise_dist(self.kernel_mean(o), self._std()).log_prob(a)  # of the actions the KERNEL sampled, around ITS mean: (T, N, A)
-        return r.t().unsqueeze(1), log_prob.permute(1, 2, 0)
+        return self._scored(self.kernel_mean(o), a, r)  # the actions the KERNEL sampled, around ITS mean
+
+    def _sample_sequence(self):
+        """The same of a recurrent actor, which quoted step by step and is scored on the whole recording."""
+        o, a, r = self._record_sequence()
+        return self._scored(self.policy_net(o), a, r)
+
+    def _scored(self, mean, actions, rewards):
+        log_prob = self.noise_dist(mean, self._std()).log_prob(actions)  # (T, N, A)
+        return rewards.t().unsqueeze(1), log_prob.permute(1, 2, 0)
+
+    def _record_sequence(self):
+        """One episode of the reference's loop: (observations (T, N, D), actions (T, N, A), rewards (T, N)) on the policy's device."""
+        observations, actions, rewards, where = *generate_trajectory(self.env, self), self._module_device()
+        return tuple(self._time_first(t, where) for t in (observations[:, :, :-1], actions, rewards[:, 0]))
 
     def _device_epoch(self):
         """(rewards, loss) of one epoch whose data never leaves the device: - mean of log N(a | mean, std) x reward-to-go (PG:58-59) as kernels"""
         from mbt_gym_amd.learning import policy_gradient_loss, rewards_to_go
 
         if self._is_recurrent:
-            observations, actions, rewards, where = *generate_trajectory(self.env, self), self._module_device()
-            o, a = (self._time_first(t, where) for t in (observations[:, :, :-1], actions))
-            r, mean = self._time_first(rewards[:, 0], where), self.policy_net(o)
+            o, a, r = self._record_sequence()
+            mean = self.policy_net(o)
         else:
             o, a, r = self._record_on_device()
             mean = self.kernel_mean(o)
@@ -191,11 +212,14 @@ class PolicyGradientAgent(Agent):
         learning_losses, learning_rewards = [], []
         self.proportion_completed = 0.0
         for epoch in range(num_epochs):
-            if self._is_recurrent or (self.has_device_policy and self._module_device() == torch.device("cuda", self.env.device)):
+            on_device = self._is_recurrent or (self.has_device_policy and self._module_device() == torch.device("cuda", self.env.device))
+            if on_device and self._epoch_is_its_own:
                 rewards, loss = self._device_epoch()
                 learning_rewards.append(float(rewards.mean()))
             else:
-                if self.has_device_policy:
+                if self._is_recurrent:
+                    rewards, log_probs = self._sample_sequence()
+                elif self.has_device_policy:
                     rewards, log_probs = self._sample_on_device()
                 else:
                     _, _, rewards, log_probs = generate_trajectory(self.env, self, include_log_probs=True)
@@ -229,3 +253,6 @@ class PolicyGradientAgent(Agent):
             following = rewards[..., k] + discount * following
             out[..., k] = following
         return out
+
+
+_OWN_SAMPLE, _OWN_FUTURE_REWARDS = PolicyGradientAgent._sample_on_device, PolicyGradientAgent._calculate_future_rewards
