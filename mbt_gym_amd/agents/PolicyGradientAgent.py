@@ -225,7 +225,7 @@ class PolicyGradientAgent(Agent):
                     _, _, rewards, log_probs = generate_trajectory(self.env, self, include_log_probs=True)
                     rewards = torch.as_tensor(rewards, device=log_probs.device)
                 learning_rewards.append(float(rewards.mean()))
-                future_rewards = self._calculate_future_rewards(rewards, self.discount)
+                future_rewards = self._calculate_future_rewards(rewards, *([] if self.discount == 1.0 else [self.discount]))  # (PG:69 takes the rewards alone)
                 loss = -torch.mean(log_probs * future_rewards)  # PG:58-59
             self.optimizer.zero_grad()
             loss.backward()

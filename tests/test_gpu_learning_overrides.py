@@ -69,3 +69,20 @@ def test_sampling_and_distribution_of_a_program_are_used():
         losses, _ = agent.train(num_epochs=1, reporting_freq=1000)
         assert calls[-1] == (10, 64, 2) and np.isfinite(losses).all()
     env.close()
+
+
+@pytest.mark.parametrize("policy", [lambda: actor().cuda(), deep, recurrent], ids=["device", "loop", "recurrent"])
+def test_rewards_to_go_with_the_reference_signature(policy):
+    """PolicyGradientAgent.py:69 takes the rewards alone: an override of it is called with them alone unless there is a discount to pass"""
+
+    class Agent(PolicyGradientAgent):
+        @staticmethod
+        def _calculate_future_rewards(rewards):
+            return torch.zeros_like(rewards)
+
+    env = make_env(64, horizon=10)
+    losses, _ = Agent(policy(), action_std=0.05, env=env).train(num_epochs=2, reporting_freq=1000)
+    assert losses == [0.0, 0.0]
+    with pytest.raises(TypeError):
+        Agent(policy(), action_std=0.05, env=env, discount=0.5).train(num_epochs=1, reporting_freq=1000)
+    env.close()
