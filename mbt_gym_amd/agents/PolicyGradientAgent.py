@@ -189,6 +189,8 @@ class PolicyGradientAgent(Agent):
 
     def _device_epoch(self):
         """(rewards, loss) of one epoch whose data never leaves the device: - mean of log N(a | mean, std) x reward-to-go (PG:58-59) as kernels"""
+        import torch
+
         from mbt_gym_amd.learning import policy_gradient_loss, rewards_to_go
 
         if self._is_recurrent:
@@ -197,7 +199,10 @@ class PolicyGradientAgent(Agent):
         else:
             o, a, r = self._record_on_device()
             mean = self.kernel_mean(o)
-        return r, policy_gradient_loss(mean, a, rewards_to_go(r, self.discount, dim=0), self._std())
+        loss = policy_gradient_loss(mean, a, rewards_to_go(r, self.discount, dim=0), self._std())
+        if bool(torch.isnan(loss)):  # (as any NaN in the means and actions makes it: the distribution refuses those, and says what it was given)
+            self.noise_dist(mean, self._std()).log_prob(a)
+        return r, loss
 
     @staticmethod
     def _time_first(array, where):

@@ -86,3 +86,17 @@ def test_rewards_to_go_with_the_reference_signature(policy):
     with pytest.raises(TypeError):
         Agent(policy(), action_std=0.05, env=env, discount=0.5).train(num_epochs=1, reporting_freq=1000)
     env.close()
+
+
+@pytest.mark.parametrize("policy", [lambda: actor().cuda(), recurrent], ids=["device", "recurrent"])
+def test_an_actor_that_answers_nan_is_refused_before_it_learns(policy):
+    """torch.distributions refuses a mean that is not a number, and `train` did not get as far as the optimiser"""
+    env = make_env(64, horizon=10)
+    net = policy()
+    with torch.no_grad():
+        list(net.parameters())[-1][0] = float("nan")
+    before = [p.detach().clone() for p in net.parameters()]
+    with pytest.raises(ValueError, match="constraint|support"):
+        PolicyGradientAgent(net, action_std=0.05, env=env).train(num_epochs=2, reporting_freq=1000)
+    assert all(torch.equal(torch.nan_to_num(p), torch.nan_to_num(b)) for p, b in zip(net.parameters(), before))
+    env.close()
