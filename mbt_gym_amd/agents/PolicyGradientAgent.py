@@ -244,10 +244,13 @@ class PolicyGradientAgent(Agent):
 
     @staticmethod
     def _calculate_future_rewards(rewards, discount: float = 1.0):
-        """Rewards-to-go along the last axis (PG:69-73): a kernel where the rewards live on the device, torch where they live on the host."""
+        """Rewards-to-go along the last axis (PG:69-73): a kernel where the rewards live on the device, torch where they live on the host or are
+        something to differentiate (any number of times, either way) or to transform."""
         import torch
 
-        if rewards.is_cuda and rewards.dtype in (torch.float32, torch.bfloat16, torch.float16):
+        from mbt_gym_amd.learning._tensors import DTYPES, transformed
+
+        if rewards.is_cuda and rewards.dtype in DTYPES and not (torch.is_grad_enabled() and rewards.requires_grad) and not transformed():
             from mbt_gym_amd.learning import rewards_to_go
 
             return rewards_to_go(rewards, discount)

@@ -17,6 +17,12 @@ def refuse_recording(what, by_autograd=False):
         raise RuntimeError(f"{what} is a kernel call that the tracer that is active cannot record")
 
 
+def transformed():
+    """Is torch at work on something that a kernel call does not take part in: a forward-mode derivative, a functorch transform, a tracer?"""
+    return (forward_ad._current_level >= 0 or torch._C._functorch.maybe_current_level() is not None or torch._C._get_tracing_state() is not None
+            or torch._C._get_dispatch_mode(_PROXY) is not None)
+
+
 def require(tensor, name, device=None, dtypes=None, shape=None):
     """A strided CUDA tensor (of this device, one of these dtypes, this shape), or a TypeError / ValueError that says what was given."""
     if not isinstance(tensor, torch.Tensor):

@@ -100,3 +100,24 @@ def test_an_actor_that_answers_nan_is_refused_before_it_learns(policy):
         PolicyGradientAgent(net, action_std=0.05, env=env).train(num_epochs=2, reporting_freq=1000)
     assert all(torch.equal(torch.nan_to_num(p), torch.nan_to_num(b)) for p, b in zip(net.parameters(), before))
     env.close()
+
+
+def test_rewards_to_go_of_rewards_that_are_differentiated():
+    """twice, in forward mode, over a batch and in a trace, as the torch operations that it was before"""
+    import torch.autograd.forward_ad as forward_ad
+
+    to_go = PolicyGradientAgent._calculate_future_rewards
+    r, ones = torch.randn(6, 1, 9, device="cuda"), torch.arange(9.0, 0.0, -1.0, device="cuda").expand(6, 1, 9)
+    leaf = r.clone().requires_grad_(True)
+    grad, = torch.autograd.grad((to_go(leaf) ** 2).sum() / 2, leaf, create_graph=True)
+    second, = torch.autograd.grad(grad.sum(), leaf)  # (J^T J 1, with J 1 the steps to go)
+    assert torch.allclose(second, torch.cumsum(ones, dim=-1))
+    with forward_ad.dual_level():
+        assert torch.equal(forward_ad.unpack_dual(to_go(forward_ad.make_dual(r, torch.ones_like(r)))).tangent, ones)
+    value, tangent = torch.func.jvp(to_go, (r,), (torch.ones_like(r),))
+    assert torch.equal(tangent, ones) and torch.allclose(value, to_go(r), atol=1e-5)
+    assert torch.allclose(torch.func.vmap(to_go)(r), to_go(r), atol=1e-5)
+    traced = torch.jit.trace(to_go, (r,), check_trace=False)
+    assert torch.allclose(traced(r + 1), to_go(r + 1), atol=1e-4)
+    with torch.no_grad():
+        assert torch.allclose(to_go(leaf), to_go(r))
