@@ -211,8 +211,10 @@ def linear_recurrence(inputs: torch.Tensor, gate: Union[float, torch.Tensor], in
     if reset is not None:
         require(reset, "reset", inputs.device, (torch.bool, torch.uint8), inputs.shape)
     if inputs.numel() == 0:
-        states = inputs.clone()
-        final = torch.zeros(batch, dtype=torch.float32, device=inputs.device) if initial is None else initial.clone()
+        # (nothing is added to the initial state, but the results depend on every operand, whose gradients are zeros)
+        joined = inputs if gate is None else inputs + gate
+        first = torch.zeros(batch, dtype=torch.float32, device=inputs.device) if initial is None else initial
+        states, final = joined + first.unsqueeze(axis).to(inputs.dtype), first + joined.sum(dim=axis, dtype=torch.float32)
         return (states, final) if return_final else states
     tracked = torch.is_grad_enabled() and (inputs.requires_grad or (gate is not None and gate.requires_grad) or (initial is not None and initial.requires_grad))
     settings = (axis, form, constant, 1 if reverse else 0)

@@ -217,3 +217,19 @@ def test_a_long_walk_decays_with_the_double_constant(steps, lanes, flags, layout
                 seed[0 if reverse else -1] = 1.0
                 grad, = torch.autograd.grad(states, leaf, seed, retain_graph=True)
             assert_within(to64(grad)[::-1], np.broadcast_to(expected[:, None], got.shape), np.broadcast_to(bound[:, None], got.shape), ("backwards", layout, reverse))
+
+
+@pytest.mark.parametrize("shape", [(0, 5), (7, 0), (0, 0), (3, 0, 2)], ids=str)
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_sequence_without_elements_has_gradients(shape, dtype):
+    """of zeros, for every operand of either result; the final state's goes to the initial one"""
+    x, gate = (torch.rand(shape, device="cuda").to(DTYPES[dtype]).requires_grad_(True) for _ in range(2))
+    h0 = torch.rand(shape[1:], device="cuda", requires_grad=True)
+    for g in (gate, 0.5):
+        states, final = learning().linear_recurrence(x, g, h0, return_final=True)
+        assert states.shape == x.shape and states.dtype == x.dtype and final.dtype == torch.float32 and torch.equal(final, h0)
+        leaves = [x, h0] + ([gate] if g is gate else [])
+        for result in (states, final):
+            grads = torch.autograd.grad(result.sum(), leaves, retain_graph=True)
+            assert [t.shape for t in grads] == [t.shape for t in leaves]
+            assert torch.equal(grads[1], torch.ones_like(h0) if result is final else torch.zeros_like(h0))
