@@ -53,7 +53,8 @@ int make_plan(const mbt_recurrence* r, bool backward, Plan& plan) {
     return mbt_set_error(MBT_ERR_INVALID, "inputs and states are needed");
   if (backward && r->grad_states.data == nullptr) return mbt_set_error(MBT_ERR_INVALID, "the backward pass needs grad_states");
   if (!gated && r->grad_gate.data != nullptr) return mbt_set_error(MBT_ERR_INVALID, "a constant gate has no gradient array");
-  if (!gated && !(r->constant - r->constant == 0.0)) return mbt_set_error(MBT_ERR_INVALID, "the constant gate is not finite");
+  if (!gated && !std::isfinite(r->constant)) return mbt_set_error(MBT_ERR_INVALID, "the constant gate is not finite");
+  if (!gated && !std::isfinite(static_cast<float>(r->constant))) return mbt_set_error(MBT_ERR_INVALID, "the constant gate %g is not finite in float32", r->constant);
 
   const int64_t steps = static_cast<int64_t>(r->steps);
   const size_t size = dtype_size(r->dtype);

@@ -2,7 +2,6 @@
 
 The rewards-to-go of the reference's learner (mbt_gym/agents/PolicyGradientAgent.py:69-73) are the recurrence walked backwards with a constant
 gate; the state of a recurrent actor is the one with learnt gates.  Kernels, splits and what bounds them: csrc/recurrence.hpp."""
-import math
 from typing import Optional, Union
 
 import torch
@@ -59,6 +58,7 @@ class _Plan:
             _native.check(code)
 
 
+_LARGEST = torch.finfo(torch.float32).max
 _plans = {}
 
 
@@ -203,8 +203,8 @@ def linear_recurrence(inputs: torch.Tensor, gate: Union[float, torch.Tensor], in
         if gate_is_logit:
             raise TypeError("gate_is_logit needs a gate tensor")
         form, constant, gate = _native.GATE_CONSTANT, float(gate), None
-        if not math.isfinite(constant):
-            raise ValueError(f"gate = {constant}: a constant gate has to be finite")
+        if not abs(constant) <= _LARGEST:
+            raise ValueError(f"gate = {constant}: a constant gate has to be finite, in float32")
     if initial is not None:
         require(initial, "initial", inputs.device, (torch.float32, inputs.dtype), batch)
         initial = initial.to(torch.float32).contiguous()

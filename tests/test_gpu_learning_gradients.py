@@ -233,3 +233,11 @@ def test_a_sequence_without_elements_has_gradients(shape, dtype):
             grads = torch.autograd.grad(result.sum(), leaves, retain_graph=True)
             assert [t.shape for t in grads] == [t.shape for t in leaves]
             assert torch.equal(grads[1], torch.ones_like(h0) if result is final else torch.zeros_like(h0))
+
+
+def test_constants_that_float32_does_not_hold_are_refused():
+    x = torch.ones(5, 2, device="cuda")
+    for constant in (3.5e38, -1e39, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="finite"):
+            learning().linear_recurrence(x, constant)
+    assert torch.equal(learning().linear_recurrence(x[:1], 3.4e38), x[:1])

@@ -43,3 +43,15 @@ def test_malformed_edges_are_refused(lib):
     bare = recurrence_struct(steps=1000, dtype=_native.BFLOAT16)
     bare.states.data = None
     refused(lib, lib.mbt_recurrence_backward(0, C.byref(bare), None), "states or edges")
+
+
+def test_constants_that_float32_does_not_hold_are_refused(lib):
+    """3.5e38 is a finite double and an infinite float32; the largest float32 is taken as far as the check of the device"""
+    for constant in (3.5e38, -1e39, 1e300):
+        r = recurrence_struct(form=_native.GATE_CONSTANT, constant=constant)
+        r.grad_gate.data = None
+        for call in (lib.mbt_recurrence_forward, lib.mbt_recurrence_backward):
+            refused(lib, call(0, C.byref(r), None), "not finite in float32")
+    r.constant = -3.4028234663852886e38
+    assert lib.mbt_recurrence_workspace(C.byref(r), 0) == 0 and lib.mbt_recurrence_forward(-1, C.byref(r), None) < 0
+    assert b"float32" not in lib.mbt_last_error()
