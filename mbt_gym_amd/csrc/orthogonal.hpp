@@ -88,6 +88,12 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
   return v;
 }
 
+// 1 / (|G| + eps) from the sum of squares; a matrix of zeros stays zero without an eps too
+__device__ __forceinline__ double inverse_norm(double sum, double eps) {
+  const double norm = sqrt(sum) + eps;
+  return norm == 0.0 ? 0.0 : 1.0 / norm;
+}
+
 __device__ __forceinline__ int find_group(const OrthogonaliseParams& P, int64_t block, int64_t& at) {
   int g = 0;
   while (g + 1 < P.groups && block >= P.group[g + 1].first) ++g;
@@ -195,7 +201,7 @@ __global__ __launch_bounds__(1024) void orthogonalise_small(const OrthogonaliseP
     sum += static_cast<double>(v[k]) * static_cast<double>(v[k]);
   }
   sum = block_sum(sum, sums);
-  const double inverse = 1.0 / (sqrt(sum) + P.eps);
+  const double inverse = inverse_norm(sum, P.eps);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int at = threadIdx.x + 1024 * k, i = at >> 6, j = at & 63;
@@ -254,7 +260,7 @@ __global__ __launch_bounds__(1024) void orthogonalise_flat(const OrthogonalisePa
   double inverse = 0.0;
   if (launch == 0) {
     const double* partials = P.partials + (which + matrices_before(P, group)) * kNormBlocks;
-    inverse = 1.0 / (sqrt(block_sum(threadIdx.x < M.norm_blocks ? partials[threadIdx.x] : 0.0, sums)) + P.eps);
+    inverse = inverse_norm(block_sum(threadIdx.x < M.norm_blocks ? partials[threadIdx.x] : 0.0, sums), P.eps);
   } else {  // A: everyone's shares, in their order
     float4v a = {0.f, 0.f, 0.f, 0.f};
     const int i = threadIdx.x >> 4, j = 4 * (threadIdx.x & 15);
@@ -390,7 +396,7 @@ __global__ __launch_bounds__(256) void orthogonalise_split(const OrthogonalisePa
     v[k] = i0 + i < M.m && j0 + j < M.n ? static_cast<float>(in[(i0 + i) * M.in_row + (j0 + j) * M.in_column]) : 0.0f;
   }
   const double* partials = P.partials + (which + matrices_before(P, group)) * kNormBlocks;
-  const float inverse = static_cast<float>(1.0 / (sqrt(block_sum(threadIdx.x < M.norm_blocks ? partials[threadIdx.x] : 0.0, lds)) + P.eps));
+  const float inverse = static_cast<float>(inverse_norm(block_sum(threadIdx.x < M.norm_blocks ? partials[threadIdx.x] : 0.0, lds), P.eps));
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
     const int e = threadIdx.x + 256 * k, i = along_n ? e >> 6 : e & 63, j = along_n ? e & 63 : e >> 6;
