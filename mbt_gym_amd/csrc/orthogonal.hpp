@@ -396,11 +396,12 @@ __global__ __launch_bounds__(256) void orthogonalise_split(const OrthogonalisePa
     v[k] = i0 + i < M.m && j0 + j < M.n ? static_cast<float>(in[(i0 + i) * M.in_row + (j0 + j) * M.in_column]) : 0.0f;
   }
   const double* partials = P.partials + (which + matrices_before(P, group)) * kNormBlocks;
-  const float inverse = static_cast<float>(inverse_norm(block_sum(threadIdx.x < M.norm_blocks ? partials[threadIdx.x] : 0.0, lds), P.eps));
+  // (in 64 bits: the inverse of a norm beyond 2^126 is no normal float32 number, that of one below 2^-128 no finite one)
+  const double inverse = inverse_norm(block_sum(threadIdx.x < M.norm_blocks ? partials[threadIdx.x] : 0.0, lds), P.eps);
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
     const int e = threadIdx.x + 256 * k, i = along_n ? e >> 6 : e & 63, j = along_n ? e & 63 : e >> 6;
-    tile[i][j] = v[k] * inverse * kScaleX;
+    tile[i][j] = static_cast<float>(v[k] * inverse) * kScaleX;
   }
   __syncthreads();
   const Planes p = planes_of(P, M, which);

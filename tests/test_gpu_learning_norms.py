@@ -21,3 +21,15 @@ def test_zeros_stay_zero_without_an_eps(shape, dtype):
     broken = some.clone()
     broken[-1, -1] = float("nan")
     assert torch.isnan(orthogonalise(broken, eps=0.0)).all()
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_a_power_of_two_in_front_of_a_matrix_changes_no_bit(shape):
+    """without an eps the norm takes it out again, exactly: every operation up to the scaled matrix commutes with it as long as the entries stay normal
+    numbers, and the norm of 2048 x 1800 entries around 2^123 is beyond float32's range"""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    g = torch.randint(-8, 9, shape, generator=gen, device="cuda").float()
+    g[0, 0] = 8.0
+    expected = orthogonalise(g, eps=0.0)
+    for exponent in (-126, -60, 60, 120, 124):
+        assert torch.equal(orthogonalise(g * 2.0 ** exponent, eps=0.0), expected), exponent
