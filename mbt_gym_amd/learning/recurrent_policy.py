@@ -10,7 +10,8 @@ class RecurrentPolicy(torch.nn.Module):
 
     forward(observations)  (T, N, D) -> (T, N, A), differentiable: the recurrence runs along T (mbt_gym_amd.learning.linear_recurrence)
     step(observation)      (N, D) -> (N, A) for the next step of the episode; begin_episode() puts the state back to zero, and lanes whose episode
-                           starts anew in between are named by `reset`
+                           starts anew in between are named by `reset`.  A step may be captured into a HIP graph, after one of the same batch that
+                           was not: the graph's replays and begin_episode() then work on the state that the capture found
     `PolicyGradientAgent` trains it as it is.  Parameters and tensors live on the device."""
 
     def __init__(self, observation_size: int, action_size: int, hidden_size: int = 64, memory: float = 2.0):
@@ -21,6 +22,7 @@ class RecurrentPolicy(torch.nn.Module):
         with torch.no_grad():
             self.inputs.bias[hidden_size:] += memory  # (the forget gates start open: sigmoid(2) = 0.88)
         self.state = None
+        self._captured = []  # states that HIP graphs go on with: they keep their place, and an episode that begins finds zeros in them
 
     def forward(self, observations: torch.Tensor, reset: torch.Tensor = None) -> torch.Tensor:
         x, gate = self.inputs(observations).split(self.hidden_size, dim=-1)
@@ -29,13 +31,36 @@ class RecurrentPolicy(torch.nn.Module):
         return self.output(torch.tanh(linear_recurrence(x, gate, dim=0, reset=reset, gate_is_logit=True)))
 
     def begin_episode(self):
+        if self.state is not None and torch.cuda.is_current_stream_capturing():
+            self._keep()
+        for state in self._captured:
+            self._clear(state)
         self.state = None
+
+    def _keep(self):
+        if not any(state is self.state for state in self._captured):
+            self._captured.append(self.state)
+
+    @staticmethod
+    def _clear(state):
+        with torch.inference_mode(state.is_inference()):
+            state.zero_()
 
     @torch.no_grad()
     def step(self, observation: torch.Tensor, reset: torch.Tensor = None) -> torch.Tensor:
         x, gate = self.inputs(observation).split(self.hidden_size, dim=-1)
+        capturing = torch.cuda.is_current_stream_capturing()
         if self.state is None or self.state.shape != x.shape or self.state.device != x.device:
-            self.state = torch.zeros(x.shape, dtype=torch.float32, device=x.device)
+            kept = next((state for state in self._captured if state.shape == x.shape and state.device == x.device), None)
+            if kept is None and capturing:
+                raise RuntimeError("the state of this batch does not exist yet, and one that is made in a graph starts from zero on every replay: take a step before")
+            if kept is None:
+                kept = torch.zeros(x.shape, dtype=torch.float32, device=x.device)
+            elif self.state is not None:  # (another batch was in between)
+                self._clear(kept)
+            self.state = kept
+        if capturing:
+            self._keep()
         if reset is not None:
             reset = reset.unsqueeze(-1).expand(x.shape)
         hidden, _ = linear_recurrence_step(self.state, x, gate, reset=reset, gate_is_logit=True, new_state=self.state)

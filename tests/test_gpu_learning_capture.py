@@ -70,3 +70,87 @@ def test_a_whole_pass_captured_twice_has_its_gradients_on_every_replay():
         expected, = torch.autograd.grad(learning.policy_gradient_loss(mean, actions, weights, 0.5), mean)
         assert torch.equal(together, expected) and torch.equal(apart, expected)
         together.mul_(0.25)
+
+
+def recurrent():
+    from mbt_gym_amd.learning import RecurrentPolicy
+
+    torch.manual_seed(3)
+    return RecurrentPolicy(4, 2, hidden_size=16).cuda()
+
+
+def captured(policy, obs, calls):
+    """(graph, its answers) of `calls`, after one step that is not captured"""
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        policy.step(obs)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            answers = calls()
+    torch.cuda.synchronize()
+    return graph, answers
+
+
+def test_a_captured_step_starts_its_episodes_with_the_policy():
+    policy, eager = recurrent(), recurrent()
+    obs, other = torch.empty(50, 4, device="cuda"), torch.randn(7, 4, device="cuda")
+    obs.copy_(torch.randn(50, 4, device="cuda"))
+    graph, answer = captured(policy, obs, lambda: policy.step(obs))
+    for episode in range(4):
+        policy.begin_episode()
+        eager.begin_episode()
+        used = [torch.full((50, 16), 9.0, device="cuda") for _ in range(20)]  # (memory that a state which was let go could lie in)
+        for t in range(6):
+            obs.copy_(torch.randn(50, 4, device="cuda"))
+            torch.cuda.synchronize()
+            if episode == 3 and t % 2:  # a step that is not a replay goes on from where the replays are
+                answer.copy_(policy.step(obs))
+            else:
+                graph.replay()
+            torch.cuda.synchronize()
+            assert torch.allclose(answer, eager.step(obs), rtol=0, atol=1e-6), (episode, t)
+        assert all(bool((u == 9.0).all()) for u in used)
+        if episode == 1:  # another batch in between: back on the first one, an episode begins
+            policy.step(other)
+            assert policy.state.shape == (7, 16)
+
+
+def test_a_captured_episode_starts_from_zero_on_every_replay():
+    policy, eager = recurrent(), recurrent()
+    obs = torch.randn(5, 50, 4, device="cuda")
+
+    def episode():
+        policy.begin_episode()
+        return torch.stack([policy.step(o) for o in obs])
+
+    graph, answers = captured(policy, obs[0], episode)
+    for _ in range(3):
+        obs.copy_(torch.randn(5, 50, 4, device="cuda"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        eager.begin_episode()
+        assert torch.allclose(answers, torch.stack([eager.step(o) for o in obs]), rtol=0, atol=1e-6)
+
+
+def test_a_first_step_is_not_captured():
+    policy, obs = recurrent(), torch.randn(50, 4, device="cuda")
+    policy(obs[None])  # (the library of the layers is ready)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        policy.inputs(obs)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="take a step before"):
+            with torch.cuda.graph(graph, stream=stream):
+                policy.step(obs)
+    torch.cuda.synchronize()
+    assert policy.state is None and policy.step(obs).shape == (50, 2)
+    with torch.inference_mode():
+        policy.begin_episode()
+        policy.step(obs)
+    policy.step(obs)
+    policy.begin_episode()
+    assert policy.state is None
