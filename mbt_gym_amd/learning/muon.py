@@ -118,6 +118,8 @@ class Muon(torch.optim.Optimizer):
         for p in params:
             if p.grad.is_sparse:
                 raise ValueError("Muon does not take sparse gradients")
+            if p.is_complex():
+                raise ValueError(f"Muon does not take parameters of {p.dtype}")
             if "momentum" not in self.state[p]:
                 self.state[p]["momentum"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
         grads, moving = [p.grad.float() for p in params], [self.state[p]["momentum"] for p in params]
