@@ -241,3 +241,27 @@ def test_constants_that_float32_does_not_hold_are_refused():
         with pytest.raises(ValueError, match="finite"):
             learning().linear_recurrence(x, constant)
     assert torch.equal(learning().linear_recurrence(x[:1], 3.4e38), x[:1])
+
+
+@pytest.mark.parametrize("lanes, steps", [(1, 1), (1000, 200), (513, 50), (3, 4000), (70000, 5)])
+def test_padded_lanes_of_a_recording_are_neither_read_nor_written(lanes, steps):
+    """rewards, gates, resets and upstream gradients as views of recordings whose lanes behind the last one hold NaN: bit for bit what they were, and the
+    results those of the lanes alone"""
+    padded = -(-lanes // 512) * 512
+    recorded = [torch.randn(steps, padded, device="cuda") for _ in range(3)]
+    recorded[1] = torch.sigmoid(recorded[1])
+    for t in recorded:
+        t[:, lanes:] = float("nan")
+    flags = torch.rand(steps, padded, device="cuda") < 0.05
+    before = [t.view(torch.int32).clone() for t in recorded] + [flags.clone()]
+    views, packed = [t[:, :lanes] for t in recorded], [t[:, :lanes].contiguous() for t in recorded]
+    results = []
+    for x, gate, up in (views, packed):
+        x, gate = x.detach().requires_grad_(True), gate.detach().requires_grad_(True)
+        to_go = learning().rewards_to_go(x.t().unsqueeze(1), 0.9, done=flags[:, :lanes].t().unsqueeze(1))
+        states = learning().linear_recurrence(x, gate, reset=flags[:, :lanes], reverse=True)
+        results.append([to_go, states] + list(torch.autograd.grad(states, [x, gate], up, retain_graph=True)) + list(torch.autograd.grad(to_go, x, up.t().unsqueeze(1))))
+    for one, other in zip(*results):
+        assert not torch.isnan(one).any() and torch.equal(one, other)
+    for t, b in zip(recorded + [flags], before):
+        assert torch.equal(t if t.dtype is torch.bool else t.view(torch.int32), b)
