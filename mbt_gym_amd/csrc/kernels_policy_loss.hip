@@ -97,7 +97,9 @@ int make_plan(const mbt_policy_loss* p, LossPlan& plan) {
   if (p->std_kind != MBT_STD_NUMBER && p->std_array.data == nullptr) return mbt_set_error(MBT_ERR_INVALID, "this std_kind needs std_array");
   if (p->std_kind == MBT_STD_NUMBER && !(p->std > 0.0 && std::isfinite(p->std))) return mbt_set_error(MBT_ERR_INVALID, "std = %g: it has to be positive", p->std);
   if (p->std_kind == MBT_STD_NUMBER && p->grad_std.data != nullptr) return mbt_set_error(MBT_ERR_INVALID, "a std given as a number has no gradient array");
-  if (!std::isfinite(p->entropy_weight)) return mbt_set_error(MBT_ERR_INVALID, "entropy_weight is not finite");
+  if (p->std_kind == MBT_STD_NUMBER && !std::isfinite(1.0f / static_cast<float>(p->std)))
+    return mbt_set_error(MBT_ERR_INVALID, "std = %g: its inverse is not finite in float32", p->std);
+  if (!std::isfinite(static_cast<float>(p->entropy_weight))) return mbt_set_error(MBT_ERR_INVALID, "entropy_weight is not finite");
   PolicyLossParams& P = plan.params;
   P = PolicyLossParams{};
   auto rows = [](const mbt_array2& a) { return Rows{a.data, a.stride[0], a.stride[1]}; };

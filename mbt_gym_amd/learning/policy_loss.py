@@ -48,6 +48,7 @@ class _Plan:
         self.workspace = _native.load_library().mbt_policy_loss_workspace(p)
 
 
+_LARGEST = torch.finfo(torch.float32).max
 _plans = {}
 
 
@@ -147,7 +148,7 @@ def policy_gradient_loss(mean: torch.Tensor, actions: torch.Tensor, weights: tor
 
     mean            (..., A) float32, bfloat16 or float16 - what the network answers with for the recorded observations; A from 1 to 8
     actions         (..., A) float32, as recorded; weights (...) float32, e.g. rewards_to_go.  Both are data: no gradient reaches them
-    std             a positive number; a float32 tensor (A,), one per component; or a tensor like mean, one per row and component
+    std             a positive number (from 3e-39 on); a float32 tensor (A,), one per component; or a tensor like mean, one per row and component
     mask            bool (or uint8) (...): rows that count.  The others count for nothing, NaN and infinities in them too, and get gradients of zero;
                     with no row left the loss is zero
     entropy_weight  of the entropy bonus H(std) = log std + log(2 pi e) / 2, per component
@@ -165,8 +166,8 @@ def policy_gradient_loss(mean: torch.Tensor, actions: torch.Tensor, weights: tor
     if mask is not None:
         require(mask, "mask", device, (torch.bool, torch.uint8), mean.shape[:-1])
     entropy_weight = float(entropy_weight)
-    if not math.isfinite(entropy_weight):
-        raise ValueError(f"entropy_weight = {entropy_weight}: it has to be finite")
+    if not abs(entropy_weight) <= _LARGEST:
+        raise ValueError(f"entropy_weight = {entropy_weight}: it has to be finite, in float32")
     number = 0.0
     if isinstance(std, torch.Tensor):
         require(std, "std", device)
@@ -182,6 +183,8 @@ def policy_gradient_loss(mean: torch.Tensor, actions: torch.Tensor, weights: tor
         number, std = float(std), None
         if not (number > 0.0 and math.isfinite(number)):
             raise ValueError(f"std = {number}: it has to be positive")
+        if not 1.0 / number <= _LARGEST:
+            raise ValueError(f"std = {number}: its inverse has to be finite, in float32")
     if mean.numel() == 0:
         zero = mean.sum(dtype=torch.float32) if std is None else mean.sum(dtype=torch.float32) + 0.0 * std.sum(dtype=torch.float32)
         return zero  # (no rows: a loss of zero that is still connected to its leaves)

@@ -245,3 +245,15 @@ def test_refusals_on_the_device():
     grad, = torch.autograd.grad(loss_of(mean, actions, weights, 0.1), mean, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(grad.sum(), mean)
+
+
+def test_numbers_that_float32_does_not_hold_are_refused():
+    from mbt_gym_amd.learning import policy_gradient_loss
+
+    mean = torch.zeros(4, 2, device="cuda")
+    for std in (1e-39, 1e-50):
+        with pytest.raises(ValueError, match="inverse"):
+            policy_gradient_loss(mean, mean, mean[:, 0], std)
+    with pytest.raises(ValueError, match="entropy_weight"):
+        policy_gradient_loss(mean, mean, mean[:, 0], 0.5, entropy_weight=3.5e38)
+    assert float(policy_gradient_loss(mean, mean, mean[:, 0] + 1.0, 4e-39)) == pytest.approx(np.log(4e-39) + 0.5 * np.log(2 * np.pi), rel=1e-6)

@@ -55,3 +55,18 @@ def test_constants_that_float32_does_not_hold_are_refused(lib):
     r.constant = -3.4028234663852886e38
     assert lib.mbt_recurrence_workspace(C.byref(r), 0) == 0 and lib.mbt_recurrence_forward(-1, C.byref(r), None) < 0
     assert b"float32" not in lib.mbt_last_error()
+
+
+def test_numbers_that_the_loss_cannot_use_in_float32_are_refused(lib):
+    """1 / 1e-39 is an infinity in float32, whose product with a difference of zero is NaN; the next ones up are taken as far as the workspace"""
+    from tests.test_learning_refusals import loss_struct
+
+    def forward(**changes):
+        return lib.mbt_policy_loss_forward(0, C.byref(loss_struct(**changes)), None)
+
+    for std in (1e-39, 2.9e-39, 1e-50, 5e-324):
+        refused(lib, forward(std=std), "not finite in float32")
+    for weight in (3.5e38, -1e300):
+        refused(lib, forward(entropy_weight=weight), "entropy_weight is not finite")
+    for std in (3e-39, 1e-20, 1e39):
+        refused(lib, forward(std=std, entropy_weight=-3.4e38), "are needed")
