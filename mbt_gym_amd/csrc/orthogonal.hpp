@@ -396,12 +396,14 @@ __global__ __launch_bounds__(256) void orthogonalise_split(const OrthogonalisePa
     v[k] = i0 + i < M.m && j0 + j < M.n ? static_cast<float>(in[(i0 + i) * M.in_row + (j0 + j) * M.in_column]) : 0.0f;
   }
   const double* partials = P.partials + (which + matrices_before(P, group)) * kNormBlocks;
-  // (in 64 bits: the inverse of a norm beyond 2^126 is no normal float32 number, that of one below 2^-128 no finite one)
-  const double inverse = inverse_norm(block_sum(threadIdx.x < M.norm_blocks ? partials[threadIdx.x] : 0.0, lds), P.eps);
+  // (the inverse of a norm beyond 2^126 is no normal float32 number, that of one below 2^-128 no finite one: a power of two, which brings an element to at
+  // most two, and what is left of it.  A product in 64 bits per element: 15.7 us instead of 11.6 at 2048 x 2048)
+  int exponent;
+  const float inverse = static_cast<float>(frexp(inverse_norm(block_sum(threadIdx.x < M.norm_blocks ? partials[threadIdx.x] : 0.0, lds), P.eps), &exponent));
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
     const int e = threadIdx.x + 256 * k, i = along_n ? e >> 6 : e & 63, j = along_n ? e & 63 : e >> 6;
-    tile[i][j] = static_cast<float>(v[k] * inverse) * kScaleX;
+    tile[i][j] = ldexpf(v[k], exponent) * inverse * kScaleX;
   }
   __syncthreads();
   const Planes p = planes_of(P, M, which);
