@@ -5,22 +5,22 @@ from torch.autograd import forward_ad
 from mbt_gym_amd import _native
 
 DTYPES = {torch.float32: _native.FLOAT32, torch.bfloat16: _native.BFLOAT16, torch.float16: _native.FLOAT16}
-
-
-_PROXY = torch._C._TorchDispatchModeKey.PROXY
+_PROXY, _dispatch_mode, _tracing_state = torch._C._TorchDispatchModeKey.PROXY, torch._C._get_dispatch_mode, torch._C._get_tracing_state
 
 
 def refuse_recording(what, by_autograd=False):
     """A recorder of torch's own operations sees the empty outputs of a kernel call and not the call, and what it records would answer with whatever lies in
-    memory.  `by_autograd`: the caller goes through an autograd function, which torch.jit.trace records as one operation."""
-    if torch._C._get_dispatch_mode(_PROXY) is not None or (not by_autograd and torch._C._get_tracing_state() is not None):
+    memory.  `by_autograd`: the caller goes through an autograd function when this returns True, which torch.jit.trace records as one operation."""
+    tracing = _tracing_state() is not None
+    if (tracing and not by_autograd) or _dispatch_mode(_PROXY) is not None:
         raise RuntimeError(f"{what} is a kernel call that the tracer that is active cannot record")
+    return tracing
 
 
 def transformed():
     """Is torch at work on something that a kernel call does not take part in: a forward-mode derivative, a functorch transform, a tracer?"""
-    return (forward_ad._current_level >= 0 or torch._C._functorch.maybe_current_level() is not None or torch._C._get_tracing_state() is not None
-            or torch._C._get_dispatch_mode(_PROXY) is not None)
+    return (forward_ad._current_level >= 0 or torch._C._functorch.maybe_current_level() is not None or _tracing_state() is not None
+            or _dispatch_mode(_PROXY) is not None)
 
 
 def require(tensor, name, device=None, dtypes=None, shape=None):

@@ -187,7 +187,7 @@ def linear_recurrence(inputs: torch.Tensor, gate: Union[float, torch.Tensor], in
     steps has no states, and its final state is the initial one.  Gradients are those of the stored inputs and gates: the
     states that they need are recomputed from them, in float32 whatever the states are stored in.  Second and
     forward-mode derivatives are refused."""
-    refuse_recording("linear_recurrence", by_autograd=True)
+    tracing = refuse_recording("linear_recurrence", by_autograd=True)
     require(inputs, "inputs", dtypes=DTYPES)
     if inputs.dim() == 0:
         raise ValueError("inputs is a scalar: it has no time axis")
@@ -218,7 +218,7 @@ def linear_recurrence(inputs: torch.Tensor, gate: Union[float, torch.Tensor], in
         return (states, final) if return_final else states
     tracked = torch.is_grad_enabled() and (inputs.requires_grad or (gate is not None and gate.requires_grad) or (initial is not None and initial.requires_grad))
     settings = (axis, form, constant, 1 if reverse else 0)
-    if tracked or torch._C._get_tracing_state() is not None:
+    if tracked or tracing:
         states, final = _LinearRecurrence.apply(inputs, gate, initial, reset, settings)
     else:
         states, final = _forward(inputs, gate, initial, reset, settings)[:2]
