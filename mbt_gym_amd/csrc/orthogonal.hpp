@@ -238,8 +238,8 @@ __global__ __launch_bounds__(1024) void orthogonalise_small(const OrthogonaliseP
 
 // One step of a flat matrix (m <= 64 < n), `shares` workgroups each, which take its blocks of 64 columns in turn.  Workspace per matrix, in floats:
 // X (64 x np, by blocks of 64 x 64), then the shares of A (64 x 64 each) of this step and the next.  Launch 0 brings X in and leaves the first shares;
-// launch s = 1 .. steps turns X, the last one into the output.  64 x 1000: 60 us for the seven launches, each the latency of its chain of four products
-// and of summing the shares; 64 x 20000: 200 us.
+// launch s = 1 .. steps turns X, the last one into the output.  64 x 1000: 61 us for the seven launches, each the latency of its chain of four products
+// and of summing the shares; 16 x 1000: 49 us; 64 x 20000: 192 us.
 template <typename E>
 __global__ __launch_bounds__(1024) void orthogonalise_flat(const OrthogonaliseParams P, int launch) {
   extern __shared__ float lds_small[];
@@ -376,7 +376,7 @@ __global__ __launch_bounds__(1024) void orthogonalise_norms(const OrthogonaliseP
   if (threadIdx.x == 0) P.partials[(which + matrices_before(P, group)) * kNormBlocks + part] = sum;
 }
 
-// X = G / (|G| + eps) in both orders, 64 x 64 at a time; M.first counts such tiles.  2048 x 2048: 11.1 us for 48 MB (16.8 with stores of single halfs)
+// X = G / (|G| + eps) in both orders, 64 x 64 at a time; M.first counts such tiles.  2048 x 2048: 11.6 us for 48 MB (17 with stores of single halfs)
 template <typename E>
 __global__ __launch_bounds__(256) void orthogonalise_split(const OrthogonaliseParams P) {
   __shared__ double lds[4];
@@ -489,7 +489,7 @@ __device__ __forceinline__ void find_tile(int t, int rows, int columns, int& ti,
 
 // One T x T tile of a product, WAVES waves of T/2 x 2 T/WAVES, k in steps of 32.  Three products of matrix instructions per step of one split
 // operand pair: 128 x 128 with eight waves has 768 cycles of them per SIMD and step, against 650 cycles of LDS (96 KB read, 32 KB written).
-// Measured at 2048 x 2048: 41 us for a symmetric product (136 workgroups on 256 compute units), 50 for the full one, where the matrix instructions
+// Measured at 2048 x 2048: 41 us for a symmetric product (136 workgroups on 256 compute units), 53 for the full one (47 at best), where the matrix instructions
 // alone - the loop without its reads, writes and loads - take 32 and 36; 64 x 64 tiles take 46 and 70 there, but 11 and 13 us instead of 21 and 23
 // at 1024 x 1024, where 128 x 128 ones are too few.  What brought it there from 70 us: a barrier that does not wait for loads from memory (60), the
 // requests strewn between the products (53), LDS without bank conflicts (44).  What bounds it now: LDS writes and the barrier per step.

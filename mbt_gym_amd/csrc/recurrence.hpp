@@ -25,15 +25,25 @@
 //   rows     time is contiguous: lanes lie along time, eight steps each, and a group of 2^n lanes scans by wave shuffles; segments as above
 //
 // Measured, against 5.15 TB/s of a copy of 839 MB and 8.6 of one that stays in the last cache (128 MB):
-//   columns, 200 steps x 65536, logit form      float32   forward 29.5 us (5.3 TB/s)   backward 57 us (4.6 TB/s)
-//                                               bfloat16  forward 29.7 us (2.6 TB/s)   backward 49 us (2.7 TB/s): the sigmoids bound it, not the bytes
-//   columns, 200 x 2^20, constant gate          float32   333 us (5.0 TB/s): a copy's rate
-//   columns, 65536 x 64, logit form             float32   forward 25 us, backward 37 us, two launches each: 2.0 and 2.3 TB/s, bound by latency - the
-//                                               segments' composites are a second walk over x and g that has to end first
-//   rows, 65536 x 200 steps, logit form         float32   forward 36.6 us (4.3 TB/s), backward 84 us (3.1 TB/s): bound by the instructions of the scans and
-//                                               the registers of the backward pass.  (The scan by DPP moves instead of shuffles: slower, it spills.)
-//                value gates                    float32   forward 31.7 us (5.0 TB/s), backward 65 us (4.1 TB/s)
-//   rows, 1665 x 1001, value gates              float32   forward 8.3 us, backward 13.4 us (2.4 and 2.5 TB/s)
+//   columns, 200 steps x 65536                  float32   logit     forward 30.3 us (5.2 TB/s)   backward 56.1 us (4.7 TB/s)
+//                                                         value     forward 29.3 us (5.4 TB/s)   backward 53.0 us (4.9 TB/s)
+//                                                         constant  forward 21.4 us (4.9 TB/s)   backward 21.8 us (4.8 TB/s)
+//                                               bfloat16  logit     forward 33.3 us (2.4 TB/s; 29.5 without edges)   backward 47.0 us (2.8 TB/s)
+//                                                         value     forward 26.5 us (3.0 TB/s; 23.9 without edges)   backward 42.1 us (3.1 TB/s)
+//                                                         constant  forward 22.9 us (2.3 TB/s)   backward 23.1 us (2.3 TB/s)
+//                                               16 bits are bound by vector instructions and by what they do not hide: logit form forward 12.6 M of a wave,
+//                                               20.5 us at four cycles each, and the loads of a tile that are asked for behind the join of the tile before
+//   columns, 200 x 2^20, constant gate          float32   336 us (5.0 TB/s): a copy's rate
+//   columns, 65536 x 64, logit form             float32   forward 10.9 + 14.7 us, backward 13.2 + 24.7 us, two launches each: 2.0 and 2.2 TB/s, bound by
+//                                               latency - the segments' composites are a second walk over x and g that has to end first
+//   rows, 65536 x 200 steps                     float32   logit     forward 35.8 us (4.4 TB/s)   backward 81.0 us (3.2 TB/s)
+//                                                         value     forward 30.9 us (5.1 TB/s)   backward 64.8 us (4.0 TB/s)
+//                                                         constant  forward 28.3 us (3.7 TB/s)   backward 30.7 us (3.4 TB/s)
+//                                               bfloat16  logit     forward 34.2 us (2.3 TB/s)   backward 71.5 us (1.8 TB/s)
+//                                                         value     forward 28.8 us (2.7 TB/s)   backward 54.2 us (2.4 TB/s)
+//                                               bound by the instructions of the scans (logit form: 30 of 36 us forward, 50 of 81 backward) and the registers of
+//                                               the backward pass.  (The scan by DPP moves instead of shuffles: slower, it spills.)
+//   rows, 1665 x 1001, value gates              float32   forward 9.0 us, backward 14.2 us (2.2 and 2.3 TB/s)
 #pragma once
 #include "learning_common.hpp"
 
@@ -717,8 +727,8 @@ __global__ __launch_bounds__(256) void recurrence_rows(const RecurrenceParams P)
 
 // ---- one step ----------------------------------------------------------------------------------------------------------------------
 // new = keep state + inject x: what a recurrent actor does between two environment steps.  n elements, V per thread; the reset mask has
-// strides of its own (a mask per lane, expanded over the lane's channels, costs one byte per lane).  2.3 us at 64000 elements, a launch's own time;
-// 47 us at 2^24 float32 (7.1 TB/s, much of it from the last cache).
+// strides of its own (a mask per lane, expanded over the lane's channels, costs one byte per lane).  2.6 us at 64000 elements, a launch's own time;
+// 58 us at 2^24 float32 (5.8 TB/s), 60 with a mask per lane.
 template <typename E, int FORM, int V>
 __global__ __launch_bounds__(256) void recurrence_step(const float* state, const E* x, const E* g, const uint8_t* reset, int64_t reset_columns, int64_t rs,
                                                        int64_t rc, E* out, float* new_state, int64_t n) {

@@ -12,7 +12,7 @@ class RecurrentPolicy(torch.nn.Module):
     step(observation)      (N, D) -> (N, A) for the next step of the episode; begin_episode() puts the state back to zero, and lanes whose episode
                            starts anew in between are named by `reset`.  A step may be captured into a HIP graph, after one of the same batch that
                            was not: the graph's replays and begin_episode() then work on the state that the capture found
-    `PolicyGradientAgent` trains it as it is.  Parameters and tensors live on the device."""
+    `PolicyGradientAgent` trains it as it is, in float32.  Parameters and tensors live on the device."""
 
     def __init__(self, observation_size: int, action_size: int, hidden_size: int = 64, memory: float = 2.0):
         super().__init__()
