@@ -122,9 +122,10 @@ class _PolicyLoss(torch.autograd.Function):
         stream = current_stream(index)
         capture = lib.mbt_stream_capture_id(stream)
         # The arrays that the forward call filled are handed out once; a graph that is walked again gets new ones.  So does a pass that is captured without the
-        # forward call: its replays come again and again, with other loss gradients and after what the program did to the arrays.
+        # forward call - its replays come again and again, with other loss gradients and after what the program did to the arrays - and one that is not captured
+        # behind a forward call that was, whose replays would write over what it handed out.
         gradients, ctx.gradients = ctx.gradients, None
-        if gradients is not None and capture in (0, ctx.capture):
+        if gradients is not None and capture == ctx.capture:
             grad_mean, grad_std = gradients
             p.gradients_ready = 1
             if grad_mean is not None:

@@ -154,3 +154,29 @@ def test_a_first_step_is_not_captured():
     policy.step(obs)
     policy.begin_episode()
     assert policy.state is None
+
+
+def test_gradients_taken_behind_a_captured_forward_pass_are_the_programs_own():
+    """the next replay of the loss does not write over them"""
+    from mbt_gym_amd import learning
+
+    mean, actions, weights = torch.randn(300, 2, device="cuda", requires_grad=True), torch.randn(300, 2, device="cuda"), torch.randn(300, device="cuda")
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        learning.policy_gradient_loss(mean, actions, weights, 0.5)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            loss = learning.policy_gradient_loss(mean, actions, weights, 0.5)
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    fresh = mean.detach().clone().requires_grad_(True)
+    expected, = torch.autograd.grad(learning.policy_gradient_loss(fresh, actions, weights, 0.5), fresh)
+    for _ in range(2):
+        grad, = torch.autograd.grad(loss, mean, retain_graph=True)
+        assert torch.equal(grad, expected)
+        grad.mul_(0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, 0.5 * expected)
