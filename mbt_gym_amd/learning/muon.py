@@ -83,7 +83,8 @@ class Muon(torch.optim.Optimizer):
 
     A parameter with more than two axes is the matrix (first axis, the rest); a vector - a bias - is a matrix of one column, whose orthogonal factor
     is the vector at length one.  Momentum and update are float32 whatever the parameters are; all parameters of a dtype and device are
-    orthogonalised in one call."""
+    orthogonalised in one call.  A step may be captured into a HIP graph, after one that was not; its replays step with the lr and the rest of the
+    group that the capture found."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5,
                  coefficients: Sequence[float] = COEFFICIENTS, eps: float = 1e-7):
@@ -121,6 +122,8 @@ class Muon(torch.optim.Optimizer):
             if p.is_complex():
                 raise ValueError(f"Muon does not take parameters of {p.dtype}")
             if "momentum" not in self.state[p]:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("a momentum that is made in a graph starts from zero on every replay: take a step before the capture")
                 self.state[p]["momentum"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
         grads, moving = [p.grad.float() for p in params], [self.state[p]["momentum"] for p in params]
         torch._foreach_mul_(moving, group["momentum"])

@@ -180,3 +180,40 @@ def test_gradients_taken_behind_a_captured_forward_pass_are_the_programs_own():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(grad, 0.5 * expected)
+
+
+def test_a_captured_step_of_the_optimiser():
+    """its momentum goes on from replay to replay; a first step, which would make it anew each time, is refused"""
+    from mbt_gym_amd.learning import Muon
+
+    def make():
+        torch.manual_seed(4)
+        p = torch.nn.Parameter(torch.randn(20, 30, device="cuda"))
+        p.grad = torch.randn(20, 30, device="cuda")
+        return p, Muon([p], lr=0.1)
+
+    (p, optimizer), (q, eager) = make(), make()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        torch.zeros(8, device="cuda").add_(1.0)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="take a step before"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+                optimizer.step()
+        torch.cuda.synchronize()
+        optimizer.step()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            optimizer.step()
+    torch.cuda.synchronize()
+    eager.step()
+    for _ in range(3):
+        gradient = torch.randn(20, 30, device="cuda")
+        p.grad.copy_(gradient)
+        q.grad.copy_(gradient)
+        torch.cuda.synchronize()
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert torch.equal(p, q)
