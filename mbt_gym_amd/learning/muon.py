@@ -122,7 +122,7 @@ class Muon(torch.optim.Optimizer):
             if p.is_complex():
                 raise ValueError(f"Muon does not take parameters of {p.dtype}")
             if "momentum" not in self.state[p]:
-                if torch.cuda.is_current_stream_capturing():
+                if p.is_cuda and torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("a momentum that is made in a graph starts from zero on every replay: take a step before the capture")
                 self.state[p]["momentum"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
         grads, moving = [p.grad.float() for p in params], [self.state[p]["momentum"] for p in params]

@@ -31,7 +31,7 @@ class RecurrentPolicy(torch.nn.Module):
         return self.output(torch.tanh(linear_recurrence(x, gate, dim=0, reset=reset, gate_is_logit=True)))
 
     def begin_episode(self):
-        if self.state is not None and torch.cuda.is_current_stream_capturing():
+        if self.state is not None and self.state.is_cuda and torch.cuda.is_current_stream_capturing():
             self._keep()
         for state in self._captured:
             self._clear(state)
@@ -49,7 +49,7 @@ class RecurrentPolicy(torch.nn.Module):
     @torch.no_grad()
     def step(self, observation: torch.Tensor, reset: torch.Tensor = None) -> torch.Tensor:
         x, gate = self.inputs(observation).split(self.hidden_size, dim=-1)
-        capturing = torch.cuda.is_current_stream_capturing()
+        capturing = x.is_cuda and torch.cuda.is_current_stream_capturing()
         if self.state is None or self.state.shape != x.shape or self.state.device != x.device:
             kept = next((state for state in self._captured if state.shape == x.shape and state.device == x.device), None)
             if kept is None and capturing:
