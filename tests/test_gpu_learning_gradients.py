@@ -265,3 +265,21 @@ def test_padded_lanes_of_a_recording_are_neither_read_nor_written(lanes, steps):
         assert not torch.isnan(one).any() and torch.equal(one, other)
     for t, b in zip(recorded + [flags], before):
         assert torch.equal(t if t.dtype is torch.bool else t.view(torch.int32), b)
+
+
+@pytest.mark.parametrize("steps", [9, 27])
+@pytest.mark.parametrize("form", ["value", "logit"])
+def test_gate_gradients_of_very_many_columns(steps, form):
+    """... which the forward pass walks eight to a thread, past the caches from some steps on, while the backward pass takes pairs; some of them against
+    the definition"""
+    lanes = 1 << 21
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    gate = torch.randn(steps, lanes, generator=gen, device="cuda") + 2.0
+    x, gate = levels((steps, lanes), "noise", 1).bfloat16(), (gate if form == "logit" else torch.sigmoid(gate)).bfloat16()
+    h0, up = torch.ones(lanes, device="cuda"), torch.randn(steps, lanes, generator=gen, device="cuda").bfloat16()
+    leaves = [t.requires_grad_(True) for t in (x, gate, h0)]
+    grads = torch.autograd.grad(learning().linear_recurrence(*leaves, gate_is_logit=form == "logit"), leaves, up)
+    pick = torch.cat([torch.arange(20, device="cuda"), torch.randint(0, lanes, (500,), generator=gen, device="cuda"), torch.arange(lanes - 20, lanes, device="cuda")])
+    ref = Float32States(to64(x[:, pick]), to64(gate[:, pick]), form, to64(h0[pick]), dtype="bfloat16")
+    for name, grad in zip(("inputs", "gate", "initial"), grads):
+        assert_within(to64(grad[..., pick]), *ref.gradients(to64(up[:, pick]))[name], (name, steps, form))
